@@ -203,6 +203,50 @@ long long tcb_mx_scales_packed_bytes(int rows, int groups);
  * preparation, not part of the GEMM).  No counterpart in the reference. */
 int tcb_mx_scales_pack(const void *src, void *dst, int rows, int groups, tcb_stream_t stream);
 
+/* ------------------------------------------------- MX FP4 operators */
+/* A quantised matrix [rows][cols] is a pair of buffers, both 16-byte aligned:
+ *   codes  : [rows][ceil(cols/32)*16] bytes, E2M1 packed two per byte along the
+ *            row (low nibble = even column), zeros past cols;
+ *   scales : E8M0 of [rows][ceil(cols/32)], in the packed layout of
+ *            tcb_mx_scales_pack (tcb_mx_scales_packed_bytes bytes).
+ * None of the entry points below has a counterpart in the reference. */
+#define TCB_MX_FLOOR 0 /* scale = 2^(floor(log2 max|v|) - 2): OCP MX, values above 6 saturate */
+#define TCB_MX_UP 1    /* least power of two with max|v| <= 6 x scale: nothing saturates */
+
+/* Quantise X [rows][cols] (TCB_T_BF16, TCB_T_FP16 or TCB_T_FP32; row pitch ld
+ * >= cols elements, any element alignment; 16-byte rows are read fastest) to
+ * (codes, scales) with groups of 32 along the rows, and/or its transpose
+ * [cols][rows] to (codes_t, scales_t) with groups of 32 down the columns, in
+ * one read of X.  Either pair may be NULL, not both.  Every byte of the outputs
+ * is written, padding included.  Rounding is to nearest even; a group of zeros
+ * gets the unit scale, a group that holds an infinity or a NaN gets the NaN
+ * scale 255 and zero codes; scales are at least 2^-127.  rows = 0 or cols = 0
+ * does nothing. */
+int tcb_mx_quantize(int dtype, const void *X, long long rows, long long cols, long long ld, int rule,
+                    void *codes, void *scales, void *codes_t, void *scales_t, tcb_stream_t stream);
+
+/* Y [rows][cols] (TCB_T_BF16, TCB_T_FP16 or TCB_T_FP32, row pitch ld elements) =
+ * the values of (codes, scales), rounded once to nearest even.  Elements of Y
+ * between cols and ld are left as they are. */
+int tcb_mx_dequantize(int dtype, const void *codes, const void *scales, long long rows, long long cols,
+                      void *Y, long long ld, tcb_stream_t stream);
+
+/* C [M][N] = A [M][K] . B [N][K]^T (+ bias [N]), A and B quantised along K,
+ * products and sums in fp32, C and bias in `dtype` (TCB_T_FP32, TCB_T_BF16 or
+ * TCB_T_FP16), row pitch ldc >= N elements, rounded once.  Any M, N and K; M = 0
+ * or N = 0 does nothing.  C elements past N are left as they are.  bias may be
+ * NULL. */
+int tcb_mx_gemm(const void *A, const void *SA, const void *B, const void *SB, const void *bias,
+                int dtype, void *C, long long ldc, int M, int N, int K, int *status_dev,
+                tcb_stream_t stream);
+
+/* Y [M][N] = X [M][K] . W [N][K]^T (+ bias [N]) with X in TCB_T_BF16 or TCB_T_FP16
+ * (row pitch ldx >= K elements) and only W quantised; Y and bias in `dtype` as
+ * above.  Meant for few rows (decoding): W is read once per 64 rows of X. */
+int tcb_mx_linear(int x_dtype, const void *X, long long ldx, const void *W, const void *SW,
+                  const void *bias, int dtype, void *Y, long long ldy, int M, int N, int K,
+                  int *status_dev, tcb_stream_t stream);
+
 /* MX FP4 GEMM that allocates nothing, for callers that cannot allocate device
  * memory (a plugin whose host framework owns all device memory through its
  * own pool, or a path where cudaMalloc/cudaFree and their synchronisation are

@@ -39,6 +39,8 @@ COEFF_IN_REGISTERS = frozenset({V_BF16, V_FP16, V_INT8_DP4A})
 T_BF16, T_FP16, T_TF32, T_FP32, T_FP64, T_INT8, T_FP8E4M3, T_MXF4 = range(8)
 TV_TCGEN05, TV_DMMA, TV_SIMT, TV_SIMT_REG = 0, 1, 2, 3
 
+MX_FLOOR, MX_UP = 0, 1
+
 FAMILY_COPY, FAMILY_READ, FAMILY_VECTOR, FAMILY_TENSOR, FAMILY_GEMM = 0, 1, 2, 3, 4
 
 # Every symbol include/tcb.h declares.
@@ -46,7 +48,8 @@ EXPORTED_SYMBOLS = (
     "tcb_strerror", "tcb_version", "tcb_device_query", "tcb_copy", "tcb_read",
     "tcb_vector_chains", "tcb_vector_chains_imm", "tcb_tensor_peak", "tcb_gemm", "tcb_mx_scales_packed_bytes",
     "tcb_mx_scales_pack", "tcb_kernel_info", "tcb_gemm_mxf4_noalloc",
-    "tcb_selftest_bounded_wait",
+    "tcb_selftest_bounded_wait", "tcb_mx_quantize", "tcb_mx_dequantize", "tcb_mx_gemm",
+    "tcb_mx_linear",
 )
 
 
@@ -144,6 +147,10 @@ def load() -> ctypes.CDLL:
         lib.tcb_mx_scales_pack.argtypes = [vp, vp, i, i, vp]
         lib.tcb_gemm_mxf4_noalloc.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, vp, vp]
         lib.tcb_mx_scales_packed_bytes.argtypes = [i, i]
+        lib.tcb_mx_quantize.argtypes = [i, vp, ll, ll, ll, i, vp, vp, vp, vp, vp]
+        lib.tcb_mx_dequantize.argtypes = [i, vp, vp, ll, ll, vp, ll, vp]
+        lib.tcb_mx_gemm.argtypes = [vp, vp, vp, vp, vp, i, vp, ll, i, i, i, vp, vp]
+        lib.tcb_mx_linear.argtypes = [i, vp, ll, vp, vp, vp, i, vp, ll, i, i, i, vp, vp]
         lib.tcb_selftest_bounded_wait.argtypes = [ll, vp, vp]
         lib.tcb_kernel_info.argtypes = [i, i, i, i, i, i, i, i, ctypes.POINTER(KernelInfo)]
         for name in EXPORTED_SYMBOLS:
@@ -276,6 +283,34 @@ def mx_scales_packed_bytes(rows: int, groups: int) -> int:
 def mx_scales_pack(src, dst, rows: int, groups: int, stream=None) -> None:
     check(load().tcb_mx_scales_pack(_ptr(src), _ptr(dst), rows, groups, _stream(stream)),
           "tcb_mx_scales_pack")
+
+
+def mx_quantize(dtype: int, x, rows: int, cols: int, ld: int, rule: int, codes, scales,
+                codes_t=None, scales_t=None, stream=None) -> None:
+    """Rows (codes, scales) and/or columns (codes_t, scales_t) of x as MX FP4."""
+    check(load().tcb_mx_quantize(dtype, _ptr(x), rows, cols, ld, rule, _ptr(codes), _ptr(scales),
+                                 _ptr(codes_t), _ptr(scales_t), _stream(stream)), "tcb_mx_quantize")
+
+
+def mx_dequantize(dtype: int, codes, scales, rows: int, cols: int, y, ld: int,
+                  stream=None) -> None:
+    check(load().tcb_mx_dequantize(dtype, _ptr(codes), _ptr(scales), rows, cols, _ptr(y), ld,
+                                   _stream(stream)), "tcb_mx_dequantize")
+
+
+def mx_gemm(a, scale_a, b, scale_b, c, m: int, n: int, k: int, *, dtype: int, ldc: int, bias=None,
+            status=None, stream=None) -> None:
+    """C = A . B^T (+ bias) of two MX FP4 matrices, C in `dtype`."""
+    check(load().tcb_mx_gemm(_ptr(a), _ptr(scale_a), _ptr(b), _ptr(scale_b), _ptr(bias), dtype,
+                             _ptr(c), ldc, m, n, k, _ptr(status), _stream(stream)), "tcb_mx_gemm")
+
+
+def mx_linear(x_dtype: int, x, ldx: int, w, scale_w, y, m: int, n: int, k: int, *, dtype: int,
+              ldy: int, bias=None, status=None, stream=None) -> None:
+    """Y = X . W^T (+ bias) with 16-bit X and an MX FP4 weight, Y in `dtype`."""
+    check(load().tcb_mx_linear(x_dtype, _ptr(x), ldx, _ptr(w), _ptr(scale_w), _ptr(bias), dtype,
+                               _ptr(y), ldy, m, n, k, _ptr(status), _stream(stream)),
+          "tcb_mx_linear")
 
 
 def selftest_bounded_wait(limit_ns: int, status, stream=None) -> None:

@@ -36,6 +36,7 @@
 
 #include "tcb_device.cuh"
 #include "tcb_gemm_common.cuh"
+#include "tcb_gemm_pair.h"
 #include "tcb_host.h"
 #include "tcb_registry.h"
 
@@ -46,9 +47,6 @@ using namespace gemm_detail;
 
 }  // namespace
 
-int gemm_pair_run(const void* A, const void* B, const void* SA, const void* SB, void* C, int M,
-                  int N, int K, int blocks, int* status, uint32_t idesc, const DeviceFacts& facts,
-                  cudaStream_t stream);
 int gemm_pair_info(tcb_kernel_info_t* out);
 
 // cuTensorMapEncodeTiled from the driver, resolved once (thread-safe static
@@ -430,6 +428,8 @@ const char* gemm_instruction(int kind) {
 
 }  // namespace
 
+uint32_t gemm_pair_idesc() { return gemm_idesc(gMXF4, 256); }
+
 int gemm_kernel_info(int dtype, int m, int n, tcb_kernel_info_t* out) {
   if (dtype == TCB_T_FP32 || dtype == TCB_T_FP64) return gemm_cuda_core_info(dtype, out);
   const int kind = gemm_kind(dtype);
@@ -542,8 +542,8 @@ extern "C" int tcb_gemm(int dtype, const void* A, const void* B, const void* SA,
   const long long kbytes = kbits / 8;
   if (kind == gMXF4 && M > 128) {
     // CTA pairs: 256 x 256 tiles, each CTA loading 128 rows of A and of B.
-    return gemm_pair_run(A, B, SA, SB, C, M, N, K, blocks, status_dev, gemm_idesc(kind, 256),
-                         facts, reinterpret_cast<cudaStream_t>(stream));
+    const PairProblem p{A, B, SA, SB, nullptr, C, N, M, N, K, kPairFp32, gemm_pair_idesc()};
+    return gemm_pair_run(p, blocks, status_dev, facts, reinterpret_cast<cudaStream_t>(stream));
   }
   const int halves = gemm_halves(kind, M, N, facts.sm_count);
   const int tile_m = 128 * halves;

@@ -70,7 +70,9 @@
 
 #include "tcb_device.cuh"
 #include "tcb_gemm_common.cuh"
+#include "tcb_gemm_pair.h"
 #include "tcb_host.h"
+#include "tcb_mx.cuh"
 #include "tcb_registry.h"
 
 namespace tcb {
@@ -117,7 +119,9 @@ static_assert(kPairEpiWarps * 2 * kEpiChunkBytes <= kPairStages * kPairStageByte
 struct PairArgs {
   const uint8_t* sa;  // packed E8M0 scales of A (tcb_mx_scales_pack layout)
   const uint8_t* sb;  // packed E8M0 scales of B
-  uint32_t* c;        // [M][N] fp32
+  void* c;            // [M][N], row pitch ldc elements
+  const void* bias;   // [N] of C's type (BIAS kernels)
+  long long ldc;
   int* status;
   int m, n;
   int tiles_m, tiles_n;
@@ -166,6 +170,55 @@ struct PairCursor {
   }
 };
 
+// The type of C: the accumulator itself, or one rounding to 16 bits (after the
+// bias, which is added in fp32).
+template <int OUT>
+struct PairOut;
+template <>
+struct PairOut<kPairFp32> { using type = float; };
+template <>
+struct PairOut<kPairBf16> { using type = __nv_bfloat16; };
+template <>
+struct PairOut<kPairFp16> { using type = __half; };
+
+// acc += bias over this warp's 64 columns from `col0` (all lanes hold the same
+// columns, so every load is a broadcast).
+template <typename T>
+__device__ __forceinline__ void add_bias(uint32_t (&r)[2][32], const T* __restrict__ bias, int col0,
+                                         int n) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (col0 + 32 * q + e < n)
+        r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) +
+                                  mx_detail::to_float(bias[col0 + 32 * q + e]));
+}
+
+// 64 fp32 columns as 32 words of two 16-bit values.
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint32_t (&r)[2][32], uint32_t (&h)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    h[i] = mx_detail::pack2<T>(__uint_as_float(r[i >> 4][2 * (i & 15)]),
+                               __uint_as_float(r[i >> 4][2 * (i & 15) + 1]));
+}
+
+// Direct store of 64 16-bit columns: acc_store's counterpart.
+__device__ __forceinline__ void acc_store16(uint16_t* dst, const uint32_t (&h)[32], int col0, int n,
+                                            bool vec) {
+  if (vec && col0 + 64 <= n) {
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+      st_stream_u4(dst + 8 * v, h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 64; ++e)
+      if (col0 + e < n) dst[e] = static_cast<uint16_t>(h[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+template <int OUT, bool BIAS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_pair_mxf4_kernel(const __grid_constant__ CUtensorMap map_a,
                           const __grid_constant__ CUtensorMap map_b,
@@ -367,10 +420,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
+      using Out = typename PairOut<OUT>::type;
+      // A 16-bit slice is one 4 KB staging chunk (64 columns), an fp32 slice two.
+      constexpr int kChunks = OUT == kPairFp32 ? 2 : 1;
       int tm, tn;
       tile_coords(pair + ti * pairs, args.tiles_m, args.tiles_n, &tm, &tn);
       const int row0 = tm * 2 * kPairRows + static_cast<int>(rank) * kPairRows + 32 * quarter;
       const int c = tn * kTileN + col0;
+      if constexpr (BIAS) add_bias(r, static_cast<const Out*>(args.bias), c, args.n);
+      auto stage_slice = [&](uint8_t* buf, int q) {
+        if constexpr (OUT == kPairFp32) {
+          stage_chunk(buf, lane, r[q]);
+        } else {
+          uint32_t h[32];
+          to_pairs<Out>(r, h);
+          stage_chunk(buf, lane, h);
+        }
+      };
       if (args.tma_store && ti + 1 == my_tiles) {
         // Last tile: every MMA has finished reading the operand ring (acc_full
         // follows their completion) and no load refills it, so each warp
@@ -379,12 +445,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         // per pair the turns were the critical path).
         uint8_t* own = smem + (warp - 2) * 2 * kEpiChunkBytes;
 #pragma unroll
-        for (int q = 0; q < 2; ++q) stage_chunk(own + q * kEpiChunkBytes, lane, r[q]);
+        for (int q = 0; q < kChunks; ++q) stage_slice(own + q * kEpiChunkBytes, q);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < kChunks; ++q)
             tma_store_2d(&map_c, c + 32 * q, row0, own + q * kEpiChunkBytes);
           bulk_commit_group();
         }
@@ -394,8 +460,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (!__all_sync(0xffffffffu, turn_wait(mine))) break;
         __threadfence_block();
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          stage_chunk(staging, lane, r[q]);
+        for (int q = 0; q < kChunks; ++q) {
+          stage_slice(staging, q);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -407,8 +473,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         if (lane == 0) store_turn[group] = mine + 1;
       } else if (row0 + lane < args.m) {
-        acc_store<2>(args.c + static_cast<size_t>(row0 + lane) * args.n + c, r, c, args.n,
-                     args.vec_store);
+        Out* dst = static_cast<Out*>(args.c) + static_cast<long long>(row0 + lane) * args.ldc + c;
+        if constexpr (OUT == kPairFp32) {
+          acc_store<2>(reinterpret_cast<uint32_t*>(dst), r, c, args.n, args.vec_store);
+        } else {
+          uint32_t h[32];
+          to_pairs<Out>(r, h);
+          acc_store16(reinterpret_cast<uint16_t*>(dst), h, c, args.n, args.vec_store);
+        }
       }
     }
     if (lane == 0) bulk_wait_group_all();  // C stores complete before the CTA retires
@@ -524,58 +596,75 @@ int pair_maps(CUtensorMap* map2, CUtensorMap* map3, const void* base, long long 
   return TCB_OK;
 }
 
-// C [rows][cols] fp32 as 32 x 32 boxes in the SWIZZLE_128B layout the
-// epilogue stages (16-byte row pitch and base required).
-int pair_map_c(CUtensorMap* map, void* base, int rows, int cols) {
+// C [rows][cols] as boxes of 32 rows x 128 bytes in the SWIZZLE_128B layout
+// the epilogue stages (16-byte row pitch and base required).
+int pair_map_c(CUtensorMap* map, void* base, int rows, int cols, long long ldc, int elem_bytes) {
   auto fn = tensor_map_encoder();
   if (fn == nullptr) return TCB_ERR_DEVICE;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 4};
-  cuuint32_t box[2] = {32, 32};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ldc) * elem_bytes};
+  cuuint32_t box[2] = {128u / elem_bytes, 32};
   cuuint32_t estr[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, base, dims, strides, box, estr,
+  return fn(map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? TCB_OK
              : TCB_ERR_INVALID_ARGUMENT;
 }
 
+using PairFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PairArgs);
+
+PairFn pair_fn(int out, bool bias) {
+  switch (out) {
+    case kPairBf16: return bias ? gemm_pair_mxf4_kernel<kPairBf16, true> : gemm_pair_mxf4_kernel<kPairBf16, false>;
+    case kPairFp16: return bias ? gemm_pair_mxf4_kernel<kPairFp16, true> : gemm_pair_mxf4_kernel<kPairFp16, false>;
+  }
+  return bias ? gemm_pair_mxf4_kernel<kPairFp32, true> : gemm_pair_mxf4_kernel<kPairFp32, false>;
+}
+
 }  // namespace
 
-// MX FP4 GEMM on CTA pairs for M > 128: tensor maps, arguments and launch of
-// `blocks / 2` persistent pairs (all the pairs that fit at once by default).
-int gemm_pair_run(const void* A, const void* B, const void* SA, const void* SB, void* C, int M,
-                  int N, int K, int blocks, int* status, uint32_t idesc, const DeviceFacts& facts,
+// MX FP4 GEMM on CTA pairs: tensor maps, arguments and launch of `blocks / 2`
+// persistent pairs (all the pairs that fit at once by default).
+int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFacts& facts,
                   cudaStream_t stream) {
-  const long long kbytes = static_cast<long long>(K) / 2;
+  const long long kbytes = static_cast<long long>(p.k) / 2;
+  const int elem_bytes = p.out == kPairFp32 ? 4 : 2;
   PairArgs args;
-  args.sa = static_cast<const uint8_t*>(SA);
-  args.sb = static_cast<const uint8_t*>(SB);
-  args.c = static_cast<uint32_t*>(C);
+  args.sa = static_cast<const uint8_t*>(p.sa);
+  args.sb = static_cast<const uint8_t*>(p.sb);
+  args.c = p.c;
+  args.bias = p.bias;
+  args.ldc = p.ldc;
   args.status = status;
-  args.m = M;
-  args.n = N;
-  args.tiles_m = (M + 2 * kPairRows - 1) / (2 * kPairRows);
-  args.tiles_n = (N + kTileN - 1) / kTileN;
+  args.m = p.m;
+  args.n = p.n;
+  const long long tiles_m = (static_cast<long long>(p.m) + 2 * kPairRows - 1) / (2 * kPairRows);
+  const long long tiles_n = (static_cast<long long>(p.n) + kTileN - 1) / kTileN;
+  if (tiles_m * tiles_n > INT_MAX / 2) return TCB_ERR_RESOURCE;
+  args.tiles_m = static_cast<int>(tiles_m);
+  args.tiles_n = static_cast<int>(tiles_n);
   args.kblocks = static_cast<int>((kbytes + kBlockBytes - 1) / kBlockBytes);
-  args.vec_store = N % 4 == 0 && aligned(C, 16);
-  args.idesc = idesc;
+  args.vec_store = p.ldc * elem_bytes % 16 == 0 && aligned(p.c, 16);
+  args.idesc = p.idesc;
   CUtensorMap map_a, map_b, map_a3, map_b3;
   int panels_a = static_cast<int>(kbytes / kBlockBytes), panels_b = panels_a;
   int rc;
-  if ((rc = pair_maps(&map_a, &map_a3, A, M, kbytes, &panels_a)) != TCB_OK) return rc;
-  if ((rc = pair_maps(&map_b, &map_b3, B, N, kbytes, &panels_b)) != TCB_OK) return rc;
+  if ((rc = pair_maps(&map_a, &map_a3, p.a, p.m, kbytes, &panels_a)) != TCB_OK) return rc;
+  if ((rc = pair_maps(&map_b, &map_b3, p.b, p.n, kbytes, &panels_b)) != TCB_OK) return rc;
   args.full_panels = panels_a < panels_b ? panels_a : panels_b;
   CUtensorMap map_c{};
-  args.tma_store = args.vec_store && pair_map_c(&map_c, C, M, N) == TCB_OK;
-  static DeviceIntCache cap_cache, resident_cache;
-  const int cap = cap_cache.get(facts.device, [&] {
-    return raise_dynamic_smem(reinterpret_cast<const void*>(gemm_pair_mxf4_kernel),
-                              facts.max_smem_optin);
+  args.tma_store =
+      args.vec_store && pair_map_c(&map_c, p.c, p.m, p.n, p.ldc, elem_bytes) == TCB_OK;
+  const PairFn fn = pair_fn(p.out, p.bias != nullptr);
+  static DeviceIntCache cap_cache[3][2], resident_cache;
+  const int cap = cap_cache[p.out][p.bias != nullptr].get(facts.device, [&] {
+    return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
   if (cap < kPairSmem) return TCB_ERR_RESOURCE;
-  // Pairs that can be resident at once: persistent pairs beyond that would
-  // only start when others finish, serialising their tiles.
+  // Pairs that can be resident at once (one CTA per SM whatever C's type):
+  // persistent pairs beyond that would only start when others finish,
+  // serialising their tiles.
   const int resident = resident_cache.get(facts.device, [&] {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * (facts.sm_count / 2), 1, 1);
@@ -589,8 +678,7 @@ int gemm_pair_run(const void* A, const void* B, const void* SA, const void* SB, 
     config.attrs = attr;
     config.numAttrs = 1;
     int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, gemm_pair_mxf4_kernel, &config) != cudaSuccess ||
-        clusters < 1) {
+    if (cudaOccupancyMaxActiveClusters(&clusters, fn, &config) != cudaSuccess || clusters < 1) {
       clear_stale_error();
       clusters = facts.sm_count / 2;
     }
@@ -602,14 +690,13 @@ int gemm_pair_run(const void* A, const void* B, const void* SA, const void* SB, 
   if (pairs > tiles) pairs = tiles;
   if (pairs > resident) pairs = resident;
   clear_stale_error();
-  gemm_pair_mxf4_kernel<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(map_a, map_b, map_a3,
-                                                                          map_b3, map_c, args);
+  fn<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(map_a, map_b, map_a3, map_b3, map_c, args);
   return launch_status();
 }
 
 int gemm_pair_info(tcb_kernel_info_t* out) {
   cudaFuncAttributes attr;
-  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(gemm_pair_mxf4_kernel)) !=
+  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(pair_fn(kPairFp32, false))) !=
       cudaSuccess)
     return TCB_ERR_DEVICE;
   fill_kernel_info(attr, out);

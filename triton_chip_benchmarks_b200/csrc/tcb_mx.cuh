@@ -1,0 +1,107 @@
+// Pieces shared by the MX FP4 kernels: E2M1 conversion, E8M0 scales, 16-bit
+// pairs and the sizes of the packed layout.
+#pragma once
+
+#include <cstdint>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace tcb {
+namespace mx_detail {
+
+// Values of a row of codes: whole groups of 32.
+__host__ __device__ inline long long mx_padded(long long n) { return (n + 31) / 32 * 32; }
+// 128-wide tiles of an axis whose packed scales are padded to 256 values.
+__host__ __device__ inline long long mx_tiles(long long n) { return (n + 255) / 256 * 2; }
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Rounds to nearest even.
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (sizeof(T) == 4) {
+    return v;
+  } else if constexpr (std::is_same_v<T, __half>) {
+    return __float2half_rn(v);
+  } else {
+    return __float2bfloat16_rn(v);
+  }
+}
+
+// The two 16-bit values of a word (low half first) as fp32, exactly.
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x, hi = f.y;
+  } else {
+    lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+  }
+}
+
+// Two fp32 values rounded to nearest even into one word (low half first).
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t w;
+  if constexpr (std::is_same_v<T, __half>) {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+  }
+  return w;
+}
+
+// E8M0 code of a group whose largest |v| has the fp32 bits `top`: the biased
+// exponent less 2 (E2M1's largest exponent), one more where rounding up needs
+// it (mantissa above 1.5 = 6 / 4), at least 0; 127 for a group of zeros and 255
+// (NaN) where a value is infinite or not a number.
+__device__ __forceinline__ uint32_t scale_code(uint32_t top, int up) {
+  int e = static_cast<int>(top >> 23) - 2;
+  if (up && (top & 0x7FFFFFu) > 0x400000u) ++e;
+  e = max(e, 0);
+  if (top == 0) e = 127;
+  if (top >= 0x7F800000u) e = 255;
+  return static_cast<uint32_t>(e);
+}
+
+// 2^(127 - code) for a code of scale_code (at most 253, or 255: any number).
+__device__ __forceinline__ float inverse_scale(uint32_t e8) {
+  return __uint_as_float((254u - min(e8, 253u)) << 23);
+}
+
+// 2^(code - 127); code 0 is the subnormal 2^-127, code 255 is NaN.
+__device__ __forceinline__ float scale_value(uint32_t e8) {
+  return __uint_as_float(e8 == 0 ? 0x00400000u : e8 == 255 ? 0x7FC00000u : e8 << 23);
+}
+
+// Eight values times `inv` as E2M1 codes, the first in the low nibble; zeros
+// where the group's scale is NaN.
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8], float inv, uint32_t e8) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(w)
+      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv),
+        "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+  return e8 == 255 ? 0u : w;
+}
+
+// Eight E2M1 codes as four fp16 pairs (exact).
+__device__ __forceinline__ void decode8(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
+}  // namespace mx_detail
+}  // namespace tcb

@@ -1,0 +1,26 @@
+// The few-row MX FP4 product behind tcb_mx_gemm and tcb_mx_linear.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "tcb_host.h"
+
+namespace tcb {
+
+enum RowsType : int { kRowsFp32 = 0, kRowsBf16 = 1, kRowsFp16 = 2, kRowsMx = 3 };
+
+struct RowsProblem {
+  const void* x;     // [m] rows of x_type, pitch ldx elements (MX: codes, whole groups)
+  const void* sx;    // packed scales of x (MX)
+  const void* w;     // [n] rows of E2M1 codes, whole groups
+  const void* sw;    // packed scales of w
+  const void* bias;  // [n] of y_type, or null
+  void* y;           // [m][n], pitch ldy elements
+  long long ldx, ldy;
+  int m, n, k;
+  int x_type, y_type;
+};
+
+int mx_rows_run(const RowsProblem& p, int* status, const DeviceFacts& facts, cudaStream_t stream);
+
+}  // namespace tcb
