@@ -122,6 +122,8 @@ def library_path() -> Path:
 def load() -> ctypes.CDLL:
     """Load libtcb.so once (raises NativeLibraryError when unavailable)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

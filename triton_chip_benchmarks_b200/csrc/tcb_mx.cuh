@@ -94,6 +94,14 @@ __device__ __forceinline__ uint32_t encode8(const float (&v)[8], float inv, uint
   return e8 == 255 ? 0u : w;
 }
 
+// One E2M1 code (0..15) as fp32: |code| 0 and 1 are 0 and 1/2, the others
+// (2 + c % 2) * 2^(c / 2 - 2).
+__device__ __forceinline__ float decode1(uint32_t code) {
+  const uint32_t c = code & 7u;
+  const uint32_t bits = c < 2 ? c * 0x3F000000u : (c << 22) + (126u << 23);
+  return __uint_as_float(bits | (code & 8u) << 28);
+}
+
 // Eight E2M1 codes as four fp16 pairs (exact).
 __device__ __forceinline__ void decode8(uint32_t w, uint32_t (&h)[4]) {
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\t"

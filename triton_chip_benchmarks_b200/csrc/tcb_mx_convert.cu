@@ -13,13 +13,19 @@
 // 128 rows x 4 groups, which is exactly one 512-byte half of the packed scale
 // layout that the GEMM reads, so the scales leave as one contiguous piece for
 // the row-wise and for the column-wise tensor, padding included (values past
-// the edge count as zero, and an all-zero group has the unit scale 127).  All
-// eight 16-byte loads of a thread are issued before the first is used.
+// the edge count as zero, and an all-zero group has the unit scale 127).  A
+// thread takes 16 values (half a group) of four rows; inside the matrix its
+// loads are straight-line code, all issued before the first is used (with a
+// bounds test around each they went out one by one: 74 us instead of TODO for
+// 8192 x 8192 bf16).  16-bit values stay packed for the search of the largest:
+// two a word, integer maxima of the magnitude bits.
 //
 // Both axes in one read.  The tile is kept in shared memory on its way through
-// the row pass; a thread then takes two neighbouring columns of one 32-row
-// group (a warp reads 32 consecutive words per row: no bank conflicts) and the
-// codes are turned round through shared memory into 64-byte runs.
+// the row pass, 16-byte chunks swizzled so that neither the row-wise stores
+// nor the column-wise loads conflict; a thread then takes 32 rows of one word
+// (two 16-bit columns, or one fp32) and the codes are turned round through
+// shared memory into 64-byte runs.  Rows that do not start on 16-byte
+// boundaries come through the same tile, element by element.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -34,7 +40,7 @@ using namespace mx_detail;
 
 constexpr int kTile = 128;       // rows and columns of a CTA's tile
 constexpr int kThreads = 256;
-constexpr int kVec = 8;          // consecutive values of one thread in one row
+constexpr int kVec = 16;         // consecutive values of one thread in one row
 constexpr int kLanesPerRow = kTile / kVec;
 constexpr int kRowsPerPass = kThreads / kLanesPerRow;
 constexpr int kPasses = kTile / kRowsPerPass;
@@ -52,32 +58,66 @@ struct QuantArgs {
   int up;
 };
 
-// Eight values of one row as fp32 bit patterns; zero past the matrix.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int valid, float (&v)[kVec]) {
-  if (VEC && valid >= kVec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// The values' words: 8 of two 16-bit values, or 16 of one fp32 value.
+template <typename T>
+constexpr int kWords = kVec * static_cast<int>(sizeof(T)) / 4;
+
+// 16 bytes of a row, zero past its end; `valid` values are in the matrix.
+template <typename T>
+__device__ __forceinline__ uint4 load_edge(const T* __restrict__ p, int valid) {
+  constexpr int kPer = 16 / sizeof(T);
+  if (valid >= kPer) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
-    }
+  for (int i = 0; i < kPer; ++i) {
+    if (i >= valid) continue;
+    if constexpr (sizeof(T) == 4)
+      w[i] = __float_as_uint(p[i]);
+    else
+      w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Byte offset of 16-byte chunk c of a row of the tile in shared memory: the
+// eight lanes of a row write chunks 2l + j (fp32: 4l + j), which the swizzle
+// spreads over all banks.
+template <typename T>
+__device__ __forceinline__ int tile_chunk(int row, int c) {
+  constexpr int kMask = sizeof(T) == 4 ? 3 : 1;
+  return row * kTile * static_cast<int>(sizeof(T)) + ((c ^ ((c >> 3) & kMask)) << 4);
+}
+
+// Running maximum of a word's magnitudes: both halves of a 16-bit pair, or one
+// fp32 pattern.
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(uint32_t top, uint32_t w) {
+  if constexpr (sizeof(T) == 4)
+    return max(top, w & 0x7FFFFFFFu);
+  else
+    return __vmaxu2(top, w & 0x7FFF7FFFu);
+}
+
+// fp32 bits of a magnitude given by T's bits.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint32_t magnitude) {
+  if constexpr (sizeof(T) == 4) {
+    return magnitude;
+  } else if constexpr (std::is_same_v<T, __half>) {
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(magnitude))));
   } else {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = i < valid ? to_float(p[i]) : 0.0f;
+    return magnitude << 16;
   }
 }
 
 template <typename T, bool VEC, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constant__ QuantArgs args) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
+    quantize_kernel(const __grid_constant__ QuantArgs args) {
+  constexpr bool kTiled = COLS || !VEC;
+  constexpr int kChunks = kWords<T> / 4;  // 16-byte chunks of a thread's values
   extern __shared__ __align__(16) uint8_t smem[];
-  // [tile as fp32 or T][row scales][column scales][column codes]
-  T* tile = reinterpret_cast<T*>(smem);
-  uint8_t* s_scales = smem + (COLS ? kTile * kTile * sizeof(T) : 0);
+  // [tile][row scales][column scales][column codes]
+  uint8_t* s_scales = smem + (kTiled ? kTile * kTile * sizeof(T) : 0);
   uint8_t* s_scales_t = s_scales + (ROWS ? kHalfBytes : 0);
   uint8_t* s_codes_t = s_scales_t + kHalfBytes;
 
@@ -85,47 +125,98 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constan
   const long long tx = static_cast<long long>(blockIdx.x) % args.tiles_x;
   const long long ty = static_cast<long long>(blockIdx.x) / args.tiles_x;
   const long long r0 = ty * kTile, c0 = tx * kTile;
-  const int col = (tid % kLanesPerRow) * kVec;
+  const int lane_col = tid % kLanesPerRow;
+  const int col = lane_col * kVec;
   const int row = tid / kLanesPerRow;
-  const long long left = args.cols - c0 - col;
-  const int valid = left <= 0 ? 0 : left >= kVec ? kVec : static_cast<int>(left);
+  const T* x = static_cast<const T*>(args.x);
 
-  float v[kPasses][kVec];
+  uint4 raw[kPasses][kChunks];
+  if constexpr (VEC) {
+    if (r0 + kTile <= args.rows && c0 + kTile <= args.cols) {
+      const T* p = x + (r0 + row) * args.ld + c0 + col;
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const long long r = r0 + row + p * kRowsPerPass;
-    load8<T, VEC>(static_cast<const T*>(args.x) + (r < args.rows ? r * args.ld + c0 + col : 0),
-                  r < args.rows ? valid : 0, v[p]);
-  }
-  const long long pitch = mx_padded(args.cols) / 2;
+      for (int i = 0; i < kPasses; ++i)
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int lr = row + p * kRowsPerPass;
-    if constexpr (COLS) {
-      // The values are T's, so converting back is exact.
-      T* dst = tile + lr * kTile + col;
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[p][0], v[p][1], v[p][2], v[p][3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[p][4], v[p][5], v[p][6], v[p][7]);
-      } else {
-        uint32_t w[4];
+        for (int q = 0; q < kChunks; ++q)
+          raw[i][q] = __ldg(reinterpret_cast<const uint4*>(p + i * kRowsPerPass * args.ld) + q);
+    } else {
+      const long long left = args.cols - c0 - col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2<T>(v[p][2 * i], v[p][2 * i + 1]);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int i = 0; i < kPasses; ++i) {
+        const long long r = r0 + row + i * kRowsPerPass;
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q) {
+          constexpr int kPer = 16 / sizeof(T);
+          const int valid = r < args.rows ? static_cast<int>(min(max(left - q * kPer, 0ll), 16ll)) : 0;
+          raw[i][q] = valid ? load_edge(x + r * args.ld + c0 + col + q * kPer, valid)
+                            : make_uint4(0, 0, 0, 0);
+        }
       }
     }
+    if constexpr (COLS) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q)
+          *reinterpret_cast<uint4*>(smem + tile_chunk<T>(row + i * kRowsPerPass,
+                                                         lane_col * kChunks + q)) = raw[i][q];
+    }
+  } else {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll 8
+    for (int i = tid; i < kTile * kTile; i += kThreads) {
+      const int r = i / kTile, c = i % kTile;
+      const bool in = r0 + r < args.rows && c0 + c < args.cols;
+      T v = from_float<T>(0.0f);
+      if (in) v = x[(r0 + r) * args.ld + c0 + c];
+      *reinterpret_cast<T*>(smem + tile_chunk<T>(r, c / kPer) + c % kPer * sizeof(T)) = v;
+    }
+    __syncthreads();
     if constexpr (ROWS) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i)
+#pragma unroll
+        for (int q = 0; q < kChunks; ++q)
+          raw[i][q] = *reinterpret_cast<const uint4*>(
+              smem + tile_chunk<T>(row + i * kRowsPerPass, lane_col * kChunks + q));
+    }
+  }
+  if constexpr (ROWS) {
+    const long long pitch = mx_padded(args.cols) / 2;
+    const bool in_cols = c0 + col < 2 * pitch;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int lr = row + i * kRowsPerPass;
+      uint32_t w[kWords<T>];
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) top = max(top, __float_as_uint(v[p][i]) & 0x7FFFFFFFu);
-      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-      top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-      const uint32_t e8 = scale_code(top, args.up);
-      const uint32_t codes = encode8(v[p], inverse_scale(e8), e8);
-      const long long r = r0 + lr;
-      if (r < args.rows && c0 + col < 2 * pitch)
-        *reinterpret_cast<uint32_t*>(args.codes + r * pitch + (c0 + col) / 2) = codes;
-      if ((tid & 3) == 0)
+      for (int q = 0; q < kChunks; ++q) {
+        w[4 * q] = raw[i][q].x, w[4 * q + 1] = raw[i][q].y;
+        w[4 * q + 2] = raw[i][q].z, w[4 * q + 3] = raw[i][q].w;
+      }
+#pragma unroll
+      for (int q = 0; q < kWords<T>; ++q) top = top_of<T>(top, w[q]);
+      top = top_of<T>(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+      if constexpr (sizeof(T) == 2) top = max(top & 0xFFFFu, top >> 16);
+      const uint32_t e8 = scale_code(top_bits<T>(top), args.up);
+      const float inv = inverse_scale(e8);
+      uint32_t codes[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if constexpr (sizeof(T) == 4)
+            v[k] = __uint_as_float(w[8 * h + k]);
+          else if (k % 2 == 0)
+            unpack2<T>(w[4 * h + k / 2], v[k], v[k + 1]);
+        }
+        codes[h] = encode8(v, inv, e8);
+      }
+      if (in_cols && r0 + lr < args.rows)
+        *reinterpret_cast<uint2*>(args.codes + (r0 + lr) * pitch + (c0 + col) / 2) =
+            make_uint2(codes[0], codes[1]);
+      if ((tid & 1) == 0)
         s_scales[(lr & 31) * 16 + (lr >> 5) * 4 + (col >> 5)] = static_cast<uint8_t>(e8);
     }
   }
@@ -138,37 +229,46 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constan
     }
   }
   if constexpr (COLS) {
-    const int pair = tid & 63, group = tid >> 6;  // columns 2 pair, 2 pair + 1; rows 32 group..
-    float a[32], b[32];
-    uint32_t ta = 0, tb = 0;
+    constexpr int kColsPerWord = 4 / sizeof(T);
+    constexpr int kLanes = kTile / kColsPerWord;  // threads across the tile's columns
+#pragma unroll 1
+    for (int task = tid; task < 4 * kLanes; task += kThreads) {
+      const int word = task % kLanes, group = task / kLanes;
+      const uint8_t* src = smem + tile_chunk<T>(group * 32, word / 4) + word % 4 * 4;
+      uint32_t w[32];
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const T* src = tile + (group * 32 + i) * kTile + 2 * pair;
-      if constexpr (sizeof(T) == 4) {
-        const float2 f = *reinterpret_cast<const float2*>(src);
-        a[i] = f.x, b[i] = f.y;
-      } else {
-        unpack2<T>(*reinterpret_cast<const uint32_t*>(src), a[i], b[i]);
+      for (int i = 0; i < 32; ++i) {
+        w[i] = *reinterpret_cast<const uint32_t*>(src + i * kTile * sizeof(T));
+        top = top_of<T>(top, w[i]);
       }
-      ta = max(ta, __float_as_uint(a[i]) & 0x7FFFFFFFu);
-      tb = max(tb, __float_as_uint(b[i]) & 0x7FFFFFFFu);
-    }
-    const uint32_t ea = scale_code(ta, args.up), eb = scale_code(tb, args.up);
-    uint32_t ca[4], cb[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float f[kVec], g[kVec];
+      for (int k = 0; k < kColsPerWord; ++k) {
+        const uint32_t magnitude = sizeof(T) == 4 ? top : (top >> (16 * k)) & 0xFFFFu;
+        const uint32_t e8 = scale_code(top_bits<T>(magnitude), args.up);
+        const float inv = inverse_scale(e8);
+        uint32_t codes[4];
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) f[i] = a[8 * q + i], g[i] = b[8 * q + i];
-      ca[q] = encode8(f, inverse_scale(ea), ea);
-      cb[q] = encode8(g, inverse_scale(eb), eb);
+        for (int q = 0; q < 4; ++q) {
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) {
+              v[i] = __uint_as_float(w[8 * q + i]);
+            } else {
+              float lo, hi;
+              unpack2<T>(w[8 * q + i], lo, hi);
+              v[i] = k ? hi : lo;
+            }
+          }
+          codes[q] = encode8(v, inv, e8);
+        }
+        const int c = word * kColsPerWord + k;
+        *reinterpret_cast<uint4*>(s_codes_t + c * kCodesPitch + group * 16) =
+            make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        s_scales_t[(c & 31) * 16 + (c >> 5) * 4 + group] = static_cast<uint8_t>(e8);
+      }
     }
-    uint8_t* dst = s_codes_t + 2 * pair * kCodesPitch + group * 16;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(ca[0], ca[1], ca[2], ca[3]);
-    *reinterpret_cast<uint4*>(dst + kCodesPitch) = make_uint4(cb[0], cb[1], cb[2], cb[3]);
-    const int ca0 = 2 * pair, cb0 = ca0 + 1;
-    s_scales_t[(ca0 & 31) * 16 + (ca0 >> 5) * 4 + group] = static_cast<uint8_t>(ea);
-    s_scales_t[(cb0 & 31) * 16 + (cb0 >> 5) * 4 + group] = static_cast<uint8_t>(eb);
     __syncthreads();
     const long long pitch_t = mx_padded(args.rows) / 2;
     const long long tiles_y = mx_tiles(args.rows);
@@ -190,8 +290,8 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constan
 template <typename T, bool VEC, bool ROWS, bool COLS>
 int launch_quantize(const QuantArgs& args, long long tiles, const DeviceFacts& facts,
                     cudaStream_t stream) {
-  const int smem = (COLS ? kTile * kTile * static_cast<int>(sizeof(T)) : 0) + (ROWS ? kHalfBytes : 0) +
-                   (COLS ? kHalfBytes + kTile * kCodesPitch : 0);
+  const int smem = (COLS || !VEC ? kTile * kTile * static_cast<int>(sizeof(T)) : 0) +
+                   (ROWS ? kHalfBytes : 0) + (COLS ? kHalfBytes + kTile * kCodesPitch : 0);
   auto fn = quantize_kernel<T, VEC, ROWS, COLS>;
   static DeviceIntCache cap_cache;
   const int cap = cap_cache.get(facts.device, [&] {
@@ -206,8 +306,7 @@ int launch_quantize(const QuantArgs& args, long long tiles, const DeviceFacts& f
 template <typename T>
 int run_quantize(const QuantArgs& args, long long tiles, const DeviceFacts& facts,
                  cudaStream_t stream) {
-  // 16-byte loads need a 16-byte base and row pitch; anything else is read
-  // element by element.
+  // 16-byte loads need a 16-byte base and row pitch.
   const bool vec = aligned(args.x, 16) && args.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const bool rows = args.codes != nullptr, cols = args.codes_t != nullptr;
   if (vec) {
@@ -226,76 +325,103 @@ struct DequantArgs {
   void* y;
   long long rows, cols, ld;
   long long tiles_x;
-  int vec;  // rows of y start on 16-byte boundaries
 };
 
-// The same tiles the other way: a thread turns 4 code bytes of a row into 8
-// values.  code * 2^e is exact in fp32 and is rounded once to T.
-template <typename T>
+// The same tiles the other way.  code * 2^e is exact in fp32 and is rounded
+// once to T.  VEC: a thread turns 4 code bytes of a row into 8 values, 16-byte
+// stores.  Otherwise rows of Y start anywhere, and a warp stores 32 values of a
+// row side by side (8 values a thread, element by element, took 42 us instead
+// of TODO for 2072 x 4099 fp32).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     dequantize_kernel(const __grid_constant__ DequantArgs args) {
+  constexpr int kDeqVec = 8;
+  constexpr int kDeqLanes = kTile / kDeqVec, kDeqRows = kThreads / kDeqLanes;
+  constexpr int kDeqPasses = kTile / kDeqRows;
   __shared__ __align__(16) uint8_t s_scales[kHalfBytes];
   const int tid = threadIdx.x;
   const long long tiles_x = args.tiles_x;  // tiles that hold values (the last may be half past the edge)
   const long long tx = static_cast<long long>(blockIdx.x) % tiles_x;
   const long long ty = static_cast<long long>(blockIdx.x) / tiles_x;
   const long long r0 = ty * kTile, c0 = tx * kTile;
-  const int col = (tid % kLanesPerRow) * kVec;
-  const int row = tid / kLanesPerRow;
   const long long pitch = mx_padded(args.cols) / 2;
+  const int col = (tid % kDeqLanes) * kDeqVec;
+  const int row = tid / kDeqLanes;
   const long long left = args.cols - c0 - col;
-  const int valid = left <= 0 ? 0 : left >= kVec ? kVec : static_cast<int>(left);
-  uint32_t w[kPasses];
+  const int valid = left <= 0 ? 0 : left >= kDeqVec ? kDeqVec : static_cast<int>(left);
+  uint32_t w[kDeqPasses];
+  if constexpr (VEC) {
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const long long r = r0 + row + p * kRowsPerPass;
-    w[p] = valid > 0 && r < args.rows
-               ? __ldg(reinterpret_cast<const uint32_t*>(args.codes + r * pitch + (c0 + col) / 2))
-               : 0u;
+    for (int p = 0; p < kDeqPasses; ++p) {
+      const long long r = r0 + row + p * kDeqRows;
+      w[p] = valid > 0 && r < args.rows
+                 ? __ldg(reinterpret_cast<const uint32_t*>(args.codes + r * pitch + (c0 + col) / 2))
+                 : 0u;
+    }
   }
   if (tid < kHalfBytes / 16)
     reinterpret_cast<uint4*>(s_scales)[tid] = __ldg(
         reinterpret_cast<const uint4*>(args.scales + (ty * mx_tiles(args.cols) + tx) * kHalfBytes) + tid);
   __syncthreads();
+  if constexpr (VEC) {
 #pragma unroll
-  for (int p = 0; p < kPasses; ++p) {
-    const int lr = row + p * kRowsPerPass;
-    const long long r = r0 + lr;
-    if (valid == 0 || r >= args.rows) continue;
-    const float scale = scale_value(s_scales[(lr & 31) * 16 + (lr >> 5) * 4 + (col >> 5)]);
-    uint32_t h[4];
-    decode8(w[p], h);
-    float v[kVec];
+    for (int p = 0; p < kDeqPasses; ++p) {
+      const int lr = row + p * kDeqRows;
+      const long long r = r0 + lr;
+      if (valid == 0 || r >= args.rows) continue;
+      const float scale = scale_value(s_scales[(lr & 31) * 16 + (lr >> 5) * 4 + (col >> 5)]);
+      uint32_t h[4];
+      decode8(w[p], h);
+      float v[kDeqVec];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      unpack2<__half>(h[i], v[2 * i], v[2 * i + 1]);
-      v[2 * i] *= scale;
-      v[2 * i + 1] *= scale;
-    }
-    T* dst = static_cast<T*>(args.y) + r * args.ld + c0 + col;
-    if (args.vec && valid == kVec) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
-                                                    pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      for (int i = 0; i < 4; ++i) {
+        unpack2<__half>(h[i], v[2 * i], v[2 * i + 1]);
+        v[2 * i] *= scale;
+        v[2 * i + 1] *= scale;
       }
-    } else {
+      T* dst = static_cast<T*>(args.y) + r * args.ld + c0 + col;
+      if (valid == kDeqVec) {
+        if constexpr (sizeof(T) == 4) {
+          reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
+                                                      pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (i < valid) dst[i] = from_float<T>(v[i]);
+        for (int i = 0; i < kDeqVec; ++i)
+          if (i < valid) dst[i] = from_float<T>(v[i]);
+      }
+    }
+  } else {
+    const int warp = tid >> 5, lane = tid & 31;
+#pragma unroll 4
+    for (int lr = warp; lr < kTile; lr += kThreads / 32) {
+      const long long r = r0 + lr;
+      if (r >= args.rows) break;
+      const uint32_t scales = *reinterpret_cast<const uint32_t*>(s_scales + (lr & 31) * 16 + (lr >> 5) * 4);
+      const uint8_t* src = args.codes + r * pitch + c0 / 2;
+      T* dst = static_cast<T*>(args.y) + r * args.ld + c0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * g + lane;
+        if (c0 + c >= args.cols) break;
+        const uint32_t code = __ldg(src + c / 2) >> (4 * (lane & 1)) & 15u;
+        dst[c] = from_float<T>(decode1(code) * scale_value((scales >> (8 * g)) & 255u));
+      }
     }
   }
 }
 
 template <typename T>
-int launch_dequantize(DequantArgs args, cudaStream_t stream) {
-  args.vec = aligned(args.y, 16) && args.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
+int launch_dequantize(const DequantArgs& args, cudaStream_t stream) {
+  const bool vec = aligned(args.y, 16) && args.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const long long tiles = args.tiles_x * ((args.rows + kTile - 1) / kTile);
   if (tiles > INT_MAX) return TCB_ERR_RESOURCE;
   clear_stale_error();
-  dequantize_kernel<T><<<static_cast<unsigned>(tiles), kThreads, 0, stream>>>(args);
+  (vec ? dequantize_kernel<T, true> : dequantize_kernel<T, false>)<<<
+      static_cast<unsigned>(tiles), kThreads, 0, stream>>>(args);
   return launch_status();
 }
 

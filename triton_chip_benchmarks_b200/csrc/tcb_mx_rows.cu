@@ -437,7 +437,7 @@ int launch_rows(const RowsProblem& p, int* status, const DeviceFacts& facts, cud
   const long long chunks = (static_cast<long long>(p.m) + R::kTokens - 1) / R::kTokens;
   // As many CTAs of a row tile as fit beside the other tiles in one round of
   // the SMs, each with at least one K block.
-  long long split = facts.sm_count / (tiles * chunks);
+  long long split = static_cast<long long>(facts.sm_count) * R::kCtas / (tiles * chunks);
   split = split > kMaxSplit ? kMaxSplit : split;
   split = split > args.kblocks ? args.kblocks : split;
   args.split = split < 1 ? 1 : static_cast<int>(split);

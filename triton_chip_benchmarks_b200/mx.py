@@ -30,7 +30,12 @@ from .validation import MX_GROUP_SIZE
 RULES = {"floor": _native.MX_FLOOR, "up": _native.MX_UP}
 _DTYPES = {torch.bfloat16: _native.T_BF16, torch.float16: _native.T_FP16,
            torch.float32: _native.T_FP32}
+_current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _code_bytes(rows: int, cols: int) -> int:
+    return rows * ((cols + MX_GROUP_SIZE - 1) // MX_GROUP_SIZE) * (MX_GROUP_SIZE // 2)
 
 
 def _packed_bytes(rows: int, cols: int) -> int:
@@ -45,7 +50,7 @@ class MxTensor:
     cols), ``scales`` the E8M0 scales in the layout of ``tcb_mx_scales_pack``.
     """
 
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("rows", "cols", "device", "codes_ptr", "scales_ptr", "_held")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -58,17 +63,23 @@ class MxTensor:
                              f"{_packed_bytes(rows, cols)} bytes, got {scales.numel()}")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("MX codes and scales are contiguous")
-        if codes.device != scales.device or not codes.is_cuda:
+        device = codes.device
+        if device != scales.device or not codes.is_cuda:
             raise ValueError("MX codes and scales are on one CUDA device")
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self.rows, self.cols, self.device = rows, cols, device
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+        self._held = (codes, scales)
 
-    @property
-    def shape(self) -> tuple[int, int]:
-        return self.rows, self.cols
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    @classmethod
+    def empty(cls, rows: int, cols: int, device: torch.device) -> "MxTensor":
+        """Uninitialised, codes and scales in one allocation."""
+        t = cls.__new__(cls)
+        offset = (_code_bytes(rows, cols) + 255) // 256 * 256
+        held = torch.empty(offset + _packed_bytes(rows, cols), dtype=torch.uint8, device=device)
+        t.rows, t.cols, t.device, t._held = rows, cols, held.device, held
+        t.codes_ptr = held.data_ptr()
+        t.scales_ptr = t.codes_ptr + offset
+        return t
 
     @classmethod
     def from_rows(cls, codes: torch.Tensor, scales: torch.Tensor, cols: int) -> "MxTensor":
@@ -83,27 +94,37 @@ class MxTensor:
                 _native.mx_scales_pack(scales, packed, rows, groups)
         return cls(codes, packed, rows, cols)
 
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if isinstance(self._held, tuple):
+            return self._held[0]
+        return self._held[:_code_bytes(self.rows, self.cols)].view(self.rows, (self.cols + 31) // 32 * 16)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if isinstance(self._held, tuple):
+            return self._held[1]
+        return self._held[self.scales_ptr - self.codes_ptr:]
+
     def __repr__(self) -> str:
         return f"MxTensor({self.rows} x {self.cols}, {self.device})"
 
 
-def _launch(device: torch.device, fn, *args, **kwargs) -> None:
-    """fn(...) on the device's current stream, with `device` current."""
+def _call(name: str, device: torch.device, *args) -> None:
+    """The library's entry point on the device's current stream, with the device current."""
     index = device.index
-    raw = _raw_stream(index)
-    if index == torch.cuda.current_device():
-        fn(*args, stream=raw, **kwargs)
+    fn = getattr(_native.load(), name)
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            fn(*args, stream=raw, **kwargs)
-
-
-def _empty(device: torch.device, rows: int, cols: int) -> MxTensor:
-    t = MxTensor.__new__(MxTensor)
-    t.codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=device)
-    t.scales = torch.empty(_packed_bytes(rows, cols), dtype=torch.uint8, device=device)
-    t.rows, t.cols = rows, cols
-    return t
+            status = fn(*args, _raw_stream(index))
+    if status:
+        raise _native.TcbError(status, name)
 
 
 def _dtype_code(dtype: torch.dtype, what: str) -> int:
@@ -164,12 +185,12 @@ def _quantize(x: torch.Tensor, rule: str, rows: bool, cols: bool):
             raise ValueError("one axis of x has to be contiguous and its rows must not overlap")
     r, c = x.shape
     device = x.device
-    by_row = _empty(device, r, c) if rows else None
-    by_col = _empty(device, c, r) if cols else None
+    by_row = MxTensor.empty(r, c, device) if rows else None
+    by_col = MxTensor.empty(c, r, device) if cols else None
     if r and c:
-        _launch(device, _native.mx_quantize, dtype, x, r, c, pitch, code,
-                by_row.codes if rows else None, by_row.scales if rows else None,
-                by_col.codes if cols else None, by_col.scales if cols else None)
+        _call("tcb_mx_quantize", device, dtype, x.data_ptr(), r, c, pitch, code,
+              by_row.codes_ptr if rows else None, by_row.scales_ptr if rows else None,
+              by_col.codes_ptr if cols else None, by_col.scales_ptr if cols else None)
     return (by_col, by_row) if swap else (by_row, by_col)
 
 
@@ -194,8 +215,8 @@ def dequantize(q: MxTensor, dtype: torch.dtype = torch.bfloat16, *, out: torch.T
     """The values of q, rounded once to `dtype` (or to out's type)."""
     y = _output(out, q.device, q.rows, q.cols, dtype)
     if q.rows and q.cols:
-        _launch(q.device, _native.mx_dequantize, _dtype_code(y.dtype, "the output"), q.codes,
-                q.scales, q.rows, q.cols, y, _pitch(y))
+        _call("tcb_mx_dequantize", q.device, _DTYPES[y.dtype], q.codes_ptr, q.scales_ptr, q.rows,
+              q.cols, y.data_ptr(), _pitch(y))
     return y
 
 
@@ -214,7 +235,8 @@ def _output(out: torch.Tensor | None, device: torch.device, rows: int, cols: int
     return out
 
 
-def _bias(bias: torch.Tensor | None, n: int, y: torch.Tensor) -> torch.Tensor | None:
+def _bias(bias: torch.Tensor | None, n: int, y: torch.Tensor) -> int | None:
+    """Address of a bias [n] of y's type."""
     if bias is None:
         return None
     if bias.dtype != y.dtype:
@@ -223,7 +245,7 @@ def _bias(bias: torch.Tensor | None, n: int, y: torch.Tensor) -> torch.Tensor | 
         raise ValueError(f"bias is a contiguous [{n}], got {list(bias.shape)}")
     if bias.device != y.device:
         raise ValueError(f"bias is on {bias.device}, the operands are on {y.device}")
-    return bias
+    return bias.data_ptr()
 
 
 def matmul(a: MxTensor, b: MxTensor, *, bias: torch.Tensor | None = None,
@@ -239,10 +261,10 @@ def matmul(a: MxTensor, b: MxTensor, *, bias: torch.Tensor | None = None,
     if a.cols == 0:
         raise ValueError("a product over no columns")
     y = _output(out, a.device, a.rows, b.rows, dtype)
-    bias = _bias(bias, b.rows, y)
+    bias_ptr = _bias(bias, b.rows, y)
     if a.rows and b.rows:
-        _launch(a.device, _native.mx_gemm, a.codes, a.scales, b.codes, b.scales, y, a.rows,
-                b.rows, a.cols, dtype=_DTYPES[y.dtype], ldc=_pitch(y), bias=bias, status=status)
+        _call("tcb_mx_gemm", a.device, a.codes_ptr, a.scales_ptr, b.codes_ptr, b.scales_ptr, bias_ptr,
+              _DTYPES[y.dtype], y.data_ptr(), _pitch(y), a.rows, b.rows, a.cols, _native._ptr(status))
     return y
 
 
@@ -268,11 +290,11 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
     if pitch is None:
         raise ValueError("the rows of x have to be contiguous and must not overlap")
     y = _output(out, m.device, m.shape[0], w.rows, x.dtype if dtype is None else dtype)
-    bias = _bias(bias, w.rows, y)
+    bias_ptr = _bias(bias, w.rows, y)
     if m.shape[0] and w.rows:
-        _launch(m.device, _native.mx_linear, _DTYPES[x.dtype], m, pitch, w.codes, w.scales, y,
-                m.shape[0], w.rows, w.cols, dtype=_DTYPES[y.dtype], ldy=_pitch(y), bias=bias,
-                status=status)
+        _call("tcb_mx_linear", m.device, _DTYPES[x.dtype], m.data_ptr(), pitch, w.codes_ptr,
+              w.scales_ptr, bias_ptr, _DTYPES[y.dtype], y.data_ptr(), _pitch(y), m.shape[0], w.rows,
+              w.cols, _native._ptr(status))
     return y if out is not None or len(lead) == 1 else y.view(*lead, w.rows)
 
 
