@@ -242,10 +242,19 @@ int tcb_mx_gemm(const void *A, const void *SA, const void *B, const void *SB, co
 
 /* Y [M][N] = X [M][K] . W [N][K]^T (+ bias [N]) with X in TCB_T_BF16 or TCB_T_FP16
  * (row pitch ldx >= K elements) and only W quantised; Y and bias in `dtype` as
- * above.  Meant for few rows (decoding): W is read once per 64 rows of X. */
+ * above.  X takes part as eight MX FP4 digits of three bits: within a group of 32
+ * values of a row, each is taken to 2^-24 of the group's largest.  Infinities and
+ * NaN propagate as in the plain product.  Meant for few rows (decoding); W is read
+ * once per 16 rows of X.  workspace (256-byte aligned) holds
+ * tcb_mx_linear_workspace_bytes(M, K) bytes that the call overwrites and needs
+ * until its work on `stream` is done; it may be NULL where that is 0. */
 int tcb_mx_linear(int x_dtype, const void *X, long long ldx, const void *W, const void *SW,
                   const void *bias, int dtype, void *Y, long long ldy, int M, int N, int K,
-                  int *status_dev, tcb_stream_t stream);
+                  void *workspace, long long workspace_bytes, int *status_dev, tcb_stream_t stream);
+
+/* Bytes of tcb_mx_linear's workspace (0 for one or two rows).
+ * TCB_ERR_INVALID_ARGUMENT for M < 0 or K <= 0. */
+long long tcb_mx_linear_workspace_bytes(int M, int K);
 
 /* MX FP4 GEMM that allocates nothing, for callers that cannot allocate device
  * memory (a plugin whose host framework owns all device memory through its

@@ -139,13 +139,21 @@ def test_entry_points_refuse_bad_arguments_before_a_device_is_touched(native):
     assert gemm(p, p, p, p, None, native.T_TF32, p, 8, 4, 8, 32, None, None) == unsupported
     assert gemm(p, p, p + 4, p, None, bf16, p, 8, 4, 8, 32, None, None) == native.ERR_ALIGNMENT
     assert gemm(None, None, None, None, None, bf16, None, 8, 0, 8, 32, None, None) == native.OK
-    linear = lib.tcb_mx_linear
-    assert linear(bf16, p, 31, p, p, None, bf16, p, 8, 1, 8, 32, None, None) == bad  # pitch below K
-    assert linear(bf16, p, 32, p, p, None, bf16, None, 8, 1, 8, 32, None, None) == bad
-    assert linear(native.T_FP32, p, 32, p, p, None, bf16, p, 8, 1, 8, 32, None, None) == unsupported
-    assert linear(bf16, p, 32, p, p, None, native.T_INT8, p, 8, 1, 8, 32, None, None) == unsupported
-    assert linear(bf16, p, 32, p, p, p + 1, bf16, p, 8, 1, 8, 32, None, None) == native.ERR_ALIGNMENT
-    assert linear(bf16, None, 32, None, None, None, bf16, None, 8, 0, 8, 32, None, None) == native.OK
+    linear, none = lib.tcb_mx_linear, (None, 0, None, None)
+    assert linear(bf16, p, 31, p, p, None, bf16, p, 8, 1, 8, 32, *none) == bad  # pitch below K
+    assert linear(bf16, p, 32, p, p, None, bf16, None, 8, 1, 8, 32, *none) == bad
+    assert linear(native.T_FP32, p, 32, p, p, None, bf16, p, 8, 1, 8, 32, *none) == unsupported
+    assert linear(bf16, p, 32, p, p, None, native.T_INT8, p, 8, 1, 8, 32, *none) == unsupported
+    assert linear(bf16, p, 32, p, p, p + 1, bf16, p, 8, 1, 8, 32, *none) == native.ERR_ALIGNMENT
+    assert linear(bf16, None, 32, None, None, None, bf16, None, 8, 0, 8, 32, *none) == native.OK
+    need = native.mx_linear_workspace_bytes(40, 1000)
+    assert need > 0 and native.mx_linear_workspace_bytes(1, 1000) == 0
+    assert linear(bf16, p, 1000, p, p, None, bf16, p, 8, 40, 8, 1000, p, need - 1, None, None) == bad
+    assert linear(bf16, p, 1000, p, p, None, bf16, p, 8, 40, 8, 1000, None, need, None, None) == bad
+    assert linear(bf16, p, 1000, p, p, None, bf16, p, 8, 40, 8, 1000, p + 16, need, None,
+                  None) == native.ERR_ALIGNMENT
+    with pytest.raises(native.TcbError):
+        native.mx_linear_workspace_bytes(1, 0)
 
 
 def test_host_tensors_and_wrong_codes_are_refused():
@@ -400,8 +408,8 @@ def test_linear_of_activations(cuda, m, n, k, x_dtype):
     w = mx.quantize((activations((n, k), FP32, seed=2) * 0.02).to(cuda))
     vw = f64(mx.dequantize(w, FP32))
     for dtype in (x_dtype, FP32):
-        # bf16 rows are rounded to 2^-39 of their block's largest value, far
-        # below the 2^-23 of the sum that holds it.
+        # A value is off by at most 2^-24 of its group's largest, on average below
+        # the 2^-23 of |x| that the bound has for each of the K terms.
         check_product(mx.linear(x.to(cuda), w, dtype=dtype), f64(x), vw)
 
 
@@ -425,10 +433,12 @@ def test_linear_of_the_smallest_normal_rows(cuda):
 
 
 @gpu
-def test_linear_with_infinite_rows(cuda):
+@pytest.mark.parametrize("rows", [2, 8])
+def test_linear_with_infinite_rows(cuda, rows):
     x = activations((4, 300), BF16, seed=3)
     x[1, 7], x[2, 9], x[3, 299] = float("inf"), float("nan"), -float("inf")
     x[1, 8] = 1e30
+    x = torch.cat((x, x.flip(0)))[:rows]
     w = mx.quantize(activations((70, 300), FP32, seed=8).to(cuda))
     vw = f64(mx.dequantize(w, FP32))
     with np.errstate(invalid="ignore"):

@@ -49,7 +49,7 @@ EXPORTED_SYMBOLS = (
     "tcb_vector_chains", "tcb_vector_chains_imm", "tcb_tensor_peak", "tcb_gemm", "tcb_mx_scales_packed_bytes",
     "tcb_mx_scales_pack", "tcb_kernel_info", "tcb_gemm_mxf4_noalloc",
     "tcb_selftest_bounded_wait", "tcb_mx_quantize", "tcb_mx_dequantize", "tcb_mx_gemm",
-    "tcb_mx_linear",
+    "tcb_mx_linear", "tcb_mx_linear_workspace_bytes",
 )
 
 
@@ -152,13 +152,15 @@ def load() -> ctypes.CDLL:
         lib.tcb_mx_quantize.argtypes = [i, vp, ll, ll, ll, i, vp, vp, vp, vp, vp]
         lib.tcb_mx_dequantize.argtypes = [i, vp, vp, ll, ll, vp, ll, vp]
         lib.tcb_mx_gemm.argtypes = [vp, vp, vp, vp, vp, i, vp, ll, i, i, i, vp, vp]
-        lib.tcb_mx_linear.argtypes = [i, vp, ll, vp, vp, vp, i, vp, ll, i, i, i, vp, vp]
+        lib.tcb_mx_linear.argtypes = [i, vp, ll, vp, vp, vp, i, vp, ll, i, i, i, vp, ll, vp, vp]
+        lib.tcb_mx_linear_workspace_bytes.argtypes = [i, i]
         lib.tcb_selftest_bounded_wait.argtypes = [ll, vp, vp]
         lib.tcb_kernel_info.argtypes = [i, i, i, i, i, i, i, i, ctypes.POINTER(KernelInfo)]
         for name in EXPORTED_SYMBOLS:
             if name not in ("tcb_strerror", "tcb_version"):
                 getattr(lib, name).restype = i
         lib.tcb_mx_scales_packed_bytes.restype = ctypes.c_longlong
+        lib.tcb_mx_linear_workspace_bytes.restype = ctypes.c_longlong
         _lib = lib
         return lib
 
@@ -308,11 +310,19 @@ def mx_gemm(a, scale_a, b, scale_b, c, m: int, n: int, k: int, *, dtype: int, ld
 
 
 def mx_linear(x_dtype: int, x, ldx: int, w, scale_w, y, m: int, n: int, k: int, *, dtype: int,
-              ldy: int, bias=None, status=None, stream=None) -> None:
+              ldy: int, workspace=None, workspace_bytes: int = 0, bias=None, status=None,
+              stream=None) -> None:
     """Y = X . W^T (+ bias) with 16-bit X and an MX FP4 weight, Y in `dtype`."""
     check(load().tcb_mx_linear(x_dtype, _ptr(x), ldx, _ptr(w), _ptr(scale_w), _ptr(bias), dtype,
-                               _ptr(y), ldy, m, n, k, _ptr(status), _stream(stream)),
-          "tcb_mx_linear")
+                               _ptr(y), ldy, m, n, k, _ptr(workspace), workspace_bytes,
+                               _ptr(status), _stream(stream)), "tcb_mx_linear")
+
+
+def mx_linear_workspace_bytes(m: int, k: int) -> int:
+    """Bytes of mx_linear's workspace for m rows of k values."""
+    n = load().tcb_mx_linear_workspace_bytes(m, k)
+    check(n if n < 0 else OK, "tcb_mx_linear_workspace_bytes")
+    return int(n)
 
 
 def selftest_bounded_wait(limit_ns: int, status, stream=None) -> None:

@@ -11,7 +11,7 @@ namespace {
 
 // Up to here the weight's bytes bound the product and the few-row kernel,
 // which spreads them over every SM, is faster than tiles of 256 rows.
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 256;
 
 bool out_type(int dtype, int* rows, int* pair, int* bytes) {
   switch (dtype) {
@@ -47,7 +47,7 @@ extern "C" int tcb_mx_gemm(const void* A, const void* SA, const void* B, const v
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (M <= kFewRows) {
     const RowsProblem p{A, SA, B, SB, bias, C, 0, ldc, M, N, K, kRowsMx, rows_type};
-    return mx_rows_run(p, status_dev, facts, s);
+    return mx_rows_run(p, nullptr, status_dev, facts, s);
   }
   const PairProblem p{A, B, SA, SB, bias, C, ldc, M, N, static_cast<int>(mx_detail::mx_padded(K)),
                       pair_type, gemm_pair_idesc()};
@@ -56,7 +56,8 @@ extern "C" int tcb_mx_gemm(const void* A, const void* SA, const void* B, const v
 
 extern "C" int tcb_mx_linear(int x_dtype, const void* X, long long ldx, const void* W, const void* SW,
                              const void* bias, int dtype, void* Y, long long ldy, int M, int N, int K,
-                             int* status_dev, tcb_stream_t stream) {
+                             void* workspace, long long workspace_bytes, int* status_dev,
+                             tcb_stream_t stream) {
   if (M < 0 || N < 0 || K <= 0 || ldx < K || ldy < N) return TCB_ERR_INVALID_ARGUMENT;
   int rows_type, pair_type, bytes;
   if (!out_type(dtype, &rows_type, &pair_type, &bytes)) return TCB_ERR_UNSUPPORTED;
@@ -64,6 +65,9 @@ extern "C" int tcb_mx_linear(int x_dtype, const void* X, long long ldx, const vo
   if (M == 0 || N == 0) return TCB_OK;
   if (X == nullptr || W == nullptr || SW == nullptr || Y == nullptr) return TCB_ERR_INVALID_ARGUMENT;
   if (K > INT_MAX - 256) return TCB_ERR_RESOURCE;
+  const long long need = mx_rows_workspace(M, K);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr)) return TCB_ERR_INVALID_ARGUMENT;
+  if (!aligned(workspace, 256)) return TCB_ERR_ALIGNMENT;
   if (!aligned(X, 2) || !aligned(W, 16) || !aligned(SW, 16) || !aligned(Y, bytes) ||
       !aligned(bias, bytes))
     return TCB_ERR_ALIGNMENT;
@@ -73,5 +77,10 @@ extern "C" int tcb_mx_linear(int x_dtype, const void* X, long long ldx, const vo
   if (facts.major != 10) return TCB_ERR_UNSUPPORTED;
   const RowsProblem p{X, nullptr, W, SW, bias, Y, ldx, ldy, M, N, K,
                       x_dtype == TCB_T_BF16 ? kRowsBf16 : kRowsFp16, rows_type};
-  return mx_rows_run(p, status_dev, facts, reinterpret_cast<cudaStream_t>(stream));
+  return mx_rows_run(p, workspace, status_dev, facts, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" long long tcb_mx_linear_workspace_bytes(int M, int K) {
+  if (M < 0 || K <= 0) return TCB_ERR_INVALID_ARGUMENT;
+  return mx_rows_workspace(M, K);
 }

@@ -1,40 +1,55 @@
-// Products of a few rows with an MX FP4 weight (sm_100a): Y = X . W^T.
+// Products of a few rows with an MX FP4 weight on 5th-generation tensor cores
+// (sm_100a): Y = X . W^T, W [N][K] in MX FP4, X a few rows of MX FP4, bf16 or fp16.
 //
-// X has M rows (tokens) of bf16, fp16 or MX FP4; W [N][K] is MX FP4.  With few
-// rows the weight's bytes are all that counts: 17/32 byte a weight, read once.
-// The tensor core does the arithmetic as mma.sync m16n8k16 (fp16 x fp16 ->
-// fp32) with 16 weight rows as the M side and 8 tokens as the N side: E2M1 is
-// exact in fp16, and one cvt decodes two codes.  (tcgen05 would want the
-// decoded weights back in shared memory or tensor memory; here they go from
-// registers straight into the MMA.)
+// With few rows the weight's bytes are all that counts (17/32 byte a weight,
+// read once), so the weight takes the M side of the MMA -- 128 rows a CTA, all
+// SMs busy -- and X the N side, 8 to 256 columns of
+// tcgen05.mma kind::mxf4.block_scale: nothing is decoded by threads.
 //
-//   y[t][n] = sum_blocks 2^ex(t, block) sum_groups 2^ew(n, group) tmp,
-//   tmp = sum over the group's 32 values of x'[t][k] * code(w[n][k]).
+// 16-bit rows as MX FP4 digits.  A group of 32 values with the largest in
+// [2^(e+1), 2^(e+2)) is split exactly into E2M1 digits,
+//   u_0 = x * 2^-e (|u_0| < 4),  d_i = RNE_E2M1(u_i),  u_{i+1} = 8 (u_i - d_i),
+//   x = sum_i d_i 2^(e - 3i):  |u_i| <= 4 keeps the rounding below 1/2, so each
+// digit gives three bits more.  Eight digits hold a value to 2^-24 of its
+// group's largest: bf16 values down to 2^-16 of it (fp16: 2^-13) without any
+// error, smaller ones as a 24-bit fixed-point number, the precision that an
+// fp32 sum holding the largest has.  The digits are eight rows of an MX tensor
+// whose scales differ by 2^3, so one block-scaled MMA sums them all, and the
+// epilogue adds a token's eight columns in fp32, smallest first.  (Decoding W to
+// fp16 for mma.sync instead was bound by issue slots: 24 us at
+// 1 x 16384 x 8192, 31 us at 16 x 8192 x 8192.)  Infinities and NaN have no
+// digits: they count as zero there, and the NaN scale on their group's last
+// digit makes the epilogue take their products with the row's weights one by
+// one (the token's results are then infinite or NaN whatever the rest sums to).
 //
-// tmp is one pair of MMAs from a zero accumulator; the group's weight scale is
-// applied to it in fp32, so any E8M0 scale is exact.  bf16 rows are brought
-// into fp16's range by a power of two per token and 256 values of K, which
-// puts the largest at 2^14..2^15: values down to 2^-31 of the largest stay
-// exact and smaller ones are rounded to 2^-39 of it, below what an fp32 sum
-// that holds the largest can show.  fp16 rows are taken as they are; MX rows
-// are decoded, their scale per group applied with the weight's.
+// Where the digits come from.  Up to kInlineTokens rows, X warps of each CTA write
+// the digits of its K slice into shared memory on the way; for more rows a
+// kernel of their own writes them once (into the caller's workspace), and the
+// product starts beside it (programmatic dependent launch): its weight loads
+// are under way before the digits are there.
 //
-// Data flow.  A CTA owns 128 rows of W and a slice of K.  A producer warp
-// TMA-loads stages of 256 K values (128 bytes of codes x 128 rows in the
-// 128-byte swizzle, 1 KB of packed scales, the X tile) into a ring; four X warps
-// turn the X tile into fp16 fragments in place; eight consumer warps take 16
-// weight rows each.  A lane's four code bytes of a row (a quarter of a group)
-// are k = 8t..8t+7 of the group; the order of k inside an MMA is free as long
-// as X follows it, so its X fragment is one 16-byte load.
+// Split over K.  With fewer row tiles than CTAs fit, up to eight CTAs of a
+// cluster share a row tile, each with a part of K.  Each sends the others their
+// share of its partial sums (stores into distributed shared memory) and adds
+// its own share in rank order: no workspace, the same result every time, and
+// one cluster barrier (the sums of up to kEarlyTokens tokens have room of their
+// own; those of more go where the ring was, which all CTAs must have left).
 //
-// Split over K.  With fewer row tiles than SMs, up to eight CTAs of a cluster
-// share a row tile, each with a part of K, and add their partial sums through
-// distributed shared memory in rank order: one launch, no workspace, the same
-// result every time.
+// Roles of a CTA (one tile each):
+//   warp 0      producer: per 256 K values, TMA loads of W (128 rows x 128 B) and X
+//               (128-byte swizzle), bulk copies of their packed scales;
+//   warp 1      MMA issuer: four MMAs a stage into one accumulator;
+//   warps 2-5   scale writers (shared -> tensor memory), then the epilogue;
+//   warps 6-9   X warps (inline digits only).
+// Every wait is bounded; a wait that runs out raises the CTA's abort flag, all
+// roles leave their loops, copies and MMAs in flight are waited for (bounded
+// too), and nothing is stored.
 #include <cudaTypedefs.h>
+#include <type_traits>
 
 #include "tcb_device.cuh"
 #include "tcb_gemm_common.cuh"
+#include "tcb_gemm_pair.h"
 #include "tcb_host.h"
 #include "tcb_mx.cuh"
 #include "tcb_mx_rows.h"
@@ -47,419 +62,567 @@ namespace {
 
 using namespace mx_detail;
 using gemm_detail::bulk_load_1d;
+using gemm_detail::kBlockBytes;
+using gemm_detail::kSfPairCols;
+using gemm_detail::kSfStageCols;
+using gemm_detail::kStepsPerBlock;
 using gemm_detail::mbar_arrive;
+using gemm_detail::sf_cols_a;
+using gemm_detail::sf_cols_b;
+using gemm_detail::sf_idesc;
 using gemm_detail::wait_or_abort;
 
-constexpr int kRowTile = 128;
-constexpr int kConsumerWarps = kRowTile / 16;
+constexpr int kRowTile = 128;                     // weight rows of a CTA
+constexpr int kBlockK = 2 * kBlockBytes;          // K values of a stage
+constexpr int kWBytes = kRowTile * kBlockBytes;   // 16 KB
+constexpr int kScaleBlock = 1024;                 // packed scales of 128 rows x 256 values
+constexpr int kMaxStages = 8;
+constexpr int kMaxCols = 256;                     // MX rows; digits take up to kPairedCols
+constexpr int kDigits = 8;
+constexpr int kDigitBits = 3;
+constexpr int kInlineTokens = 2;
+constexpr int kDigitRows = 128;                   // digit rows of a column tile, used or not
 constexpr int kXWarps = 4;
-constexpr int kProducerWarp = kConsumerWarps;
-constexpr int kRowsThreads = (kConsumerWarps + 1 + kXWarps) * 32;
-constexpr int kBlockK = 256;                       // K values of a stage
-constexpr int kWBytes = kRowTile * kBlockK / 2;    // 16 KB of codes
-constexpr int kScaleBytes = kRowTile * kBlockK / 32;
-constexpr int kMaxRingStages = 8;
-constexpr int kPartialPitch = kRowTile + 4;        // floats of a token's partial sums
 constexpr int kMaxSplit = 8;
+constexpr int kEarlyTokens = 16;
+// Two CTAs share an SM while X has at most this many columns.
+constexpr int kPairedCols = 128;
+constexpr int kPairedSmem = 112 * 1024;
+constexpr int kAloneSmem = 224 * 1024;
 
-// NT token tiles of 8.
-template <int XT, int NT>
-struct Rows {
-  static constexpr int kTokens = 8 * NT;
-  static constexpr int kXBytes = kTokens * kBlockK * 2;                       // fp16 fragments
-  static constexpr int kXScales = XT == kRowsMx ? 8 * kTokens : kTokens;      // fp32 factors
-  static constexpr int kRawBytes = XT == kRowsMx ? kTokens * kBlockK / 2 + kScaleBytes : 0;
-  static constexpr int kStageBytes =
-      (kWBytes + kScaleBytes + kXBytes + kRawBytes + kXScales * 4 + 1023) / 1024 * 1024;
-  static constexpr int kCtas = NT <= 2 ? 2 : 1;    // per SM
-  static constexpr int kBudget = (kCtas == 2 ? 112 : 224) * 1024 - 1024;
-  static constexpr int kStages =
-      kBudget / kStageBytes > kMaxRingStages ? kMaxRingStages : kBudget / kStageBytes;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;
-  static_assert(kStages >= 2, "a ring needs two stages");
-  static_assert(kTokens * kPartialPitch * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
-};
+enum XMode : int { kXRows = 0, kXDigits = 1, kXInline = 2 };
 
 struct RowsArgs {
-  const uint8_t* sw;    // packed scales of W
-  const uint8_t* sx;    // packed scales of X (MX)
-  const void* x;        // X, for rows that TMA cannot read
+  const uint8_t* sw;     // packed scales of W
+  const uint8_t* sx;     // packed scales of X's rows or digits
+  const uint8_t* w;      // W's codes (products of infinities and NaN)
+  const void* x;         // 16-bit X
   const void* bias;
   void* y;
+  long long pitch;       // code bytes of a row of W
   long long ldx, ldy;
   int* status;
   int m, n, k;
   int kblocks;
-  int split;            // CTAs of a cluster
-  int x_tma;
-  int y_type;           // RowsType of y and the bias
+  int split;             // CTAs of a cluster
+  int stages, stage_bytes;
+  int cols;              // columns of a column tile (a multiple of 8)
+  int tmem_cols;
+  int x_bf16;
+  int y_type;            // RowsType of y and the bias
+  uint32_t idesc;
 };
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1, const float (&c)[4]) {
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate, uint32_t tsfa, uint32_t tsfb) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]),
-        "f"(c[2]), "f"(c[3]));
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, "
+      "[%5], [%6], p;\n\t}" ::"r"(d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(tsfa), "r"(tsfb));
 }
 
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
-  return v;
+__device__ __forceinline__ void tmem_ld_8cols(uint32_t taddr, float (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+      : "r"(taddr)
+      : "memory");
 }
 
-// 16-byte chunk c of a token's 512 bytes of fragments: tokens 2i and 2i + 1,
-// which a quarter-warp reads together, use opposite halves of a 128-byte line.
-__device__ __forceinline__ int x_chunk(int token, int c) { return token * 32 + (c ^ ((token & 1) << 2)); }
+__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
 
-// One lane's 8 values of a token (16-bit words) as fp16 fragments; returns the
-// factor that the block's sums are multiplied with.
-template <int XT>
-__device__ __forceinline__ float x_fragment(const uint32_t (&w)[4], uint32_t (&h)[4]) {
-  if constexpr (XT == kRowsFp16) {
+// Returns once the kernel launched before this one has finished (at once where
+// nothing was launched to overlap).
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_next_kernel_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ float value16(uint16_t bits, bool bf16) {
+  return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
+              : __half2float(__ushort_as_half(bits));
+}
+
+// The 16-bit values x[k..k+7] of a row, zeros past the end.
+__device__ __forceinline__ uint4 load_values(const uint16_t* row, int k, int end, bool vec) {
+  if (vec && k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = w[i];
-    return 1.0f;
-  } else {
-    float v[8];
-    uint32_t top = 0;  // largest finite |x|
+  for (int i = 0; i < 8; ++i)
+    if (k + i < end) w[i / 2] |= static_cast<uint32_t>(__ldg(row + k + i)) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A lane's eight values in fp32; infinities and NaN become zeros and set `*odd`,
+// for all four lanes of the group.
+__device__ __forceinline__ void to_values(uint4 raw, bool bf16, float (&v)[8], bool* odd) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  *odd = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) unpack2<__nv_bfloat16>(w[i], v[2 * i], v[2 * i + 1]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = __float_as_uint(v[i]) & 0x7FFFFFFFu;
-      top = max(top, u < 0x7F800000u ? u : 0u);
+  for (int i = 0; i < 8; ++i) {
+    v[i] = value16(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))), bf16);
+    if ((__float_as_uint(v[i]) & 0x7FFFFFFFu) >= 0x7F800000u) {
+      v[i] = 0.0f;
+      *odd = true;
     }
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
-    // 2^(14 - exponent of the largest), at most 2^127, and its reciprocal.
-    const uint32_t fe = min(268u - (top >> 23), 254u);
-    const float factor = __uint_as_float(fe << 23);
+  }
+  const uint32_t lanes = 0xFu << (threadIdx.x & 28u);
+  *odd = (__ballot_sync(0xFFFFFFFFu, *odd) & lanes) != 0;
+}
+
+// The scale code of digit d: a digit whose scale would be below 2^-127 has none.
+__device__ __forceinline__ uint8_t digit_code(int code, int d, bool odd) {
+  return d == kDigits - 1 && odd ? 255 : static_cast<uint8_t>(max(code, 0));
+}
+
+// E8M0 code of the first digit of a group (four lanes of eight values); digit i
+// has kDigitBits * i less.  127 + (kDigits - 1) * kDigitBits for a group of zeros,
+// so that its digits' codes are valid.
+__device__ __forceinline__ int digit_scale(const float (&v)[8]) {
+  uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = pack2<__half>(v[2 * i] * factor, v[2 * i + 1] * factor);
-    return __uint_as_float(fe == 254u ? 0x00400000u : (254u - fe) << 23);
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  if (top == 0) return 127 + (kDigits - 1) * kDigitBits;
+  return max(static_cast<int>(top >> 23) - 1, 0);
+}
+
+// The next digit of eight values u (times 2^e8 - 127 of the digit): its codes; u
+// becomes what is left, times 8.
+__device__ __forceinline__ uint32_t next_digit(float (&u)[8]) {
+  const uint32_t codes = encode8(u, 1.0f, 0);
+  uint32_t h[4];
+  decode8(codes, h);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    unpack2<__half>(h[i], lo, hi);
+    u[2 * i] = (u[2 * i] - lo) * static_cast<float>(1 << kDigitBits);
+    u[2 * i + 1] = (u[2 * i + 1] - hi) * static_cast<float>(1 << kDigitBits);
+  }
+  return codes;
+}
+
+// Digits of all tokens as rows of an MX tensor, one warp per token and K block:
+// digit i of token j of a tile of `per_tile` tokens is row 128 tile + 8 j + i.
+__global__ void __launch_bounds__(256)
+    mx_digits_kernel(const uint16_t* __restrict__ x, long long ldx, int m, int k, long long pitch,
+                     int kblocks, int per_tile, int vec, int bf16, uint8_t* __restrict__ codes,
+                     uint8_t* __restrict__ scales) {
+  let_next_kernel_start();
+  const int lane = threadIdx.x & 31;
+  const long long task = static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
+  const long long token = task / kblocks;
+  const int kb = static_cast<int>(task % kblocks);
+  if (token >= m) return;
+  float u[8];
+  bool odd;
+  to_values(load_values(x + token * ldx, kb * kBlockK + lane * 8, k, vec), bf16, u, &odd);
+  const int e8 = digit_scale(u);
+  const float inv = inverse_scale(static_cast<uint32_t>(e8));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] *= inv;
+  const long long byte = static_cast<long long>(kb) * kBlockBytes + lane * 4;
+  const int group = lane >> 2;
+#pragma unroll
+  for (int d = 0; d < kDigits; ++d) {
+    const long long row = token / per_tile * kDigitRows + token % per_tile * kDigits + d;
+    const int code = e8 - kDigitBits * d;
+    const uint32_t w = next_digit(u);
+    if (byte < pitch) *reinterpret_cast<uint32_t*>(codes + row * pitch + byte) = code >= 0 ? w : 0u;
+    if ((lane & 3) == 0)
+      scales[((row >> 7) * kblocks + kb) * kScaleBlock + (group >> 2) * 512 + (row & 31) * 16 +
+             ((row & 127) >> 5) * 4 + (group & 3)] = digit_code(code, d, odd);
   }
 }
 
-template <int XT, int NT>
-__global__ void __launch_bounds__(kRowsThreads, Rows<XT, NT>::kCtas)
-    mx_rows_kernel(const __grid_constant__ CUtensorMap map_w,
-                   const __grid_constant__ CUtensorMap map_x,
+// The last step of a CTA: its rows' sums over the ranks in order, the bias, one
+// rounding.  A warp takes every kth token, eight at a time, a lane one row.
+struct Finish {
+  const float* sums;  // [split][tokens][share], shared memory
+  int split, tokens, share, rows;
+  int warp, warps, lane;
+
+  template <typename T>
+  __device__ __forceinline__ void run(const T* bias, long long n0, T* y, long long ldy) const {
+    constexpr int kBatch = 8;
+    for (int row = lane; row < rows; row += 32) {
+      const float b = bias == nullptr ? 0.0f : to_float(bias[n0 + row]);
+      for (int first = warp; first < tokens; first += kBatch * warps) {
+        float v[kBatch] = {};
+        for (int q = 0; q < split; ++q) {
+          const float* s = sums + q * tokens * share + row;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) v[i] += s[min(first + i * warps, tokens - 1) * share];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int token = first + i * warps;
+          if (token < tokens) y[token * ldy + row] = from_float<T>(v[i] + b);
+        }
+      }
+    }
+  }
+};
+
+template <int XMODE>
+__global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
+    mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ RowsArgs args) {
-  using R = Rows<XT, NT>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t loaded[R::kStages];
-  __shared__ __align__(8) uint64_t ready[R::kStages];
-  __shared__ __align__(8) uint64_t empty[R::kStages];
+  __shared__ __align__(8) uint64_t loaded[kMaxStages];  // operand and scale bytes landed
+  __shared__ __align__(8) uint64_t digits[kMaxStages];  // X warps wrote the stage's digits
+  __shared__ __align__(8) uint64_t full[kMaxStages];    // scales are in tensor memory
+  __shared__ __align__(8) uint64_t empty[kMaxStages];   // the stage's MMAs have finished
+  __shared__ __align__(8) uint64_t acc_full;
+  __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
+
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / args.split, rank = blockIdx.x % args.split;
-  const int token0 = blockIdx.y * R::kTokens;
   const int kb0 = static_cast<int>(static_cast<long long>(args.kblocks) * rank / args.split);
   const int kb1 = static_cast<int>(static_cast<long long>(args.kblocks) * (rank + 1) / args.split);
+  const int nkb = kb1 - kb0;
+  constexpr int kPerToken = XMODE == kXRows ? 1 : kDigits;  // columns of a token
+  const int token0 = static_cast<int>(blockIdx.y) * (args.cols / kPerToken);
+  // X's first row: column tiles of digits start on 128-row blocks of scales.
+  const int row0 = static_cast<int>(blockIdx.y) * (XMODE == kXDigits ? kDigitRows : args.cols);
+  const int tokens = min(args.cols / kPerToken, args.m - token0);
+  const int x_bytes = args.cols * kBlockBytes;
+  const int sx_blocks = args.cols > 128 ? 2 : 1;
 
+  auto load_w = [&](int it) {
+    const int s = it % args.stages, kb = kb0 + it;
+    uint8_t* stage = smem + s * args.stage_bytes;
+    mbar_arrive_expect_tx(&loaded[s], kWBytes + kScaleBlock +
+                                          (XMODE == kXInline ? 0 : x_bytes + sx_blocks * kScaleBlock));
+    tma_load_2d(stage, &map_w, kb * kBlockBytes, tile * kRowTile, &loaded[s]);
+    bulk_load_1d(stage + kWBytes + x_bytes,
+                 args.sw + (static_cast<long long>(tile) * args.kblocks + kb) * kScaleBlock,
+                 kScaleBlock, &loaded[s]);
+  };
+  auto load_x = [&](int it) {
+    uint8_t* stage = smem + (it % args.stages) * args.stage_bytes;
+    uint64_t* bar = &loaded[it % args.stages];
+    const int kb = kb0 + it;
+    tma_load_2d(stage + kWBytes, &map_x, kb * kBlockBytes, row0, bar);
+    const uint8_t* sx = args.sx + (static_cast<long long>(row0 / 128) * args.kblocks + kb) * kScaleBlock;
+    uint8_t* dst = stage + kWBytes + x_bytes + kScaleBlock;
+    bulk_load_1d(dst, sx, kScaleBlock, bar);
+    if (sx_blocks == 2)
+      bulk_load_1d(dst + kScaleBlock, sx + static_cast<long long>(args.kblocks) * kScaleBlock, kScaleBlock,
+                   bar);
+  };
+  // An X warp's next values (inline digits): asked for one round ahead, the first
+  // ones before the weights, behind whose bytes they would otherwise queue.
+  [[maybe_unused]] uint4 x_next[kInlineTokens];
+  auto ask_x = [&](int it) {
+    const bool vec = (reinterpret_cast<uintptr_t>(args.x) & 15) == 0 && (args.ldx % 8 == 0 || args.m == 1);
+#pragma unroll
+    for (int i = 0; i < kInlineTokens; ++i)
+      if (i < tokens && it < nkb)
+        x_next[i] = load_values(static_cast<const uint16_t*>(args.x) + (token0 + i) * args.ldx,
+                                (kb0 + it) * kBlockK + lane * 8, args.k, vec);
+  };
+  if constexpr (XMODE == kXInline) {
+    if (warp >= 6) ask_x(warp - 6);
+  }
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
-    if (args.x_tma) prefetch_tensormap(&map_x);
-    for (int s = 0; s < R::kStages; ++s) {
+    if (XMODE != kXInline) prefetch_tensormap(&map_x);
+    for (int s = 0; s < args.stages; ++s) {
       mbar_init(&loaded[s], 1);
-      mbar_init(&ready[s], kXWarps);
-      mbar_init(&empty[s], kConsumerWarps);
+      mbar_init(&digits[s], 1);
+      mbar_init(&full[s], 4);
+      mbar_init(&empty[s], 1);
     }
+    mbar_init(&acc_full, 1);
     abort_flag = 0;
     fence_mbar_init();
+    // The first round of loads goes out before anything else is set up.
+    for (int it = 0; it < min(nkb, args.stages); ++it) {
+      load_w(it);
+      if constexpr (XMODE == kXRows) load_x(it);
+    }
   }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, args.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = tmem_slot;
+  const uint32_t tsf = tbase + static_cast<uint32_t>((args.cols + 31) & ~31);
 
-  float total[NT][4];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) total[n][i] = 0.0f;
-
-  if (warp == kProducerWarp) {
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
     if (lane == 0) {
-      const uint32_t bytes = kWBytes + kScaleBytes +
-                             (args.x_tma ? (XT == kRowsMx ? R::kTokens * kBlockK / 2 : R::kXBytes) : 0) +
-                             (XT == kRowsMx ? kScaleBytes : 0);
-      int it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % R::kStages;
-        if (!wait_or_abort(&empty[s], (static_cast<uint32_t>(it / R::kStages) & 1u) ^ 1u,
+      int it = min(nkb, args.stages);
+      if constexpr (XMODE == kXDigits) {
+        wait_for_previous_kernel();
+        for (int j = 0; j < it; ++j) load_x(j);
+      }
+      for (; it < nkb; ++it) {
+        if (!wait_or_abort(&empty[it % args.stages], (static_cast<uint32_t>(it / args.stages) & 1u) ^ 1u,
                            &abort_flag, args.status))
           break;
-        uint8_t* stage = smem + s * R::kStageBytes;
-        mbar_arrive_expect_tx(&loaded[s], bytes);
-        tma_load_2d(stage, &map_w, kb * (kBlockK / 2), tile * kRowTile, &loaded[s]);
-        bulk_load_1d(stage + kWBytes,
-                     args.sw + (static_cast<long long>(tile) * args.kblocks + kb) * kScaleBytes,
-                     kScaleBytes, &loaded[s]);
-        uint8_t* xs = stage + kWBytes + kScaleBytes;
-        if constexpr (XT == kRowsMx) {
-          tma_load_2d(xs + R::kXBytes, &map_x, kb * (kBlockK / 2), token0, &loaded[s]);
-          bulk_load_1d(xs + R::kXBytes + R::kTokens * kBlockK / 2,
-                       args.sx + (static_cast<long long>(token0 / 128) * args.kblocks + kb) * kScaleBytes,
-                       kScaleBytes, &loaded[s]);
-        } else if (args.x_tma) {
-          tma_load_2d(xs, &map_x, kb * kBlockK, token0, &loaded[s]);
-        }
+        load_w(it);
+        if constexpr (XMODE != kXInline) load_x(it);
       }
-      // After an abort too, no load is left in flight (each of the last round's
-      // barriers is still in the phase it was armed for).
-      for (int j = it > R::kStages ? it - R::kStages : 0; j < it; ++j)
-        mbar_wait(&loaded[j % R::kStages], static_cast<uint32_t>(j / R::kStages) & 1u);
+      // No load stays in flight after an abort either: each barrier of the last
+      // round is in the phase that it was armed for.
+      for (int j = it > args.stages ? it - args.stages : 0; j < it; ++j)
+        mbar_wait(&loaded[j % args.stages], static_cast<uint32_t>(j / args.stages) & 1u);
     }
     __syncwarp();
-  } else if (warp > kProducerWarp) {
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    if (lane == 0) {
+      const uint64_t desc_const = smem_desc(0, 16, 8 * kBlockBytes, 2u);
+      const uint32_t smem0 = smem_addr(smem) >> 4;
+      for (int it = 0; it < nkb; ++it) {
+        const int s = it % args.stages;
+        const uint32_t phase = static_cast<uint32_t>(it / args.stages) & 1u;
+        // `full` follows `loaded` (and `digits`) in the scale writers, which have
+        // waited for both.
+        if (!wait_or_abort(&loaded[s], phase, &abort_flag, args.status)) break;
+        if (XMODE == kXInline && !wait_or_abort(&digits[s], phase, &abort_flag, args.status)) break;
+        if (!wait_or_abort(&full[s], phase, &abort_flag, args.status)) break;
+        tc_fence_after();
+        const uint32_t w_lo = smem0 + static_cast<uint32_t>(s * args.stage_bytes >> 4);
+        const uint32_t x_lo = w_lo + (kWBytes >> 4);
+        const uint32_t sf = tsf + static_cast<uint32_t>(s * kSfStageCols);
+#pragma unroll
+        for (int k = 0; k < kStepsPerBlock; ++k)
+          mma_mxf4(tbase, desc_const | (w_lo + static_cast<uint32_t>(k * 2)),
+                   desc_const | (x_lo + static_cast<uint32_t>(k * 2)), sf_idesc(args.idesc, k),
+                   (it | k) != 0, sf_cols_a(sf, k), sf_cols_b(sf, k));
+        tc_commit(&empty[s]);
+      }
+      // After an abort too, nothing this thread issued runs on.
+      tc_commit(&acc_full);
+      if (!mbar_wait(&acc_full, 0)) {
+        abort_flag = 1;
+        report_status(args.status, TCB_ERR_TIMEOUT);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    // ------------------------------------------------------ scale writers
+    const uint32_t lane_base = tsf + ((32u * (warp & 3)) << 16);
+    for (int it = 0; it < nkb; ++it) {
+      const int s = it % args.stages;
+      const uint32_t phase = static_cast<uint32_t>(it / args.stages) & 1u;
+      bool ok = wait_or_abort(&loaded[s], phase, &abort_flag, args.status);
+      if (XMODE == kXInline) ok = ok && wait_or_abort(&digits[s], phase, &abort_flag, args.status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;  // tcgen05.st needs the whole warp
+      const uint8_t* sw = smem + s * args.stage_bytes + kWBytes + x_bytes + lane * 16;
+      gemm_detail::write_scale_block(lane_base + static_cast<uint32_t>(s * kSfStageCols), sw,
+                                     sw + kScaleBlock, sw + sx_blocks * kScaleBlock);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+    }
+  } else if (XMODE == kXInline) {
     // -------------------------------------------------------------- X warps
-    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-      const int s = it % R::kStages;
-      if (!__all_sync(0xFFFFFFFFu, wait_or_abort(&loaded[s], static_cast<uint32_t>(it / R::kStages) & 1u,
-                                                 &abort_flag, args.status)))
-        break;
-      uint8_t* x = smem + s * R::kStageBytes + kWBytes + kScaleBytes;
-      uint4* chunks = reinterpret_cast<uint4*>(x);
-      float* factors = reinterpret_cast<float*>(x + R::kXBytes + R::kRawBytes);
-#pragma unroll 4
-      for (int token = warp - kProducerWarp - 1; token < R::kTokens; token += kXWarps) {
-        uint32_t h[4];
-        if constexpr (XT == kRowsMx) {
-          const uint8_t* raw = x + R::kXBytes;
-          decode8(reinterpret_cast<const uint32_t*>(raw + token * (kBlockK / 2))[lane], h);
-          if (lane < 8) {
-            const int r = (token0 + token) & 127;
-            factors[token * 8 + lane] = scale_value(
-                raw[R::kTokens * kBlockK / 2 + (lane >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (lane & 3)]);
-          }
-        } else {
-          uint32_t w[4];
-          if (args.x_tma) {
-            const uint4 q = chunks[token * 32 + lane];
-            w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
-          } else {
-            const uint16_t* src = static_cast<const uint16_t*>(args.x) +
-                                  static_cast<long long>(token0 + token) * args.ldx;
-            const int k = kb * kBlockK + lane * 8;
-            const bool in = token0 + token < args.m;
+    // One warp a stage: digit d of token i is row 8 i + d of the X tile, whose
+    // 16-byte chunk c lies at c ^ d (the 128-byte swizzle).
+    for (int it = warp - 6; it < nkb; it += kXWarps) {
+      const int s = it % args.stages;
+      const bool ok = wait_or_abort(&empty[s], (static_cast<uint32_t>(it / args.stages) & 1u) ^ 1u,
+                                    &abort_flag, args.status);
+      if (!__all_sync(0xFFFFFFFFu, ok)) break;
+      uint8_t* xt = smem + s * args.stage_bytes + kWBytes;
+      uint8_t* sx = xt + x_bytes + kScaleBlock;
+      uint4 x_now[kInlineTokens];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t lo = in && k + 2 * i < args.k ? src[k + 2 * i] : 0u;
-              const uint32_t hi = in && k + 2 * i + 1 < args.k ? src[k + 2 * i + 1] : 0u;
-              w[i] = lo | hi << 16;
-            }
-          }
-          const float factor = x_fragment<XT>(w, h);
-          if (lane == 0) factors[token] = factor;
-          __syncwarp();  // every lane has read its chunk before any is overwritten
+      for (int i = 0; i < kInlineTokens; ++i) x_now[i] = x_next[i];
+#pragma unroll
+      for (int token = 0; token < kInlineTokens; ++token) {
+        if (token >= tokens) break;
+        float u[8];
+        bool odd;
+        to_values(x_now[token], args.x_bf16, u, &odd);
+        const int e8 = digit_scale(u);
+        const float inv = inverse_scale(static_cast<uint32_t>(e8));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] *= inv;
+        const int group = lane >> 2;
+#pragma unroll
+        for (int d = 0; d < kDigits; ++d) {
+          const int row = token * kDigits + d;
+          const int code = e8 - kDigitBits * d;
+          const uint32_t w = next_digit(u);
+          *reinterpret_cast<uint32_t*>(xt + row * kBlockBytes + ((group ^ d) << 4) + (lane & 3) * 4) =
+              code >= 0 ? w : 0u;
+          if ((lane & 3) == 0)
+            sx[(group >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (group & 3)] =
+                digit_code(code, d, odd);
         }
-        chunks[x_chunk(token, lane)] = make_uint4(h[0], h[1], h[2], h[3]);
       }
-      fence_proxy_async_smem();  // the ring's next TMA load of these bytes comes after them
+      fence_proxy_async_smem();  // the MMA reads the tile through the async proxy
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ready[s]);
-    }
-  } else {
-    // ------------------------------------------------------------ consumers
-    const int g = lane >> 2, t = lane & 3;
-    const int r = warp * 16 + g;  // this lane's rows of the tile: r and r + 8
-    for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
-      const int s = it % R::kStages;
-      const uint32_t phase = static_cast<uint32_t>(it / R::kStages) & 1u;
-      if (!__all_sync(0xFFFFFFFFu, wait_or_abort(&loaded[s], phase, &abort_flag, args.status) &&
-                                       wait_or_abort(&ready[s], phase, &abort_flag, args.status)))
-        break;
-      const uint8_t* stage = smem + s * R::kStageBytes;
-      const uint8_t* wa = stage + r * 128 + 4 * t;
-      const uint8_t* sc = stage + kWBytes + (r & 31) * 16 + (r >> 5) * 4;
-      const uint4* chunks = reinterpret_cast<const uint4*>(stage + kWBytes + kScaleBytes);
-      const float* factors = reinterpret_cast<const float*>(stage + kWBytes + kScaleBytes + R::kXBytes +
-                                                            R::kRawBytes);
-      float block[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) block[n][i] = 0.0f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(sc + half * 512);
-        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(sc + half * 512 + 8 * 16);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int j = half * 4 + q;
-          uint32_t h0[4], h1[4];
-          decode8(*reinterpret_cast<const uint32_t*>(wa + ((j ^ g) << 4)), h0);
-          decode8(*reinterpret_cast<const uint32_t*>(wa + 8 * 128 + ((j ^ g) << 4)), h1);
-          const float f0 = scale_value((s0 >> (8 * q)) & 255u);
-          const float f1 = scale_value((s1 >> (8 * q)) & 255u);
-          const uint32_t a0[4] = {h0[0], h1[0], h0[1], h1[1]};
-          const uint32_t a1[4] = {h0[2], h1[2], h0[3], h1[3]};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint4 b = chunks[x_chunk(8 * n + g, 4 * j + t)];
-            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            float d[4];
-            mma_f16(d, a0, b.x, b.y, zero);
-            mma_f16(d, a1, b.z, b.w, d);
-            if constexpr (XT == kRowsMx) {
-              const float x0 = factors[(8 * n + 2 * t) * 8 + j];
-              const float x1 = factors[(8 * n + 2 * t + 1) * 8 + j];
-              total[n][0] = fmaf(d[0] * f0, x0, total[n][0]);
-              total[n][1] = fmaf(d[1] * f0, x1, total[n][1]);
-              total[n][2] = fmaf(d[2] * f1, x0, total[n][2]);
-              total[n][3] = fmaf(d[3] * f1, x1, total[n][3]);
-            } else {
-              block[n][0] = fmaf(d[0], f0, block[n][0]);
-              block[n][1] = fmaf(d[1], f0, block[n][1]);
-              block[n][2] = fmaf(d[2], f1, block[n][2]);
-              block[n][3] = fmaf(d[3], f1, block[n][3]);
-            }
-          }
-        }
-      }
-      if constexpr (XT != kRowsMx) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float2 x = *reinterpret_cast<const float2*>(factors + 8 * n + 2 * t);
-          total[n][0] = fmaf(block[n][0], x.x, total[n][0]);
-          total[n][1] = fmaf(block[n][1], x.y, total[n][1]);
-          total[n][2] = fmaf(block[n][2], x.x, total[n][2]);
-          total[n][3] = fmaf(block[n][3], x.y, total[n][3]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      if (lane == 0) mbar_arrive(&digits[s]);
+      ask_x(it + kXWarps);  // after the fence, which waits for loads in flight too
     }
   }
+  __syncthreads();  // the abort flag is final and the ring is free
 
-  // Partial sums [token][row] where the ring was: every load has landed and
-  // been read (after an abort the output is void and nothing is stored).
-  __syncthreads();
-  if (abort_flag) {
-    cluster_sync_all();
-    cluster_sync_all();
-    return;
-  }
-  float* partial = reinterpret_cast<float*>(smem);
-  if (warp < kConsumerWarps) {
-    const int g = lane >> 2, t = lane & 3, r = warp * 16 + g;
+  const bool aborted = abort_flag != 0;
+  // Row r of the tile belongs to the cluster's rank r / share; the sums of its
+  // rows lie in that CTA as [rank of origin][token][r % share].
+  const int share = (kRowTile + args.split - 1) / args.split;
+  const bool early = tokens <= kEarlyTokens;
+  float* sums = reinterpret_cast<float*>(smem + (early ? args.stages * args.stage_bytes : 0));
+  if (!early) cluster_sync_all();
+  if (!aborted && warp >= 2 && warp < 6) {
+    tc_fence_after();
+    const int row = 32 * (warp & 3) + lane;
+    const uint32_t taddr = tbase + ((32u * (warp & 3)) << 16);
+    const int owner = row / share;
+    const uint32_t to =
+        mapa_shared(smem_addr(sums + rank * tokens * share + (row - owner * share)), owner);
+    auto send = [&](int token, float v) {
+      st_shared_cluster_f32(to + static_cast<uint32_t>(token * share * 4), v);
+    };
+    for (int c = 0; c < tokens * kPerToken; c += 8) {
+      float r[8];
+      tmem_ld_8cols(taddr + static_cast<uint32_t>(c), r);
+      tmem_wait_ld();
+      if constexpr (XMODE == kXRows) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float* p = partial + (8 * n + 2 * t) * kPartialPitch + r;
-      p[0] = total[n][0];
-      p[kPartialPitch] = total[n][1];
-      p[8] = total[n][2];
-      p[kPartialPitch + 8] = total[n][3];
+        for (int i = 0; i < 8; ++i)
+          if (c + i < tokens) send(c + i, r[i]);
+      } else {
+        const int token = c / kDigits;
+        const bool odd = isnan(r[kDigits - 1]);  // infinities or NaN in x (or a NaN scale in w)
+        float sum = odd ? 0.0f : r[kDigits - 1];
+#pragma unroll
+        for (int d = kDigits - 2; d >= 0; --d) sum += r[d];
+        const long long n = static_cast<long long>(tile) * kRowTile + row;
+        if (odd && n < args.n) {
+          const uint16_t* x = static_cast<const uint16_t*>(args.x) + (token0 + token) * args.ldx;
+          const int end = static_cast<int>(min(static_cast<long long>(kb1) * kBlockK,
+                                               static_cast<long long>(args.k)));
+          for (int k = kb0 * kBlockK; k < end; ++k) {
+            const float v = value16(x[k], args.x_bf16);
+            if ((__float_as_uint(v) & 0x7FFFFFFFu) < 0x7F800000u) continue;
+            const uint32_t code = args.w[n * args.pitch + k / 2] >> (4 * (k & 1)) & 15u;
+            const int group = k / 32;
+            const uint32_t e8 = args.sw[(static_cast<long long>(tile) * args.kblocks + group / 8) * kScaleBlock +
+                                        (group % 8 / 4) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (group & 3)];
+            sum += v * (decode1(code) * scale_value(e8));
+          }
+        }
+        send(token, sum);
+      }
     }
-  }
-  cluster_sync_all();
-  const int tokens = min(R::kTokens, args.m - token0);
-  const uint32_t base = smem_addr(partial);
-  // Output i = (token, row) belongs to rank i / kRowsThreads mod split.
-  for (int i = rank * kRowsThreads + threadIdx.x; i < tokens * kRowTile;
-       i += args.split * kRowsThreads) {
-    const int token = i / kRowTile, row = i % kRowTile;
-    const long long n = static_cast<long long>(tile) * kRowTile + row;
-    if (n >= args.n) continue;
-    const uint32_t at = base + static_cast<uint32_t>((token * kPartialPitch + row) * 4);
-    float sum = 0.0f;
-    for (int q = 0; q < args.split; ++q) sum += ld_shared_cluster_f32(mapa_shared(at, q));
-    const long long out = (token0 + token) * args.ldy + n;
-    if (args.y_type == kRowsFp32) {
-      if (args.bias) sum += static_cast<const float*>(args.bias)[n];
-      static_cast<float*>(args.y)[out] = sum;
-    } else if (args.y_type == kRowsBf16) {
-      if (args.bias) sum += to_float(static_cast<const __nv_bfloat16*>(args.bias)[n]);
-      static_cast<__nv_bfloat16*>(args.y)[out] = from_float<__nv_bfloat16>(sum);
-    } else {
-      if (args.bias) sum += to_float(static_cast<const __half*>(args.bias)[n]);
-      static_cast<__half*>(args.y)[out] = from_float<__half>(sum);
-    }
+    tc_fence_before();
   }
   __syncthreads();
-  cluster_sync_all();  // no CTA leaves while a peer may still read its partial sums
+  cluster_sync_all();
+  if (!aborted) {
+    const long long n0 = static_cast<long long>(tile) * kRowTile + rank * share;
+    const int rows = static_cast<int>(min(static_cast<long long>(min(share, kRowTile - rank * share)),
+                                          args.n - n0));
+    constexpr int kWarps = 6 + (XMODE == kXInline ? kXWarps : 0);
+    const Finish f{sums, args.split, tokens, share, rows, warp, kWarps, lane};
+    const long long at = token0 * args.ldy + n0;
+    if (args.y_type == kRowsFp32)
+      f.run(static_cast<const float*>(args.bias), n0, static_cast<float*>(args.y) + at, args.ldy);
+    else if (args.y_type == kRowsBf16)
+      f.run(static_cast<const __nv_bfloat16*>(args.bias), n0, static_cast<__nv_bfloat16*>(args.y) + at,
+            args.ldy);
+    else
+      f.run(static_cast<const __half*>(args.bias), n0, static_cast<__half*>(args.y) + at, args.ldy);
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, args.tmem_cols);
+  }
 }
 
-// 2-D map of 128 rows of codes in the 128-byte swizzle (W), or of the X tile.
-int rows_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long inner,
-             long long rows, long long pitch_bytes, int box_inner, int box_rows,
-             CUtensorMapSwizzle swizzle) {
+// Codes [rows][pitch bytes] as boxes of box_rows x 128 bytes in the 128-byte swizzle.
+int rows_map(CUtensorMap* map, const void* base, long long rows, long long pitch, int box_rows) {
   auto fn = tensor_map_encoder();
   if (fn == nullptr) return TCB_ERR_DEVICE;
-  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(rows)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch_bytes)};
-  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_rows)};
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(kBlockBytes), static_cast<cuuint32_t>(box_rows)};
   cuuint32_t estr[2] = {1, 1};
-  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? TCB_OK
              : TCB_ERR_INVALID_ARGUMENT;
 }
 
-template <int XT, int NT>
-int launch_rows(const RowsProblem& p, int* status, const DeviceFacts& facts, cudaStream_t stream) {
-  using R = Rows<XT, NT>;
-  const long long kp = mx_padded(p.k);
-  RowsArgs args;
-  args.sw = static_cast<const uint8_t*>(p.sw);
-  args.sx = static_cast<const uint8_t*>(p.sx);
-  args.x = p.x;
-  args.bias = p.bias;
-  args.y = p.y;
-  args.ldx = p.ldx;
-  args.ldy = p.ldy;
-  args.status = status;
-  args.m = p.m;
-  args.n = p.n;
-  args.k = p.k;
-  args.kblocks = static_cast<int>((kp + kBlockK - 1) / kBlockK);
-  args.y_type = p.y_type;
-  CUtensorMap map_w, map_x{};
-  int rc = rows_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, kp / 2, p.n, kp / 2, kBlockK / 2,
-                    kRowTile, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (rc != TCB_OK) return rc;
-  if (XT == kRowsMx) {
-    args.x_tma = 1;
-    rc = rows_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, kp / 2, p.m, kp / 2, kBlockK / 2,
-                  R::kTokens, CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (rc != TCB_OK) return rc;
-  } else {
-    // TMA wants 16-byte rows; other rows are read by the X warps.
-    args.x_tma = aligned(p.x, 16) && p.ldx % 8 == 0 &&
-                 rows_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.x, p.k, p.m, p.ldx * 2, kBlockK,
-                          R::kTokens, CU_TENSOR_MAP_SWIZZLE_NONE) == TCB_OK;
+// The workspace of mx_rows_run for 16-bit rows: [scales][codes] of their digits.
+struct DigitSpace {
+  long long tiles, codes_at, bytes;  // column tiles
+  int per_tile;                      // tokens of a column tile
+  DigitSpace(long long m, long long k) {
+    constexpr int kMost = kDigitRows / kDigits;
+    tiles = (m + kMost - 1) / kMost;
+    per_tile = static_cast<int>((m + tiles - 1) / tiles);
+    const long long kblocks = (mx_padded(k) + kBlockK - 1) / kBlockK;
+    codes_at = (tiles + 1) / 2 * 2 * kScaleBlock * kblocks;
+    bytes = m <= kInlineTokens ? 0 : codes_at + tiles * kDigitRows * (mx_padded(k) / 2);
   }
-  const long long tiles = (static_cast<long long>(p.n) + kRowTile - 1) / kRowTile;
-  const long long chunks = (static_cast<long long>(p.m) + R::kTokens - 1) / R::kTokens;
-  // As many CTAs of a row tile as fit beside the other tiles in one round of
-  // the SMs, each with at least one K block.
-  long long split = static_cast<long long>(facts.sm_count) * R::kCtas / (tiles * chunks);
+};
+
+template <int XMODE>
+int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, long long chunks,
+                const DeviceFacts& facts, cudaStream_t stream) {
+  const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile;
+  args.stage_bytes = kWBytes + args.cols * kBlockBytes + (args.cols > 128 ? 3 : 2) * kScaleBlock;
+  const bool paired = args.cols <= kPairedCols;
+  constexpr int kSumBytes = kEarlyTokens * (kRowTile + kMaxSplit) * 4;  // a share is rounded up
+  args.stages = ((paired ? kPairedSmem : kAloneSmem) - 1024 - kSumBytes) / args.stage_bytes;
+  if (args.stages > kMaxStages) args.stages = kMaxStages;
+  // Two CTAs of an SM get half of its tensor memory each.
+  args.tmem_cols = paired ? 256 : 512;
+  const int acc_cols = (args.cols + 31) / 32 * 32;
+  while (acc_cols + args.stages * kSfStageCols > args.tmem_cols) --args.stages;
+  const int smem = args.stages * args.stage_bytes + kSumBytes + 1024;
+  long long split = static_cast<long long>(facts.sm_count) * (paired ? 2 : 1) / (tiles * chunks);
   split = split > kMaxSplit ? kMaxSplit : split;
   split = split > args.kblocks ? args.kblocks : split;
   args.split = split < 1 ? 1 : static_cast<int>(split);
   if (tiles * args.split > INT_MAX || chunks > 65535) return TCB_ERR_RESOURCE;
-  auto fn = mx_rows_kernel<XT, NT>;
+  // N of the instruction; M = 128, E2M1 x E2M1, E8M0 scales as the pair MMA.
+  args.idesc = (gemm_pair_idesc() & ~(0x3Fu << 17 | 0x1Fu << 24)) |
+               static_cast<uint32_t>(args.cols >> 3) << 17 | static_cast<uint32_t>(kRowTile >> 4) << 24;
+  auto fn = mx_rows_kernel<XMODE>;
   static DeviceIntCache cap_cache;
   const int cap = cap_cache.get(facts.device, [&] {
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
-  if (cap < R::kSmem) return TCB_ERR_RESOURCE;
+  if (cap < smem) return TCB_ERR_RESOURCE;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(tiles * args.split), static_cast<unsigned>(chunks), 1);
-  config.blockDim = dim3(kRowsThreads, 1, 1);
-  config.dynamicSmemBytes = R::kSmem;
+  config.blockDim = dim3((6 + (XMODE == kXInline ? kXWarps : 0)) * 32, 1, 1);
+  config.dynamicSmemBytes = static_cast<size_t>(smem);
   config.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(args.split);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
-  config.numAttrs = 1;
+  config.numAttrs = XMODE == kXDigits ? 2 : 1;
   clear_stale_error();
   if (cudaLaunchKernelEx(&config, fn, map_w, map_x, args) != cudaSuccess) {
     clear_stale_error();
@@ -468,23 +631,55 @@ int launch_rows(const RowsProblem& p, int* status, const DeviceFacts& facts, cud
   return TCB_OK;
 }
 
-template <int XT>
-int run_tokens(const RowsProblem& p, int* status, const DeviceFacts& facts, cudaStream_t stream) {
-  if (p.m <= 8) return launch_rows<XT, 1>(p, status, facts, stream);
-  if (p.m <= 16) return launch_rows<XT, 2>(p, status, facts, stream);
-  if (p.m <= 32) return launch_rows<XT, 4>(p, status, facts, stream);
-  return launch_rows<XT, 8>(p, status, facts, stream);
-}
-
 }  // namespace
 
-int mx_rows_run(const RowsProblem& p, int* status, const DeviceFacts& facts, cudaStream_t stream) {
-  switch (p.x_type) {
-    case kRowsBf16: return run_tokens<kRowsBf16>(p, status, facts, stream);
-    case kRowsFp16: return run_tokens<kRowsFp16>(p, status, facts, stream);
-    case kRowsMx: return run_tokens<kRowsMx>(p, status, facts, stream);
+long long mx_rows_workspace(long long m, long long k) { return DigitSpace(m, k).bytes; }
+
+int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const DeviceFacts& facts,
+                cudaStream_t stream) {
+  RowsArgs args = {};
+  args.sw = static_cast<const uint8_t*>(p.sw);
+  args.sx = static_cast<const uint8_t*>(p.sx);
+  args.w = static_cast<const uint8_t*>(p.w);
+  args.x = p.x;
+  args.bias = p.bias;
+  args.y = p.y;
+  args.pitch = mx_padded(p.k) / 2;
+  args.ldx = p.ldx;
+  args.ldy = p.ldy;
+  args.status = status;
+  args.m = p.m;
+  args.n = p.n;
+  args.k = p.k;
+  args.kblocks = static_cast<int>((args.pitch + kBlockBytes - 1) / kBlockBytes);
+  args.x_bf16 = p.x_type == kRowsBf16;
+  args.y_type = p.y_type;
+  CUtensorMap map_w, map_x{};
+  int rc = rows_map(&map_w, p.w, p.n, args.pitch, kRowTile);
+  if (rc != TCB_OK) return rc;
+  if (p.x_type == kRowsMx) {
+    args.cols = p.m > kMaxCols ? kMaxCols : (p.m + 7) / 8 * 8;
+    if ((rc = rows_map(&map_x, p.x, p.m, args.pitch, args.cols)) != TCB_OK) return rc;
+    return launch_rows<kXRows>(map_w, map_x, args, (p.m + args.cols - 1) / args.cols, facts, stream);
   }
-  return TCB_ERR_UNSUPPORTED;
+  if (p.m <= kInlineTokens) {
+    args.cols = p.m * kDigits;
+    return launch_rows<kXInline>(map_w, map_x, args, 1, facts, stream);
+  }
+  const DigitSpace space(p.m, p.k);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  args.sx = base;
+  args.cols = space.per_tile * kDigits;
+  if ((rc = rows_map(&map_x, base + space.codes_at, space.tiles * kDigitRows, args.pitch, args.cols)) != TCB_OK)
+    return rc;
+  const long long warps = static_cast<long long>(p.m) * args.kblocks;
+  if ((warps + 7) / 8 > INT_MAX) return TCB_ERR_RESOURCE;
+  clear_stale_error();
+  mx_digits_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(
+      static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, args.pitch, args.kblocks, space.per_tile,
+      aligned(p.x, 16) && p.ldx % 8 == 0, args.x_bf16, base + space.codes_at, base);
+  if ((rc = launch_status()) != TCB_OK) return rc;
+  return launch_rows<kXDigits>(map_w, map_x, args, space.tiles, facts, stream);
 }
 
 }  // namespace tcb

@@ -21,6 +21,10 @@ struct RowsProblem {
   int x_type, y_type;
 };
 
-int mx_rows_run(const RowsProblem& p, int* status, const DeviceFacts& facts, cudaStream_t stream);
+// Bytes of workspace that mx_rows_run needs for m 16-bit rows of k values (MX
+// rows need none).
+long long mx_rows_workspace(long long m, long long k);
+int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const DeviceFacts& facts,
+                cudaStream_t stream);
 
 }  // namespace tcb

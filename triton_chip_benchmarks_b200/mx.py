@@ -272,7 +272,7 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
            dtype: torch.dtype | None = None, out: torch.Tensor | None = None, status=None) -> torch.Tensor:
     """x [..., K] . w [N][K]^T (+ bias [N]) with bf16 or fp16 x, in `dtype` (default x's).
 
-    Only the weight is rounded to MX FP4.  Meant for few rows: w is read once per 64
+    Only the weight is rounded to MX FP4.  Meant for few rows: w is read once per 16
     rows of x (for many rows quantise x too and take :func:`matmul`).  ``out`` is a
     matrix [rows][N].
     """
@@ -292,9 +292,11 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
     y = _output(out, m.device, m.shape[0], w.rows, x.dtype if dtype is None else dtype)
     bias_ptr = _bias(bias, w.rows, y)
     if m.shape[0] and w.rows:
+        need = _native.mx_linear_workspace_bytes(m.shape[0], w.cols)
+        space = torch.empty(need, dtype=torch.uint8, device=m.device) if need else None
         _call("tcb_mx_linear", m.device, _DTYPES[x.dtype], m.data_ptr(), pitch, w.codes_ptr,
               w.scales_ptr, bias_ptr, _DTYPES[y.dtype], y.data_ptr(), _pitch(y), m.shape[0], w.rows,
-              w.cols, _native._ptr(status))
+              w.cols, _native._ptr(space), need, _native._ptr(status))
     return y if out is not None or len(lead) == 1 else y.view(*lead, w.rows)
 
 
