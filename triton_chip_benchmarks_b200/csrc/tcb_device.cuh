@@ -75,6 +75,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   return true;
 }
 
+// Programmatic dependent launch.  A kernel launched with the attribute may start
+// while the kernels before it in the stream still run: it waits for them (and
+// their memory) here, before it touches global memory.  A no-op otherwise.
+__device__ __forceinline__ void wait_for_previous_kernels() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Lets the next kernel in the stream start (it waits as above).  Called once the
+// CTA holds all that it allocates: a waiting kernel must not take it away.
+__device__ __forceinline__ void let_next_kernel_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // Generic-proxy shared-memory writes become visible to the async proxy
 // (TMA stores, tcgen05.mma operand reads) only after this fence.
 __device__ __forceinline__ void fence_proxy_async_smem() {

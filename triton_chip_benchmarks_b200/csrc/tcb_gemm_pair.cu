@@ -284,6 +284,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   tc_fence_before();
   cluster_sync_all();  // both CTAs' barriers initialised and tensor memory allocated
   tc_fence_after();
+  let_next_kernel_start();
+  wait_for_previous_kernels();
   const uint32_t tbase = tmem_slot;
   // An abort on either CTA stops both: a wait that fails also raises the
   // peer's flag (a store into its shared memory, which stays valid until the
@@ -689,6 +691,9 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
   if (pairs < 1) pairs = 1;
   if (pairs > tiles) pairs = tiles;
   if (pairs > resident) pairs = resident;
+  if (p.overlap)
+    return launch_overlapping(fn, dim3(static_cast<unsigned>(2 * pairs)), kPairThreads, kPairSmem, 1, stream,
+                              map_a, map_b, map_a3, map_b3, map_c, args);
   clear_stale_error();
   fn<<<2 * pairs, kPairThreads, kPairSmem, stream>>>(map_a, map_b, map_a3, map_b3, map_c, args);
   return launch_status();

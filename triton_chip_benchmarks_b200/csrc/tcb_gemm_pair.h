@@ -22,6 +22,7 @@ struct PairProblem {
   int m, n, k;       // k a multiple of 32
   int out;           // PairOutType
   uint32_t idesc;
+  bool overlap;      // may start while the kernels before it still run (launch_overlapping)
 };
 
 int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFacts& facts,

@@ -33,6 +33,34 @@ inline int launch_status() {
   return err == cudaSuccess ? TCB_OK : TCB_ERR_LAUNCH;
 }
 
+// Launch `fn` so that it may start (and set itself up) while the kernels before
+// it in the stream still run; `fn` waits for them before it touches global
+// memory.  cluster: CTAs of a cluster along x (1: none).
+template <typename... Params, typename... Args>
+int launch_overlapping(void (*fn)(Params...), dim3 grid, int threads, size_t smem, int cluster,
+                       cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  config.attrs = attr;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  clear_stale_error();
+  if (cudaLaunchKernelEx(&config, fn, args...) != cudaSuccess) {
+    clear_stale_error();
+    return TCB_ERR_LAUNCH;
+  }
+  return TCB_OK;
+}
+
 // Allow `fn` the device's opt-in shared memory minus its static shared
 // memory; returns the dynamic bytes a launch may request, or -1.
 inline int raise_dynamic_smem(const void* fn, int max_optin) {

@@ -129,6 +129,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
   const int col = lane_col * kVec;
   const int row = tid / kLanesPerRow;
   const T* x = static_cast<const T*>(args.x);
+  let_next_kernel_start();
+  wait_for_previous_kernels();
 
   uint4 raw[kPasses][kChunks];
   if constexpr (VEC) {
@@ -298,9 +300,8 @@ int launch_quantize(const QuantArgs& args, long long tiles, const DeviceFacts& f
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
   if (cap < smem) return TCB_ERR_RESOURCE;
-  clear_stale_error();
-  fn<<<static_cast<unsigned>(tiles), kThreads, smem, stream>>>(args);
-  return launch_status();
+  return launch_overlapping(fn, dim3(static_cast<unsigned>(tiles)), kThreads, static_cast<size_t>(smem), 1,
+                            stream, args);
 }
 
 template <typename T>
@@ -350,6 +351,8 @@ __global__ void __launch_bounds__(kThreads)
   const long long left = args.cols - c0 - col;
   const int valid = left <= 0 ? 0 : left >= kDeqVec ? kDeqVec : static_cast<int>(left);
   uint32_t w[kDeqPasses];
+  let_next_kernel_start();
+  wait_for_previous_kernels();
   if constexpr (VEC) {
 #pragma unroll
     for (int p = 0; p < kDeqPasses; ++p) {
@@ -419,10 +422,8 @@ int launch_dequantize(const DequantArgs& args, cudaStream_t stream) {
   const bool vec = aligned(args.y, 16) && args.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const long long tiles = args.tiles_x * ((args.rows + kTile - 1) / kTile);
   if (tiles > INT_MAX) return TCB_ERR_RESOURCE;
-  clear_stale_error();
-  (vec ? dequantize_kernel<T, true> : dequantize_kernel<T, false>)<<<
-      static_cast<unsigned>(tiles), kThreads, 0, stream>>>(args);
-  return launch_status();
+  return launch_overlapping(vec ? dequantize_kernel<T, true> : dequantize_kernel<T, false>,
+                            dim3(static_cast<unsigned>(tiles)), kThreads, 0, 1, stream, args);
 }
 
 }  // namespace

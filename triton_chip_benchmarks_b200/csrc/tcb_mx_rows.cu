@@ -25,7 +25,7 @@
 // Where the digits come from.  Up to kInlineTokens rows, X warps of each CTA write
 // the digits of its K slice into shared memory on the way; for more rows a
 // kernel of their own writes them once (into the caller's workspace), and the
-// product starts beside it (programmatic dependent launch): its weight loads
+// product starts beside it: its weight loads
 // are under way before the digits are there.
 //
 // Split over K.  With fewer row tiles than CTAs fit, up to eight CTAs of a
@@ -134,15 +134,6 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
-// Returns once the kernel launched before this one has finished (at once where
-// nothing was launched to overlap).
-__device__ __forceinline__ void wait_for_previous_kernel() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void let_next_kernel_start() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 __device__ __forceinline__ float value16(uint16_t bits, bool bf16) {
   return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
               : __half2float(__ushort_as_half(bits));
@@ -215,6 +206,9 @@ __global__ void __launch_bounds__(256)
     mx_digits_kernel(const uint16_t* __restrict__ x, long long ldx, int m, int k, long long pitch,
                      int kblocks, int per_tile, int vec, int bf16, uint8_t* __restrict__ codes,
                      uint8_t* __restrict__ scales) {
+  // The product may start once the kernels before this one are done: its weight
+  // may be theirs.
+  wait_for_previous_kernels();
   let_next_kernel_start();
   const int lane = threadIdx.x & 31;
   const long long task = static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
@@ -333,7 +327,10 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
                                 (kb0 + it) * kBlockK + lane * 8, args.k, vec);
   };
   if constexpr (XMODE == kXInline) {
-    if (warp >= 6) ask_x(warp - 6);
+    if (warp >= 6) {
+      wait_for_previous_kernels();
+      ask_x(warp - 6);
+    }
   }
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
@@ -347,7 +344,9 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     mbar_init(&acc_full, 1);
     abort_flag = 0;
     fence_mbar_init();
-    // The first round of loads goes out before anything else is set up.
+    // The first round of loads goes out before anything else is set up.  (The
+    // digits' kernel has waited for the kernels before it.)
+    if (XMODE != kXDigits) wait_for_previous_kernels();
     for (int it = 0; it < min(nkb, args.stages); ++it) {
       load_w(it);
       if constexpr (XMODE == kXRows) load_x(it);
@@ -360,6 +359,8 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  let_next_kernel_start();
+  wait_for_previous_kernels();
   const uint32_t tbase = tmem_slot;
   const uint32_t tsf = tbase + static_cast<uint32_t>((args.cols + 31) & ~31);
 
@@ -368,7 +369,6 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     if (lane == 0) {
       int it = min(nkb, args.stages);
       if constexpr (XMODE == kXDigits) {
-        wait_for_previous_kernel();
         for (int j = 0; j < it; ++j) load_x(j);
       }
       for (; it < nkb; ++it) {
@@ -609,26 +609,9 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
   if (cap < smem) return TCB_ERR_RESOURCE;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(tiles * args.split), static_cast<unsigned>(chunks), 1);
-  config.blockDim = dim3((6 + (XMODE == kXInline ? kXWarps : 0)) * 32, 1, 1);
-  config.dynamicSmemBytes = static_cast<size_t>(smem);
-  config.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(args.split);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = XMODE == kXDigits ? 2 : 1;
-  clear_stale_error();
-  if (cudaLaunchKernelEx(&config, fn, map_w, map_x, args) != cudaSuccess) {
-    clear_stale_error();
-    return TCB_ERR_LAUNCH;
-  }
-  return TCB_OK;
+  return launch_overlapping(fn, dim3(static_cast<unsigned>(tiles * args.split), static_cast<unsigned>(chunks)),
+                            (6 + (XMODE == kXInline ? kXWarps : 0)) * 32, static_cast<size_t>(smem),
+                            args.split, stream, map_w, map_x, args);
 }
 
 }  // namespace
@@ -674,11 +657,11 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
     return rc;
   const long long warps = static_cast<long long>(p.m) * args.kblocks;
   if ((warps + 7) / 8 > INT_MAX) return TCB_ERR_RESOURCE;
-  clear_stale_error();
-  mx_digits_kernel<<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(
-      static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, args.pitch, args.kblocks, space.per_tile,
-      aligned(p.x, 16) && p.ldx % 8 == 0, args.x_bf16, base + space.codes_at, base);
-  if ((rc = launch_status()) != TCB_OK) return rc;
+  rc = launch_overlapping(mx_digits_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, 1, stream,
+                          static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, args.pitch, args.kblocks,
+                          space.per_tile, static_cast<int>(aligned(p.x, 16) && p.ldx % 8 == 0),
+                          args.x_bf16, base + space.codes_at, base);
+  if (rc != TCB_OK) return rc;
   return launch_rows<kXDigits>(map_w, map_x, args, space.tiles, facts, stream);
 }
 
