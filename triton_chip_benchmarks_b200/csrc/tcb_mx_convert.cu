@@ -20,12 +20,14 @@
 // 8192 x 8192 bf16).  16-bit values stay packed for the search of the largest:
 // two a word, integer maxima of the magnitude bits.
 //
-// Both axes in one read.  The tile is kept in shared memory on its way through
-// the row pass, 16-byte chunks swizzled so that neither the row-wise stores
-// nor the column-wise loads conflict; a thread then takes 32 rows of one word
-// (two 16-bit columns, or one fp32) and the codes are turned round through
-// shared memory into 64-byte runs.  Rows that do not start on 16-byte
-// boundaries come through the same tile, element by element.
+// Both axes in one read.  The tile goes to shared memory with cp.async (zeros
+// past the edge), 16-byte chunks swizzled so that neither the row-wise nor the
+// column-wise loads conflict; a thread takes four times 16 values of a row, then
+// 32 rows of one word (two 16-bit columns, or one fp32), and the column codes
+// are turned round through shared memory into 64-byte runs.  (Loading through
+// registers held more of them and fewer CTAs: 23.5 us instead of TODO for
+// 8192 x 4096 bf16.)  Rows that do not start on 16-byte boundaries come through
+// the same tile, element by element.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -79,8 +81,15 @@ __device__ __forceinline__ uint4 load_edge(const T* __restrict__ p, int valid) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// 16 bytes global -> shared, of which the first `bytes` are read and the rest
+// are zeros.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes)
+               : "memory");
+}
+
 // Byte offset of 16-byte chunk c of a row of the tile in shared memory: the
-// eight lanes of a row write chunks 2l + j (fp32: 4l + j), which the swizzle
+// eight lanes of a row read chunks 2l + j (fp32: 4l + j), which the swizzle
 // spreads over all banks.
 template <typename T>
 __device__ __forceinline__ int tile_chunk(int row, int c) {
@@ -111,7 +120,7 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t magnitude) {
 }
 
 template <typename T, bool VEC, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : (COLS ? 5 : 4))
     quantize_kernel(const __grid_constant__ QuantArgs args) {
   constexpr bool kTiled = COLS || !VEC;
   constexpr int kChunks = kWords<T> / 4;  // 16-byte chunks of a thread's values
@@ -132,8 +141,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
   let_next_kernel_start();
   wait_for_previous_kernels();
 
-  uint4 raw[kPasses][kChunks];
-  if constexpr (VEC) {
+  // Rows alone: a thread's values straight into registers.
+  [[maybe_unused]] uint4 raw[kTiled ? 1 : kPasses][kChunks];
+  if constexpr (!kTiled) {
     if (r0 + kTile <= args.rows && c0 + kTile <= args.cols) {
       const T* p = x + (r0 + row) * args.ld + c0 + col;
 #pragma unroll
@@ -155,14 +165,21 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
         }
       }
     }
-    if constexpr (COLS) {
+  } else if constexpr (VEC) {
+    constexpr int kRowChunks = kTile * static_cast<int>(sizeof(T)) / 16;
+    constexpr int kStep = kThreads / kRowChunks;  // rows a round of loads covers
+    const int c = tid % kRowChunks;
+    const long long at = c0 + c * (16 / static_cast<int>(sizeof(T)));
+    const long long left = (args.cols - at) * static_cast<long long>(sizeof(T));
+    const int bytes = left <= 0 ? 0 : left >= 16 ? 16 : static_cast<int>(left);
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i)
-#pragma unroll
-        for (int q = 0; q < kChunks; ++q)
-          *reinterpret_cast<uint4*>(smem + tile_chunk<T>(row + i * kRowsPerPass,
-                                                         lane_col * kChunks + q)) = raw[i][q];
+    for (int i = 0; i < kTile / kStep; ++i) {
+      const int lr = tid / kRowChunks + i * kStep;
+      const bool in = bytes > 0 && r0 + lr < args.rows;
+      cp_async16(smem + tile_chunk<T>(lr, c), in ? x + (r0 + lr) * args.ld + at : x, in ? bytes : 0);
     }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
   } else {
     constexpr int kPer = 16 / sizeof(T);
 #pragma unroll 8
@@ -174,14 +191,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
       *reinterpret_cast<T*>(smem + tile_chunk<T>(r, c / kPer) + c % kPer * sizeof(T)) = v;
     }
     __syncthreads();
-    if constexpr (ROWS) {
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i)
-#pragma unroll
-        for (int q = 0; q < kChunks; ++q)
-          raw[i][q] = *reinterpret_cast<const uint4*>(
-              smem + tile_chunk<T>(row + i * kRowsPerPass, lane_col * kChunks + q));
-    }
   }
   if constexpr (ROWS) {
     const long long pitch = mx_padded(args.cols) / 2;
@@ -193,8 +202,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 4)
       uint32_t top = 0;
 #pragma unroll
       for (int q = 0; q < kChunks; ++q) {
-        w[4 * q] = raw[i][q].x, w[4 * q + 1] = raw[i][q].y;
-        w[4 * q + 2] = raw[i][q].z, w[4 * q + 3] = raw[i][q].w;
+        uint4 v;
+        if constexpr (kTiled)
+          v = *reinterpret_cast<const uint4*>(smem + tile_chunk<T>(lr, lane_col * kChunks + q));
+        else
+          v = raw[i][q];
+        w[4 * q] = v.x, w[4 * q + 1] = v.y, w[4 * q + 2] = v.z, w[4 * q + 3] = v.w;
       }
 #pragma unroll
       for (int q = 0; q < kWords<T>; ++q) top = top_of<T>(top, w[q]);
@@ -326,13 +339,16 @@ struct DequantArgs {
   void* y;
   long long rows, cols, ld;
   long long tiles_x;
+  int wide;  // fp32 rows start on 32-byte boundaries
 };
 
 // The same tiles the other way.  code * 2^e is exact in fp32 and is rounded
 // once to T.  VEC: a thread turns 4 code bytes of a row into 8 values, 16-byte
-// stores.  Otherwise rows of Y start anywhere, and a warp stores 32 values of a
-// row side by side (8 values a thread, element by element, took 42 us instead
-// of TODO for 2072 x 4099 fp32).
+// stores (fp32 rows on 32-byte boundaries: one 32-byte store; as two 16-byte
+// stores of half a sector each they took 13.6 us instead of TODO for 4099 x 2072).
+// Otherwise rows of Y start anywhere, and a warp stores 32 values of a row side
+// by side, their codes brought round by a shuffle (8 values a thread, element by
+// element, took 42 us instead of TODO for 2072 x 4099 fp32).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     dequantize_kernel(const __grid_constant__ DequantArgs args) {
@@ -385,8 +401,14 @@ __global__ void __launch_bounds__(kThreads)
       T* dst = static_cast<T*>(args.y) + r * args.ld + c0 + col;
       if (valid == kDeqVec) {
         if constexpr (sizeof(T) == 4) {
-          reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          if (args.wide) {
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "f"(v[0]),
+                         "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                         : "memory");
+          } else {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          }
         } else {
           *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
                                                       pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
@@ -398,27 +420,39 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
   } else {
+    // A lane's word i holds codes 8 (lane % 16).. of row 2 i + lane / 16 of the
+    // warp's 16.
+    constexpr int kRows = kTile / (kThreads / 32);
     const int warp = tid >> 5, lane = tid & 31;
-#pragma unroll 4
-    for (int lr = warp; lr < kTile; lr += kThreads / 32) {
+    uint32_t codes[kRows / 2];
+#pragma unroll
+    for (int i = 0; i < kRows / 2; ++i) {
+      const long long r = r0 + warp * kRows + 2 * i + (lane >> 4);
+      const long long at = c0 / 2 + (lane & 15) * 4;
+      codes[i] = r < args.rows && at < pitch
+                     ? __ldg(reinterpret_cast<const uint32_t*>(args.codes + r * pitch + at))
+                     : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int lr = warp * kRows + i;
       const long long r = r0 + lr;
-      if (r >= args.rows) break;
       const uint32_t scales = *reinterpret_cast<const uint32_t*>(s_scales + (lr & 31) * 16 + (lr >> 5) * 4);
-      const uint8_t* src = args.codes + r * pitch + c0 / 2;
       T* dst = static_cast<T*>(args.y) + r * args.ld + c0;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int c = 32 * g + lane;
-        if (c0 + c >= args.cols) break;
-        const uint32_t code = __ldg(src + c / 2) >> (4 * (lane & 1)) & 15u;
-        dst[c] = from_float<T>(decode1(code) * scale_value((scales >> (8 * g)) & 255u));
+        const uint32_t word = __shfl_sync(0xFFFFFFFFu, codes[i / 2], (i & 1) * 16 + 4 * g + (lane >> 3));
+        const float v = decode1(word >> (4 * (lane & 7)) & 15u) * scale_value((scales >> (8 * g)) & 255u);
+        if (r < args.rows && c0 + c < args.cols) dst[c] = from_float<T>(v);
       }
     }
   }
 }
 
 template <typename T>
-int launch_dequantize(const DequantArgs& args, cudaStream_t stream) {
+int launch_dequantize(DequantArgs args, cudaStream_t stream) {
+  args.wide = sizeof(T) == 4 && aligned(args.y, 32) && args.ld % 8 == 0;
   const bool vec = aligned(args.y, 16) && args.ld * static_cast<long long>(sizeof(T)) % 16 == 0;
   const long long tiles = args.tiles_x * ((args.rows + kTile - 1) / kTile);
   if (tiles > INT_MAX) return TCB_ERR_RESOURCE;

@@ -50,7 +50,7 @@ class MxTensor:
     cols), ``scales`` the E8M0 scales in the layout of ``tcb_mx_scales_pack``.
     """
 
-    __slots__ = ("rows", "cols", "device", "codes_ptr", "scales_ptr", "_held")
+    __slots__ = ("rows", "cols", "index", "codes_ptr", "scales_ptr", "_held")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -63,20 +63,20 @@ class MxTensor:
                              f"{_packed_bytes(rows, cols)} bytes, got {scales.numel()}")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("MX codes and scales are contiguous")
-        device = codes.device
-        if device != scales.device or not codes.is_cuda:
+        index = codes.get_device()
+        if index < 0 or index != scales.get_device():
             raise ValueError("MX codes and scales are on one CUDA device")
-        self.rows, self.cols, self.device = rows, cols, device
+        self.rows, self.cols, self.index = rows, cols, index
         self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
         self._held = (codes, scales)
 
     @classmethod
-    def empty(cls, rows: int, cols: int, device: torch.device) -> "MxTensor":
-        """Uninitialised, codes and scales in one allocation."""
+    def empty_on(cls, other: torch.Tensor, rows: int, cols: int) -> "MxTensor":
+        """Uninitialised, codes and scales in one allocation on another tensor's device."""
         t = cls.__new__(cls)
         offset = (_code_bytes(rows, cols) + 255) // 256 * 256
-        held = torch.empty(offset + _packed_bytes(rows, cols), dtype=torch.uint8, device=device)
-        t.rows, t.cols, t.device, t._held = rows, cols, held.device, held
+        held = other.new_empty(offset + _packed_bytes(rows, cols), dtype=torch.uint8)
+        t.rows, t.cols, t.index, t._held = rows, cols, held.get_device(), held
         t.codes_ptr = held.data_ptr()
         t.scales_ptr = t.codes_ptr + offset
         return t
@@ -99,6 +99,13 @@ class MxTensor:
         return self.rows, self.cols
 
     @property
+    def device(self) -> torch.device:
+        return torch.device("cuda", self.index)
+
+    def _any(self) -> torch.Tensor:
+        return self._held[0] if isinstance(self._held, tuple) else self._held
+
+    @property
     def codes(self) -> torch.Tensor:
         if isinstance(self._held, tuple):
             return self._held[0]
@@ -114,9 +121,8 @@ class MxTensor:
         return f"MxTensor({self.rows} x {self.cols}, {self.device})"
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """The library's entry point on the device's current stream, with the device current."""
-    index = device.index
+def _call(name: str, index: int, *args) -> None:
+    """The library's entry point on the current stream of device `index`, with it current."""
     fn = getattr(_native.load(), name)
     if index == _current_device():
         status = fn(*args, _raw_stream(index))
@@ -142,10 +148,6 @@ def _rule_code(rule: str) -> int:
 
 def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     """x [..., cols] as a matrix [rows][cols] of the same memory."""
-    if not x.is_cuda:
-        raise ValueError(f"{what} is on a CUDA device")
-    if x.dim() == 2:
-        return x
     if x.dim() == 0:
         raise ValueError(f"{what} has at least one axis")
     if x.dim() == 1:
@@ -160,35 +162,42 @@ def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
                          "pass a contiguous tensor") from None
 
 
-def _pitch(x: torch.Tensor) -> int | None:
-    """Elements from one row of a matrix to the next; None where its rows are not
-    contiguous or overlap."""
+def _layout(x: torch.Tensor) -> tuple[int, int, int | None]:
+    """Rows, columns and pitch (elements from one row to the next) of a matrix; no
+    pitch where its rows are not contiguous or overlap."""
     rows, cols = x.shape
-    if cols > 1 and x.stride(1) != 1:
-        return None
+    down, along = x.stride()
+    if along != 1 and cols > 1:
+        return rows, cols, None
     if rows <= 1:
-        return (cols + 7) // 8 * 8  # one row: any pitch does
-    return x.stride(0) if x.stride(0) >= cols else None
+        return rows, cols, (cols + 7) // 8 * 8  # one row: any pitch does
+    return rows, cols, down if down >= cols else None
+
+
+def _device_index(x: torch.Tensor, what: str) -> int:
+    index = x.get_device()
+    if index < 0:
+        raise ValueError(f"{what} is on a CUDA device")
+    return index
 
 
 def _quantize(x: torch.Tensor, rule: str, rows: bool, cols: bool):
     dtype = _dtype_code(x.dtype, "x")
     code = _rule_code(rule)
-    x = _matrix(x, "x")
-    pitch = _pitch(x)
+    index = _device_index(x, "x")
+    if x.dim() != 2:
+        x = _matrix(x, "x")
+    r, c, pitch = _layout(x)
     swap = pitch is None
     if swap:  # a transposed view: its rows are the columns of what lies in memory
-        x = x.t()
         rows, cols = cols, rows
-        pitch = _pitch(x)
+        r, c, pitch = _layout(x.t())
         if pitch is None:
             raise ValueError("one axis of x has to be contiguous and its rows must not overlap")
-    r, c = x.shape
-    device = x.device
-    by_row = MxTensor.empty(r, c, device) if rows else None
-    by_col = MxTensor.empty(c, r, device) if cols else None
+    by_row = MxTensor.empty_on(x, r, c) if rows else None
+    by_col = MxTensor.empty_on(x, c, r) if cols else None
     if r and c:
-        _call("tcb_mx_quantize", device, dtype, x.data_ptr(), r, c, pitch, code,
+        _call("tcb_mx_quantize", index, dtype, x.data_ptr(), r, c, pitch, code,
               by_row.codes_ptr if rows else None, by_row.scales_ptr if rows else None,
               by_col.codes_ptr if cols else None, by_col.scales_ptr if cols else None)
     return (by_col, by_row) if swap else (by_row, by_col)
@@ -211,28 +220,31 @@ def quantize_pair(x: torch.Tensor, *, rule: str = "floor") -> tuple[MxTensor, Mx
     return _quantize(x, rule, True, True)
 
 
-def dequantize(q: MxTensor, dtype: torch.dtype = torch.bfloat16, *, out: torch.Tensor | None = None) -> torch.Tensor:
+def dequantize(q: MxTensor, dtype: torch.dtype = torch.bfloat16, *,
+               out: torch.Tensor | None = None) -> torch.Tensor:
     """The values of q, rounded once to `dtype` (or to out's type)."""
-    y = _output(out, q.device, q.rows, q.cols, dtype)
+    y, code, pitch = _output(out, q, q.rows, q.cols, dtype)
     if q.rows and q.cols:
-        _call("tcb_mx_dequantize", q.device, _DTYPES[y.dtype], q.codes_ptr, q.scales_ptr, q.rows,
-              q.cols, y.data_ptr(), _pitch(y))
+        _call("tcb_mx_dequantize", q.index, code, q.codes_ptr, q.scales_ptr, q.rows, q.cols,
+              y.data_ptr(), pitch)
     return y
 
 
-def _output(out: torch.Tensor | None, device: torch.device, rows: int, cols: int,
-            dtype: torch.dtype) -> torch.Tensor:
+def _output(out: torch.Tensor | None, q: MxTensor, rows: int, cols: int,
+            dtype: torch.dtype) -> tuple[torch.Tensor, int, int]:
+    """`out`, or a new tensor on q's device; the library's code of its type; its pitch."""
     if out is None:
-        _dtype_code(dtype, "the output")
-        return torch.empty((rows, cols), dtype=dtype, device=device)
-    _dtype_code(out.dtype, "out")
+        code = _dtype_code(dtype, "the output")
+        return q._any().new_empty((rows, cols), dtype=dtype), code, cols
+    code = _dtype_code(out.dtype, "out")
     if out.shape != (rows, cols):
         raise ValueError(f"out is [{rows}][{cols}], got {list(out.shape)}")
-    if out.device != device:
-        raise ValueError(f"out is on {out.device}, the operands are on {device}")
-    if _pitch(out) is None:
+    if out.get_device() != q.index:
+        raise ValueError(f"out is on {out.device}, the operands are on {q.device}")
+    pitch = _layout(out)[2]
+    if pitch is None:
         raise ValueError("the rows of out have to be contiguous and must not overlap")
-    return out
+    return out, code, pitch
 
 
 def _bias(bias: torch.Tensor | None, n: int, y: torch.Tensor) -> int | None:
@@ -243,61 +255,65 @@ def _bias(bias: torch.Tensor | None, n: int, y: torch.Tensor) -> int | None:
         raise TypeError(f"bias has the output's type {y.dtype}, got {bias.dtype}")
     if bias.shape != (n,) or (n > 1 and bias.stride(0) != 1):
         raise ValueError(f"bias is a contiguous [{n}], got {list(bias.shape)}")
-    if bias.device != y.device:
+    if bias.get_device() != y.get_device():
         raise ValueError(f"bias is on {bias.device}, the operands are on {y.device}")
     return bias.data_ptr()
 
 
 def matmul(a: MxTensor, b: MxTensor, *, bias: torch.Tensor | None = None,
-           dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None, status=None) -> torch.Tensor:
+           dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+           status: torch.Tensor | None = None) -> torch.Tensor:
     """a [M][K] . b [N][K]^T (+ bias [N]) in `dtype` (or out's type).
 
     ``status`` (an int32 device word) receives an error of a device-side wait.
     """
-    if a.cols != b.cols:
-        raise ValueError(f"a has {a.cols} columns and b {b.cols}")
-    if a.device != b.device:
+    m, n, k = a.rows, b.rows, a.cols
+    if k != b.cols:
+        raise ValueError(f"a has {k} columns and b {b.cols}")
+    if a.index != b.index:
         raise ValueError(f"a is on {a.device} and b on {b.device}")
-    if a.cols == 0:
+    if k == 0:
         raise ValueError("a product over no columns")
-    y = _output(out, a.device, a.rows, b.rows, dtype)
-    bias_ptr = _bias(bias, b.rows, y)
-    if a.rows and b.rows:
-        _call("tcb_mx_gemm", a.device, a.codes_ptr, a.scales_ptr, b.codes_ptr, b.scales_ptr, bias_ptr,
-              _DTYPES[y.dtype], y.data_ptr(), _pitch(y), a.rows, b.rows, a.cols, _native._ptr(status))
+    y, code, pitch = _output(out, a, m, n, dtype)
+    bias_ptr = _bias(bias, n, y)
+    if m and n:
+        _call("tcb_mx_gemm", a.index, a.codes_ptr, a.scales_ptr, b.codes_ptr, b.scales_ptr, bias_ptr,
+              code, y.data_ptr(), pitch, m, n, k, _native._ptr(status))
     return y
 
 
 def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
-           dtype: torch.dtype | None = None, out: torch.Tensor | None = None, status=None) -> torch.Tensor:
+           dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+           status: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] . w [N][K]^T (+ bias [N]) with bf16 or fp16 x, in `dtype` (default x's).
 
     Only the weight is rounded to MX FP4.  Meant for few rows: w is read once per 16
     rows of x (for many rows quantise x too and take :func:`matmul`).  ``out`` is a
     matrix [rows][N].
     """
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"x is bf16 or fp16, got {x.dtype}")
-    lead = x.shape[:-1]
-    m = _matrix(x, "x")
-    if m.shape[1] != w.cols:
-        raise ValueError(f"x has {m.shape[1]} columns and w {w.cols}")
-    if m.device != w.device:
-        raise ValueError(f"x is on {m.device} and w on {w.device}")
-    if w.cols == 0:
+    x_dtype = x.dtype
+    if x_dtype != torch.bfloat16 and x_dtype != torch.float16:
+        raise TypeError(f"x is bf16 or fp16, got {x_dtype}")
+    if _device_index(x, "x") != w.index:
+        raise ValueError(f"x is on {x.device} and w on {w.device}")
+    flat = x if x.dim() == 2 else _matrix(x, "x")
+    m, k, x_pitch = _layout(flat)
+    n = w.rows
+    if k != w.cols:
+        raise ValueError(f"x has {k} columns and w {w.cols}")
+    if k == 0:
         raise ValueError("a product over no columns")
-    pitch = _pitch(m)
-    if pitch is None:
+    if x_pitch is None:
         raise ValueError("the rows of x have to be contiguous and must not overlap")
-    y = _output(out, m.device, m.shape[0], w.rows, x.dtype if dtype is None else dtype)
-    bias_ptr = _bias(bias, w.rows, y)
-    if m.shape[0] and w.rows:
-        need = _native.mx_linear_workspace_bytes(m.shape[0], w.cols)
-        space = torch.empty(need, dtype=torch.uint8, device=m.device) if need else None
-        _call("tcb_mx_linear", m.device, _DTYPES[x.dtype], m.data_ptr(), pitch, w.codes_ptr,
-              w.scales_ptr, bias_ptr, _DTYPES[y.dtype], y.data_ptr(), _pitch(y), m.shape[0], w.rows,
-              w.cols, _native._ptr(space), need, _native._ptr(status))
-    return y if out is not None or len(lead) == 1 else y.view(*lead, w.rows)
+    y, code, pitch = _output(out, w, m, n, x_dtype if dtype is None else dtype)
+    bias_ptr = _bias(bias, n, y)
+    if m and n:
+        need = _native.mx_linear_workspace_bytes(m, k)
+        space = flat.new_empty(need, dtype=torch.uint8) if need else None
+        _call("tcb_mx_linear", w.index, _DTYPES[x_dtype], flat.data_ptr(), x_pitch, w.codes_ptr,
+              w.scales_ptr, bias_ptr, code, y.data_ptr(), pitch, m, n, k, _native._ptr(space), need,
+              _native._ptr(status))
+    return y if out is not None or flat is x else y.view(*x.shape[:-1], n)
 
 
 @dataclass
@@ -321,13 +337,13 @@ def linear_forward(x: torch.Tensor, w: torch.Tensor, *,
     """
     if w.dim() != 2 or x.dim() == 0 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"x is [..., in] and w [out][in], got {list(x.shape)} and {list(w.shape)}")
-    if x.device != w.device:
+    if x.get_device() != w.get_device():
         raise ValueError(f"x is on {x.device} and w on {w.device}")
     x_rows, x_cols = quantize_pair(x, rule=rule)
     w_rows, w_cols = quantize_pair(w, rule=rule)
     y = matmul(x_rows, w_rows, dtype=x.dtype)
     saved = LinearSaved(x_cols, w_cols, tuple(x.shape), x.dtype, w.dtype, rule)
-    return y.view(*x.shape[:-1], w.shape[0]), saved
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0]), saved
 
 
 def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = True,
@@ -341,13 +357,15 @@ def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = Tru
     shape = saved.x_shape[:-1] + (out_features,)
     if tuple(dy.shape) != shape:
         raise ValueError(f"dy is {list(shape)}, got {list(dy.shape)}")
-    if dy.device != saved.x.device:
+    if dy.get_device() != saved.x.index:
         raise ValueError(f"dy is on {dy.device}, the forward pass was on {saved.x.device}")
     dy_rows, dy_cols = _quantize(dy, saved.rule, need_dx, need_dw) \
         if need_dx or need_dw else (None, None)
     dx = dw = None
     if need_dx:
-        dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype).view(saved.x_shape)
+        dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype)
+        if len(saved.x_shape) != 2:
+            dx = dx.view(saved.x_shape)
     if need_dw:
         if saved.x.cols == 0:
             dw = torch.zeros((out_features, in_features), dtype=saved.w_dtype, device=dy.device)
