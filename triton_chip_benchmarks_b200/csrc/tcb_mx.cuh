@@ -78,9 +78,8 @@ __device__ __forceinline__ float scale_value(uint32_t e8) {
   return __uint_as_float(e8 == 0 ? 0x00400000u : e8 == 255 ? 0x7FC00000u : e8 << 23);
 }
 
-// Eight values times `inv` as E2M1 codes, the first in the low nibble; zeros
-// where the group's scale is NaN.
-__device__ __forceinline__ uint32_t encode8(const float (&v)[8], float inv, uint32_t e8) {
+// Eight values as E2M1 codes, the first in the low nibble (nearest even, saturating).
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8]) {
   uint32_t w;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -89,9 +88,17 @@ __device__ __forceinline__ uint32_t encode8(const float (&v)[8], float inv, uint
       "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(w)
-      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv),
-        "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
-  return e8 == 255 ? 0u : w;
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return w;
+}
+
+// The two bf16 values of a word times the bf16 power of two `factor`, in fp32:
+// one instruction a value (adding -0 keeps the sign of zeros).
+__device__ __forceinline__ void scale2(uint32_t w, uint16_t factor, float& lo, float& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "fma.rn.f32.bf16 %0, l, %3, 0f80000000;\n\tfma.rn.f32.bf16 %1, h, %3, 0f80000000;\n\t}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(w), "h"(factor));
 }
 
 // One E2M1 code (0..15) as fp32: |code| 0 and 1 are 0 and 1/2, the others

@@ -18,7 +18,7 @@
 // loads are straight-line code, all issued before the first is used (with a
 // bounds test around each they went out one by one: 74 us instead of TODO for
 // 8192 x 8192 bf16).  16-bit values stay packed for the search of the largest:
-// two a word, integer maxima of the magnitude bits.
+// two a word, one instruction a word.
 //
 // Both axes in one read.  The tile goes to shared memory with cp.async (zeros
 // past the edge), 16-byte chunks swizzled so that neither the row-wise nor the
@@ -97,14 +97,52 @@ __device__ __forceinline__ int tile_chunk(int row, int c) {
   return row * kTile * static_cast<int>(sizeof(T)) + ((c ^ ((c >> 3) & kMask)) << 4);
 }
 
-// Running maximum of a word's magnitudes: both halves of a 16-bit pair, or one
-// fp32 pattern.
+// Running maximum of magnitudes, a word at a time: one fp32 pattern, or the two
+// halves of a 16-bit pair with a NaN winning (the hardware's magnitude maximum
+// leaves some sign in `top`).
 template <typename T>
 __device__ __forceinline__ uint32_t top_of(uint32_t top, uint32_t w) {
   if constexpr (sizeof(T) == 4)
     return max(top, w & 0x7FFFFFFFu);
+  else if constexpr (std::is_same_v<T, __half>)
+    asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(top) : "r"(w));
   else
-    return __vmaxu2(top, w & 0x7FFF7FFFu);
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(w));
+  return top;
+}
+
+// fp32 bits of the larger (which = -1) or of one of the magnitudes in `top`.
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude(uint32_t top, int which) {
+  if constexpr (sizeof(T) == 4) {
+    return top;
+  } else {
+    top &= 0x7FFF7FFFu;
+    return which < 0 ? max(top & 0xFFFFu, top >> 16) : which ? top >> 16 : top & 0xFFFFu;
+  }
+}
+
+// Eight consecutive values (their words) times 2^-e as E2M1 codes; zeros where
+// the scale is NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t encode_words(const uint32_t* w, uint32_t e8) {
+  const float inv = inverse_scale(e8);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(w[i]) * inv;
+    } else if (i % 2 == 0) {
+      if constexpr (std::is_same_v<T, __half>) {
+        unpack2<T>(w[i / 2], v[i], v[i + 1]);
+        v[i] *= inv;
+        v[i + 1] *= inv;
+      } else {
+        scale2(w[i / 2], static_cast<uint16_t>(__float_as_uint(inv) >> 16), v[i], v[i + 1]);
+      }
+    }
+  }
+  return e8 == 255 ? 0u : encode8(v);
 }
 
 // fp32 bits of a magnitude given by T's bits.
@@ -120,7 +158,7 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t magnitude) {
 }
 
 template <typename T, bool VEC, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : (COLS ? 5 : 4))
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : COLS && !std::is_same_v<T, __half> ? 5 : 4)
     quantize_kernel(const __grid_constant__ QuantArgs args) {
   constexpr bool kTiled = COLS || !VEC;
   constexpr int kChunks = kWords<T> / 4;  // 16-byte chunks of a thread's values
@@ -212,22 +250,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : (C
 #pragma unroll
       for (int q = 0; q < kWords<T>; ++q) top = top_of<T>(top, w[q]);
       top = top_of<T>(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-      if constexpr (sizeof(T) == 2) top = max(top & 0xFFFFu, top >> 16);
-      const uint32_t e8 = scale_code(top_bits<T>(top), args.up);
-      const float inv = inverse_scale(e8);
+      const uint32_t e8 = scale_code(top_bits<T>(magnitude<T>(top, -1)), args.up);
       uint32_t codes[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if constexpr (sizeof(T) == 4)
-            v[k] = __uint_as_float(w[8 * h + k]);
-          else if (k % 2 == 0)
-            unpack2<T>(w[4 * h + k / 2], v[k], v[k + 1]);
-        }
-        codes[h] = encode8(v, inv, e8);
-      }
+      for (int h = 0; h < 2; ++h) codes[h] = encode_words<T>(w + h * (kWords<T> / 2), e8);
       if (in_cols && r0 + lr < args.rows)
         *reinterpret_cast<uint2*>(args.codes + (r0 + lr) * pitch + (c0 + col) / 2) =
             make_uint2(codes[0], codes[1]);
@@ -259,24 +285,20 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : (C
       }
 #pragma unroll
       for (int k = 0; k < kColsPerWord; ++k) {
-        const uint32_t magnitude = sizeof(T) == 4 ? top : (top >> (16 * k)) & 0xFFFFu;
-        const uint32_t e8 = scale_code(top_bits<T>(magnitude), args.up);
-        const float inv = inverse_scale(e8);
+        const uint32_t e8 = scale_code(top_bits<T>(magnitude<T>(top, k)), args.up);
         uint32_t codes[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float v[8];
+          if constexpr (sizeof(T) == 4) {
+            codes[q] = encode_words<T>(w + 8 * q, e8);
+          } else {
+            // This column's values of eight rows, two a word.
+            uint32_t pairs[4];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if constexpr (sizeof(T) == 4) {
-              v[i] = __uint_as_float(w[8 * q + i]);
-            } else {
-              float lo, hi;
-              unpack2<T>(w[8 * q + i], lo, hi);
-              v[i] = k ? hi : lo;
-            }
+            for (int i = 0; i < 4; ++i)
+              pairs[i] = __byte_perm(w[8 * q + 2 * i], w[8 * q + 2 * i + 1], k ? 0x7632 : 0x5410);
+            codes[q] = encode_words<T>(pairs, e8);
           }
-          codes[q] = encode8(v, inv, e8);
         }
         const int c = word * kColsPerWord + k;
         *reinterpret_cast<uint4*>(s_codes_t + c * kCodesPitch + group * 16) =

@@ -187,7 +187,7 @@ __device__ __forceinline__ int digit_scale(const float (&v)[8]) {
 // The next digit of eight values u (times 2^e8 - 127 of the digit): its codes; u
 // becomes what is left, times 8.
 __device__ __forceinline__ uint32_t next_digit(float (&u)[8]) {
-  const uint32_t codes = encode8(u, 1.0f, 0);
+  const uint32_t codes = encode8(u);
   uint32_t h[4];
   decode8(codes, h);
 #pragma unroll
