@@ -244,8 +244,9 @@ int tcb_mx_gemm(const void *A, const void *SA, const void *B, const void *SB, co
  * (row pitch ldx >= K elements) and only W quantised; Y and bias in `dtype` as
  * above.  X takes part as eight MX FP4 digits of three bits: within a group of 32
  * values of a row, each is taken to 2^-24 of the group's largest.  Infinities and
- * NaN propagate as in the plain product.  Meant for few rows (decoding); W is read
- * once per 16 rows of X.  workspace (256-byte aligned) holds
+ * NaN propagate as in the plain product.  Up to 16 rows are bound by
+ * reading W once; more cost what an MX FP4 product of eight times the rows costs.
+ * workspace (256-byte aligned) holds
  * tcb_mx_linear_workspace_bytes(M, K) bytes that the call overwrites and needs
  * until its work on `stream` is done; it may be NULL where that is 0. */
 int tcb_mx_linear(int x_dtype, const void *X, long long ldx, const void *W, const void *SW,

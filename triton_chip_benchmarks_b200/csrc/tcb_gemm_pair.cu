@@ -72,7 +72,7 @@
 #include "tcb_gemm_common.cuh"
 #include "tcb_gemm_pair.h"
 #include "tcb_host.h"
-#include "tcb_mx.cuh"
+#include "tcb_mx_digits.cuh"
 #include "tcb_registry.h"
 
 namespace tcb {
@@ -130,6 +130,10 @@ struct PairArgs {
   int vec_store;    // C rows are 16-byte aligned
   int tma_store;    // C is written through the C tensor map (requires vec_store)
   uint32_t idesc;
+  const uint16_t* x;  // DIGITS kernels: the 16-bit rows, A's codes and their row bytes
+  const uint8_t* a;
+  long long ldx, pitch;
+  int x_k, x_bf16;
 };
 
 __device__ __forceinline__ void pair_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc,
@@ -218,7 +222,31 @@ __device__ __forceinline__ void acc_store16(uint16_t* dst, const uint32_t (&h)[3
   }
 }
 
-template <int OUT, bool BIAS>
+// DIGITS: B's rows are eight digits a token.  A lane (a row n of A) adds the eight
+// columns of each of its slice's eight tokens and stores C[token][n]: 32
+// neighbours a store.
+template <typename T>
+__device__ __forceinline__ void store_digits(const PairArgs& args, const uint32_t (&r)[2][32], int n, int c) {
+  if (n >= args.m) return;
+  const T* bias = static_cast<const T*>(args.bias);
+  const float b = bias == nullptr ? 0.0f : mx_detail::to_float(bias[n]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float v[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) v[d] = __uint_as_float(r[i >> 2][8 * (i & 3) + d]);
+    bool odd;
+    float sum = mx_detail::sum_digits(v, &odd);
+    const int token = c / mx_detail::kDigits + i;
+    if (token * mx_detail::kDigits >= args.n) break;
+    if (odd)
+      sum += mx_detail::odd_products(args.x + token * args.ldx, args.x_bf16, args.a, args.pitch, args.sa,
+                                     args.kblocks, n, 0, args.x_k);
+    static_cast<T*>(args.c)[token * args.ldc + n] = mx_detail::from_float<T>(sum + b);
+  }
+}
+
+template <int OUT, bool BIAS, bool DIGITS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_pair_mxf4_kernel(const __grid_constant__ CUtensorMap map_a,
                           const __grid_constant__ CUtensorMap map_b,
@@ -429,6 +457,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tile_coords(pair + ti * pairs, args.tiles_m, args.tiles_n, &tm, &tn);
       const int row0 = tm * 2 * kPairRows + static_cast<int>(rank) * kPairRows + 32 * quarter;
       const int c = tn * kTileN + col0;
+      if constexpr (DIGITS) {
+        store_digits<Out>(args, r, row0 + lane, c);
+        __syncwarp();
+        continue;
+      }
       if constexpr (BIAS) add_bias(r, static_cast<const Out*>(args.bias), c, args.n);
       auto stage_slice = [&](uint8_t* buf, int q) {
         if constexpr (OUT == kPairFp32) {
@@ -616,12 +649,18 @@ int pair_map_c(CUtensorMap* map, void* base, int rows, int cols, long long ldc, 
 
 using PairFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PairArgs);
 
-PairFn pair_fn(int out, bool bias) {
+template <int OUT>
+PairFn pair_fn_of(bool bias, bool digits) {
+  if (digits) return gemm_pair_mxf4_kernel<OUT, false, true>;
+  return bias ? gemm_pair_mxf4_kernel<OUT, true, false> : gemm_pair_mxf4_kernel<OUT, false, false>;
+}
+
+PairFn pair_fn(int out, bool bias, bool digits) {
   switch (out) {
-    case kPairBf16: return bias ? gemm_pair_mxf4_kernel<kPairBf16, true> : gemm_pair_mxf4_kernel<kPairBf16, false>;
-    case kPairFp16: return bias ? gemm_pair_mxf4_kernel<kPairFp16, true> : gemm_pair_mxf4_kernel<kPairFp16, false>;
+    case kPairBf16: return pair_fn_of<kPairBf16>(bias, digits);
+    case kPairFp16: return pair_fn_of<kPairFp16>(bias, digits);
   }
-  return bias ? gemm_pair_mxf4_kernel<kPairFp32, true> : gemm_pair_mxf4_kernel<kPairFp32, false>;
+  return pair_fn_of<kPairFp32>(bias, digits);
 }
 
 }  // namespace
@@ -647,7 +686,14 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
   args.tiles_m = static_cast<int>(tiles_m);
   args.tiles_n = static_cast<int>(tiles_n);
   args.kblocks = static_cast<int>((kbytes + kBlockBytes - 1) / kBlockBytes);
-  args.vec_store = p.ldc * elem_bytes % 16 == 0 && aligned(p.c, 16);
+  const bool digits = p.digits_of != nullptr;
+  args.x = static_cast<const uint16_t*>(p.digits_of);
+  args.a = static_cast<const uint8_t*>(p.a);
+  args.ldx = p.digits_ld;
+  args.pitch = kbytes;
+  args.x_k = p.digits_k;
+  args.x_bf16 = p.digits_bf16;
+  args.vec_store = !digits && p.ldc * elem_bytes % 16 == 0 && aligned(p.c, 16);
   args.idesc = p.idesc;
   CUtensorMap map_a, map_b, map_a3, map_b3;
   int panels_a = static_cast<int>(kbytes / kBlockBytes), panels_b = panels_a;
@@ -658,9 +704,9 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
   CUtensorMap map_c{};
   args.tma_store =
       args.vec_store && pair_map_c(&map_c, p.c, p.m, p.n, p.ldc, elem_bytes) == TCB_OK;
-  const PairFn fn = pair_fn(p.out, p.bias != nullptr);
-  static DeviceIntCache cap_cache[3][2], resident_cache;
-  const int cap = cap_cache[p.out][p.bias != nullptr].get(facts.device, [&] {
+  const PairFn fn = pair_fn(p.out, p.bias != nullptr, digits);
+  static DeviceIntCache cap_cache[3][3], resident_cache;
+  const int cap = cap_cache[p.out][digits ? 2 : p.bias != nullptr].get(facts.device, [&] {
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
   if (cap < kPairSmem) return TCB_ERR_RESOURCE;
@@ -701,7 +747,7 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
 
 int gemm_pair_info(tcb_kernel_info_t* out) {
   cudaFuncAttributes attr;
-  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(pair_fn(kPairFp32, false))) !=
+  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(pair_fn(kPairFp32, false, false))) !=
       cudaSuccess)
     return TCB_ERR_DEVICE;
   fill_kernel_info(attr, out);

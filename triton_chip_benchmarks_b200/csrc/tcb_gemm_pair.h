@@ -23,6 +23,12 @@ struct PairProblem {
   int out;           // PairOutType
   uint32_t idesc;
   bool overlap;      // may start while the kernels before it still run (launch_overlapping)
+  // Non-null: b's rows are the MX FP4 digits of these 16-bit rows of digits_k
+  // values, and c is their product with a's rows, transposed: [n / 8][m].
+  const void* digits_of;
+  long long digits_ld;
+  int digits_k;
+  int digits_bf16;
 };
 
 int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFacts& facts,

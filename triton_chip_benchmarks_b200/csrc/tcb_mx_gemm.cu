@@ -9,9 +9,13 @@
 namespace tcb {
 namespace {
 
-// Up to here the weight's bytes bound the product and the few-row kernel,
-// which spreads them over every SM, is faster than tiles of 256 rows.
-constexpr int kFewRows = 256;
+// Up to here the weight's bytes bound the product and the few-row kernel, which
+// spreads them over every SM, is faster than tiles of 256 rows.  Measured
+// (us, few-row / CTA pairs, M = 8, 64, 128): N = K = 4096 6.7/9.4, 9.9/9.8,
+// 13.4/10.3; N = K = 8192 10.6/16.7, 12.8/16.6, 15.4/17.2; N = 4096, K = 1024
+// 4.2/6.0, 6.0/6.4, 7.5/6.8.
+constexpr int kFewRows = 64;
+static_assert(kFewRows <= kRowsMostMx, "one column tile of the few-row kernel");
 
 bool out_type(int dtype, int* rows, int* pair, int* bytes) {
   switch (dtype) {
@@ -50,7 +54,7 @@ extern "C" int tcb_mx_gemm(const void* A, const void* SA, const void* B, const v
     return mx_rows_run(p, nullptr, status_dev, facts, s);
   }
   const PairProblem p{A, B, SA, SB, bias, C, ldc, M, N, static_cast<int>(mx_detail::mx_padded(K)),
-                      pair_type, gemm_pair_idesc(), true};
+                      pair_type, gemm_pair_idesc(), true, nullptr, 0, 0, 0};
   return gemm_pair_run(p, 0, status_dev, facts, s);
 }
 

@@ -3,30 +3,18 @@
 //
 // With few rows the weight's bytes are all that counts (17/32 byte a weight,
 // read once), so the weight takes the M side of the MMA -- 128 rows a CTA, all
-// SMs busy -- and X the N side, 8 to 256 columns of
+// SMs busy -- and X the N side, 8 to 128 columns of
 // tcgen05.mma kind::mxf4.block_scale: nothing is decoded by threads.
 //
-// 16-bit rows as MX FP4 digits.  A group of 32 values with the largest in
-// [2^(e+1), 2^(e+2)) is split exactly into E2M1 digits,
-//   u_0 = x * 2^-e (|u_0| < 4),  d_i = RNE_E2M1(u_i),  u_{i+1} = 8 (u_i - d_i),
-//   x = sum_i d_i 2^(e - 3i):  |u_i| <= 4 keeps the rounding below 1/2, so each
-// digit gives three bits more.  Eight digits hold a value to 2^-24 of its
-// group's largest: bf16 values down to 2^-16 of it (fp16: 2^-13) without any
-// error, smaller ones as a 24-bit fixed-point number, the precision that an
-// fp32 sum holding the largest has.  The digits are eight rows of an MX tensor
-// whose scales differ by 2^3, so one block-scaled MMA sums them all, and the
-// epilogue adds a token's eight columns in fp32, smallest first.  (Decoding W to
-// fp16 for mma.sync instead was bound by issue slots: 24 us at
-// 1 x 16384 x 8192, 31 us at 16 x 8192 x 8192.)  Infinities and NaN have no
-// digits: they count as zero there, and the NaN scale on their group's last
-// digit makes the epilogue take their products with the row's weights one by
-// one (the token's results are then infinite or NaN whatever the rest sums to).
+// 16-bit rows take part as eight MX FP4 digits each (tcb_mx_digits.cuh), columns that
+// the epilogue adds.  (Decoding W to fp16 for mma.sync instead was bound by issue
+// slots: 24 us at 1 x 16384 x 8192, 31 us for 16 MX rows at 8192 x 8192.)
 //
 // Where the digits come from.  Up to kInlineTokens rows, X warps of each CTA write
 // the digits of its K slice into shared memory on the way; for more rows a
 // kernel of their own writes them once (into the caller's workspace), and the
-// product starts beside it: its weight loads
-// are under way before the digits are there.
+// product starts beside it: its weight loads are under way before the digits
+// are there.  More than kRowsMostDigits rows become columns of the CTA-pair GEMM.
 //
 // Split over K.  With fewer row tiles than CTAs fit, up to eight CTAs of a
 // cluster share a row tile, each with a part of K.  Each sends the others their
@@ -51,7 +39,7 @@
 #include "tcb_gemm_common.cuh"
 #include "tcb_gemm_pair.h"
 #include "tcb_host.h"
-#include "tcb_mx.cuh"
+#include "tcb_mx_digits.cuh"
 #include "tcb_mx_rows.h"
 
 namespace tcb {
@@ -77,18 +65,13 @@ constexpr int kBlockK = 2 * kBlockBytes;          // K values of a stage
 constexpr int kWBytes = kRowTile * kBlockBytes;   // 16 KB
 constexpr int kScaleBlock = 1024;                 // packed scales of 128 rows x 256 values
 constexpr int kMaxStages = 8;
-constexpr int kMaxCols = 256;                     // MX rows; digits take up to kPairedCols
-constexpr int kDigits = 8;
-constexpr int kDigitBits = 3;
 constexpr int kInlineTokens = 2;
-constexpr int kDigitRows = 128;                   // digit rows of a column tile, used or not
 constexpr int kXWarps = 4;
 constexpr int kMaxSplit = 8;
 constexpr int kEarlyTokens = 16;
-// Two CTAs share an SM while X has at most this many columns.
-constexpr int kPairedCols = 128;
-constexpr int kPairedSmem = 112 * 1024;
-constexpr int kAloneSmem = 224 * 1024;
+// Two CTAs share an SM: half of its shared memory and of its tensor memory each.
+constexpr int kSmemBudget = 112 * 1024;
+constexpr int kCtaTmemCols = 256;
 
 enum XMode : int { kXRows = 0, kXDigits = 1, kXInline = 2 };
 
@@ -106,8 +89,7 @@ struct RowsArgs {
   int kblocks;
   int split;             // CTAs of a cluster
   int stages, stage_bytes;
-  int cols;              // columns of a column tile (a multiple of 8)
-  int tmem_cols;
+  int cols;              // columns of the MMA (a multiple of 8, at most 128)
   int x_bf16;
   int y_type;            // RowsType of y and the bias
   uint32_t idesc;
@@ -134,11 +116,6 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
-__device__ __forceinline__ float value16(uint16_t bits, bool bf16) {
-  return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
-              : __half2float(__ushort_as_half(bits));
-}
-
 // The 16-bit values x[k..k+7] of a row, zeros past the end.
 __device__ __forceinline__ uint4 load_values(const uint16_t* row, int k, int end, bool vec) {
   if (vec && k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
@@ -157,7 +134,7 @@ __device__ __forceinline__ void to_values(uint4 raw, bool bf16, float (&v)[8], b
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     v[i] = value16(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))), bf16);
-    if ((__float_as_uint(v[i]) & 0x7FFFFFFFu) >= 0x7F800000u) {
+    if (is_odd(v[i])) {
       v[i] = 0.0f;
       *odd = true;
     }
@@ -201,10 +178,10 @@ __device__ __forceinline__ uint32_t next_digit(float (&u)[8]) {
 }
 
 // Digits of all tokens as rows of an MX tensor, one warp per token and K block:
-// digit i of token j of a tile of `per_tile` tokens is row 128 tile + 8 j + i.
+// digit i of token j is row 8 j + i.
 __global__ void __launch_bounds__(256)
     mx_digits_kernel(const uint16_t* __restrict__ x, long long ldx, int m, int k, long long pitch,
-                     int kblocks, int per_tile, int vec, int bf16, uint8_t* __restrict__ codes,
+                     int kblocks, int vec, int bf16, uint8_t* __restrict__ codes,
                      uint8_t* __restrict__ scales) {
   // The product may start once the kernels before this one are done: its weight
   // may be theirs.
@@ -226,7 +203,7 @@ __global__ void __launch_bounds__(256)
   const int group = lane >> 2;
 #pragma unroll
   for (int d = 0; d < kDigits; ++d) {
-    const long long row = token / per_tile * kDigitRows + token % per_tile * kDigits + d;
+    const long long row = token * kDigits + d;
     const int code = e8 - kDigitBits * d;
     const uint32_t w = next_digit(u);
     if (byte < pitch) *reinterpret_cast<uint32_t*>(codes + row * pitch + byte) = code >= 0 ? w : 0u;
@@ -286,18 +263,14 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   const int kb1 = static_cast<int>(static_cast<long long>(args.kblocks) * (rank + 1) / args.split);
   const int nkb = kb1 - kb0;
   constexpr int kPerToken = XMODE == kXRows ? 1 : kDigits;  // columns of a token
-  const int token0 = static_cast<int>(blockIdx.y) * (args.cols / kPerToken);
-  // X's first row: column tiles of digits start on 128-row blocks of scales.
-  const int row0 = static_cast<int>(blockIdx.y) * (XMODE == kXDigits ? kDigitRows : args.cols);
-  const int tokens = min(args.cols / kPerToken, args.m - token0);
+  const int tokens = args.m;
   const int x_bytes = args.cols * kBlockBytes;
-  const int sx_blocks = args.cols > 128 ? 2 : 1;
 
   auto load_w = [&](int it) {
     const int s = it % args.stages, kb = kb0 + it;
     uint8_t* stage = smem + s * args.stage_bytes;
     mbar_arrive_expect_tx(&loaded[s], kWBytes + kScaleBlock +
-                                          (XMODE == kXInline ? 0 : x_bytes + sx_blocks * kScaleBlock));
+                                          (XMODE == kXInline ? 0 : x_bytes + kScaleBlock));
     tma_load_2d(stage, &map_w, kb * kBlockBytes, tile * kRowTile, &loaded[s]);
     bulk_load_1d(stage + kWBytes + x_bytes,
                  args.sw + (static_cast<long long>(tile) * args.kblocks + kb) * kScaleBlock,
@@ -307,13 +280,9 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     uint8_t* stage = smem + (it % args.stages) * args.stage_bytes;
     uint64_t* bar = &loaded[it % args.stages];
     const int kb = kb0 + it;
-    tma_load_2d(stage + kWBytes, &map_x, kb * kBlockBytes, row0, bar);
-    const uint8_t* sx = args.sx + (static_cast<long long>(row0 / 128) * args.kblocks + kb) * kScaleBlock;
-    uint8_t* dst = stage + kWBytes + x_bytes + kScaleBlock;
-    bulk_load_1d(dst, sx, kScaleBlock, bar);
-    if (sx_blocks == 2)
-      bulk_load_1d(dst + kScaleBlock, sx + static_cast<long long>(args.kblocks) * kScaleBlock, kScaleBlock,
-                   bar);
+    tma_load_2d(stage + kWBytes, &map_x, kb * kBlockBytes, 0, bar);
+    bulk_load_1d(stage + kWBytes + x_bytes + kScaleBlock,
+                 args.sx + static_cast<long long>(kb) * kScaleBlock, kScaleBlock, bar);
   };
   // An X warp's next values (inline digits): asked for one round ahead, the first
   // ones before the weights, behind whose bytes they would otherwise queue.
@@ -323,7 +292,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
 #pragma unroll
     for (int i = 0; i < kInlineTokens; ++i)
       if (i < tokens && it < nkb)
-        x_next[i] = load_values(static_cast<const uint16_t*>(args.x) + (token0 + i) * args.ldx,
+        x_next[i] = load_values(static_cast<const uint16_t*>(args.x) + i * args.ldx,
                                 (kb0 + it) * kBlockK + lane * 8, args.k, vec);
   };
   if constexpr (XMODE == kXInline) {
@@ -353,7 +322,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     }
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_slot, args.tmem_cols);
+    tmem_alloc(&tmem_slot, kCtaTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -427,7 +396,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
       if (!__all_sync(0xFFFFFFFFu, ok)) break;  // tcgen05.st needs the whole warp
       const uint8_t* sw = smem + s * args.stage_bytes + kWBytes + x_bytes + lane * 16;
       gemm_detail::write_scale_block(lane_base + static_cast<uint32_t>(s * kSfStageCols), sw,
-                                     sw + kScaleBlock, sw + sx_blocks * kScaleBlock);
+                                     sw + kScaleBlock, sw + kScaleBlock);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -505,25 +474,14 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
           if (c + i < tokens) send(c + i, r[i]);
       } else {
         const int token = c / kDigits;
-        const bool odd = isnan(r[kDigits - 1]);  // infinities or NaN in x (or a NaN scale in w)
-        float sum = odd ? 0.0f : r[kDigits - 1];
-#pragma unroll
-        for (int d = kDigits - 2; d >= 0; --d) sum += r[d];
+        bool odd;
+        float sum = sum_digits(r, &odd);
         const long long n = static_cast<long long>(tile) * kRowTile + row;
-        if (odd && n < args.n) {
-          const uint16_t* x = static_cast<const uint16_t*>(args.x) + (token0 + token) * args.ldx;
-          const int end = static_cast<int>(min(static_cast<long long>(kb1) * kBlockK,
-                                               static_cast<long long>(args.k)));
-          for (int k = kb0 * kBlockK; k < end; ++k) {
-            const float v = value16(x[k], args.x_bf16);
-            if ((__float_as_uint(v) & 0x7FFFFFFFu) < 0x7F800000u) continue;
-            const uint32_t code = args.w[n * args.pitch + k / 2] >> (4 * (k & 1)) & 15u;
-            const int group = k / 32;
-            const uint32_t e8 = args.sw[(static_cast<long long>(tile) * args.kblocks + group / 8) * kScaleBlock +
-                                        (group % 8 / 4) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (group & 3)];
-            sum += v * (decode1(code) * scale_value(e8));
-          }
-        }
+        if (odd && n < args.n)
+          sum += odd_products(static_cast<const uint16_t*>(args.x) + token * args.ldx, args.x_bf16, args.w,
+                              args.pitch, args.sw, args.kblocks, n, kb0 * kBlockK,
+                              static_cast<int>(min(static_cast<long long>(kb1) * kBlockK,
+                                                   static_cast<long long>(args.k))));
         send(token, sum);
       }
     }
@@ -537,18 +495,17 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
                                           args.n - n0));
     constexpr int kWarps = 6 + (XMODE == kXInline ? kXWarps : 0);
     const Finish f{sums, args.split, tokens, share, rows, warp, kWarps, lane};
-    const long long at = token0 * args.ldy + n0;
     if (args.y_type == kRowsFp32)
-      f.run(static_cast<const float*>(args.bias), n0, static_cast<float*>(args.y) + at, args.ldy);
+      f.run(static_cast<const float*>(args.bias), n0, static_cast<float*>(args.y) + n0, args.ldy);
     else if (args.y_type == kRowsBf16)
-      f.run(static_cast<const __nv_bfloat16*>(args.bias), n0, static_cast<__nv_bfloat16*>(args.y) + at,
+      f.run(static_cast<const __nv_bfloat16*>(args.bias), n0, static_cast<__nv_bfloat16*>(args.y) + n0,
             args.ldy);
     else
-      f.run(static_cast<const __half*>(args.bias), n0, static_cast<__half*>(args.y) + at, args.ldy);
+      f.run(static_cast<const __half*>(args.bias), n0, static_cast<__half*>(args.y) + n0, args.ldy);
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tbase, args.tmem_cols);
+    tmem_dealloc(tbase, kCtaTmemCols);
   }
 }
 
@@ -567,39 +524,34 @@ int rows_map(CUtensorMap* map, const void* base, long long rows, long long pitch
              : TCB_ERR_INVALID_ARGUMENT;
 }
 
-// The workspace of mx_rows_run for 16-bit rows: [scales][codes] of their digits.
+// The digits of m rows of k values as an MX tensor: [scales][codes].
 struct DigitSpace {
-  long long tiles, codes_at, bytes;  // column tiles
-  int per_tile;                      // tokens of a column tile
+  long long codes_at, bytes;
   DigitSpace(long long m, long long k) {
-    constexpr int kMost = kDigitRows / kDigits;
-    tiles = (m + kMost - 1) / kMost;
-    per_tile = static_cast<int>((m + tiles - 1) / tiles);
     const long long kblocks = (mx_padded(k) + kBlockK - 1) / kBlockK;
-    codes_at = (tiles + 1) / 2 * 2 * kScaleBlock * kblocks;
-    bytes = m <= kInlineTokens ? 0 : codes_at + tiles * kDigitRows * (mx_padded(k) / 2);
+    codes_at = (m * kDigits + 255) / 256 * 2 * kScaleBlock * kblocks;
+    bytes = codes_at + m * kDigits * (mx_padded(k) / 2);
   }
 };
 
 template <int XMODE>
-int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, long long chunks,
-                const DeviceFacts& facts, cudaStream_t stream) {
+int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, const DeviceFacts& facts, cudaStream_t stream) {
   const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile;
-  args.stage_bytes = kWBytes + args.cols * kBlockBytes + (args.cols > 128 ? 3 : 2) * kScaleBlock;
-  const bool paired = args.cols <= kPairedCols;
+  args.stage_bytes = kWBytes + args.cols * kBlockBytes + 2 * kScaleBlock;
   constexpr int kSumBytes = kEarlyTokens * (kRowTile + kMaxSplit) * 4;  // a share is rounded up
-  args.stages = ((paired ? kPairedSmem : kAloneSmem) - 1024 - kSumBytes) / args.stage_bytes;
+  args.stages = (kSmemBudget - 1024 - kSumBytes) / args.stage_bytes;
   if (args.stages > kMaxStages) args.stages = kMaxStages;
-  // Two CTAs of an SM get half of its tensor memory each.
-  args.tmem_cols = paired ? 256 : 512;
   const int acc_cols = (args.cols + 31) / 32 * 32;
-  while (acc_cols + args.stages * kSfStageCols > args.tmem_cols) --args.stages;
+  while (acc_cols + args.stages * kSfStageCols > kCtaTmemCols) --args.stages;
   const int smem = args.stages * args.stage_bytes + kSumBytes + 1024;
-  long long split = static_cast<long long>(facts.sm_count) * (paired ? 2 : 1) / (tiles * chunks);
-  split = split > kMaxSplit ? kMaxSplit : split;
-  split = split > args.kblocks ? args.kblocks : split;
-  args.split = split < 1 ? 1 : static_cast<int>(split);
-  if (tiles * args.split > INT_MAX || chunks > 65535) return TCB_ERR_RESOURCE;
+  // A power of two of CTAs to a row tile, each with at least one K block, such
+  // that all fit at once: clusters of four pack two CTAs on every SM, clusters of
+  // seven or eight leave SMs of a GPC over (5000 x 4136, 1 row: 8.5 us with four,
+  // 13.4 with seven; 4096 x 4096, 16 rows: 9.8 with four, 12.2 with eight).
+  args.split = 1;
+  for (int split = 2; split <= kMaxSplit; split *= 2)
+    if (split <= args.kblocks && tiles * split <= (split < 8 ? 2ll : 1ll) * facts.sm_count) args.split = split;
+  if (tiles * args.split > INT_MAX) return TCB_ERR_RESOURCE;
   // N of the instruction; M = 128, E2M1 x E2M1, E8M0 scales as the pair MMA.
   args.idesc = (gemm_pair_idesc() & ~(0x3Fu << 17 | 0x1Fu << 24)) |
                static_cast<uint32_t>(args.cols >> 3) << 17 | static_cast<uint32_t>(kRowTile >> 4) << 24;
@@ -609,14 +561,16 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
   if (cap < smem) return TCB_ERR_RESOURCE;
-  return launch_overlapping(fn, dim3(static_cast<unsigned>(tiles * args.split), static_cast<unsigned>(chunks)),
+  return launch_overlapping(fn, dim3(static_cast<unsigned>(tiles * args.split)),
                             (6 + (XMODE == kXInline ? kXWarps : 0)) * 32, static_cast<size_t>(smem),
                             args.split, stream, map_w, map_x, args);
 }
 
 }  // namespace
 
-long long mx_rows_workspace(long long m, long long k) { return DigitSpace(m, k).bytes; }
+long long mx_rows_workspace(long long m, long long k) {
+  return m <= kInlineTokens ? 0 : DigitSpace(m, k).bytes;
+}
 
 int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const DeviceFacts& facts,
                 cudaStream_t stream) {
@@ -641,28 +595,49 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
   int rc = rows_map(&map_w, p.w, p.n, args.pitch, kRowTile);
   if (rc != TCB_OK) return rc;
   if (p.x_type == kRowsMx) {
-    args.cols = p.m > kMaxCols ? kMaxCols : (p.m + 7) / 8 * 8;
+    args.cols = (p.m + 7) / 8 * 8;
     if ((rc = rows_map(&map_x, p.x, p.m, args.pitch, args.cols)) != TCB_OK) return rc;
-    return launch_rows<kXRows>(map_w, map_x, args, (p.m + args.cols - 1) / args.cols, facts, stream);
+    return launch_rows<kXRows>(map_w, map_x, args, facts, stream);
   }
   if (p.m <= kInlineTokens) {
     args.cols = p.m * kDigits;
-    return launch_rows<kXInline>(map_w, map_x, args, 1, facts, stream);
+    return launch_rows<kXInline>(map_w, map_x, args, facts, stream);
   }
   const DigitSpace space(p.m, p.k);
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  args.sx = base;
-  args.cols = space.per_tile * kDigits;
-  if ((rc = rows_map(&map_x, base + space.codes_at, space.tiles * kDigitRows, args.pitch, args.cols)) != TCB_OK)
-    return rc;
   const long long warps = static_cast<long long>(p.m) * args.kblocks;
-  if ((warps + 7) / 8 > INT_MAX) return TCB_ERR_RESOURCE;
+  if ((warps + 7) / 8 > INT_MAX || p.m > INT_MAX / (2 * kDigits)) return TCB_ERR_RESOURCE;
   rc = launch_overlapping(mx_digits_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, 1, stream,
                           static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, args.pitch, args.kblocks,
-                          space.per_tile, static_cast<int>(aligned(p.x, 16) && p.ldx % 8 == 0),
-                          args.x_bf16, base + space.codes_at, base);
+                          static_cast<int>(aligned(p.x, 16) && p.ldx % 8 == 0), args.x_bf16,
+                          base + space.codes_at, base);
   if (rc != TCB_OK) return rc;
-  return launch_rows<kXDigits>(map_w, map_x, args, space.tiles, facts, stream);
+  if (p.m > kRowsMostDigits) {
+    // Columns of the CTA-pair GEMM, whose M side is the weight.
+    PairProblem q = {};
+    q.a = p.w;
+    q.b = base + space.codes_at;
+    q.sa = p.sw;
+    q.sb = base;
+    q.bias = p.bias;
+    q.c = p.y;
+    q.ldc = p.ldy;
+    q.m = p.n;
+    q.n = p.m * kDigits;
+    q.k = static_cast<int>(mx_padded(p.k));
+    q.out = p.y_type == kRowsFp32 ? kPairFp32 : p.y_type == kRowsBf16 ? kPairBf16 : kPairFp16;
+    q.idesc = gemm_pair_idesc();
+    q.overlap = true;
+    q.digits_of = p.x;
+    q.digits_ld = p.ldx;
+    q.digits_k = p.k;
+    q.digits_bf16 = args.x_bf16;
+    return gemm_pair_run(q, 0, status, facts, stream);
+  }
+  args.sx = base;
+  args.cols = p.m * kDigits;
+  if ((rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols)) != TCB_OK) return rc;
+  return launch_rows<kXDigits>(map_w, map_x, args, facts, stream);
 }
 
 }  // namespace tcb

@@ -8,7 +8,7 @@ tensors' device and on its current stream, allocate their outputs through torch 
 * :func:`quantize`, :func:`quantize_pair`, :func:`dequantize`: between torch tensors
   (bf16, fp16, fp32) and MX tensors, along one axis or both in one read;
 * :func:`matmul`: ``a . b^T`` of two MX tensors;
-* :func:`linear`: 16-bit rows times an MX weight, for few rows (decoding);
+* :func:`linear`: 16-bit rows times an MX weight (decoding);
 * :func:`linear_forward`, :func:`linear_backward`: a linear layer's training step in
   MX products (both passes quantise their operands along the axis that the
   product sums over; gradients pass the rounding unchanged).
@@ -287,9 +287,9 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
            status: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] . w [N][K]^T (+ bias [N]) with bf16 or fp16 x, in `dtype` (default x's).
 
-    Only the weight is rounded to MX FP4.  Meant for few rows: w is read once per 16
-    rows of x (for many rows quantise x too and take :func:`matmul`).  ``out`` is a
-    matrix [rows][N].
+    Only the weight is rounded to MX FP4: x takes part as eight MX digits, so up to
+    16 rows cost what reading w costs, and many rows eight times as many of
+    :func:`matmul` (quantise x too where that matters).  ``out`` is a matrix [rows][N].
     """
     x_dtype = x.dtype
     if x_dtype != torch.bfloat16 and x_dtype != torch.float16:
