@@ -70,6 +70,9 @@ constexpr int kXWarps = 4;
 constexpr int kMaxSplit = 8;
 constexpr int kEarlyTokens = 16;
 // Two CTAs share an SM: half of its shared memory and of its tensor memory each.
+// (One CTA with twice the stages has the same bytes in flight but one MMA thread
+// and no second tile to cover its start and end: 28.6 us instead of 17.0 at
+// 1 x 32768 x 4096.)
 constexpr int kSmemBudget = 112 * 1024;
 constexpr int kCtaTmemCols = 256;
 
@@ -93,6 +96,17 @@ struct RowsArgs {
   int x_bf16;
   int y_type;            // RowsType of y and the bias
   uint32_t idesc;
+};
+
+// A role's place in the ring of stages.  Counted up, not divided out of a stage
+// number: two divisions a stage cost the MMA thread 400 of its 900 cycles.
+struct RingPlace {
+  int s = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int by, int stages) {
+    s += by;
+    if (s >= stages) s -= stages, phase ^= 1u;  // by <= stages
+  }
 };
 
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -266,8 +280,8 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   const int tokens = args.m;
   const int x_bytes = args.cols * kBlockBytes;
 
-  auto load_w = [&](int it) {
-    const int s = it % args.stages, kb = kb0 + it;
+  auto load_w = [&](int it, int s) {
+    const int kb = kb0 + it;
     uint8_t* stage = smem + s * args.stage_bytes;
     mbar_arrive_expect_tx(&loaded[s], kWBytes + kScaleBlock +
                                           (XMODE == kXInline ? 0 : x_bytes + kScaleBlock));
@@ -276,9 +290,9 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
                  args.sw + (static_cast<long long>(tile) * args.kblocks + kb) * kScaleBlock,
                  kScaleBlock, &loaded[s]);
   };
-  auto load_x = [&](int it) {
-    uint8_t* stage = smem + (it % args.stages) * args.stage_bytes;
-    uint64_t* bar = &loaded[it % args.stages];
+  auto load_x = [&](int it, int s) {
+    uint8_t* stage = smem + s * args.stage_bytes;
+    uint64_t* bar = &loaded[s];
     const int kb = kb0 + it;
     tma_load_2d(stage + kWBytes, &map_x, kb * kBlockBytes, 0, bar);
     bulk_load_1d(stage + kWBytes + x_bytes + kScaleBlock,
@@ -317,8 +331,8 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     // digits' kernel has waited for the kernels before it.)
     if (XMODE != kXDigits) wait_for_previous_kernels();
     for (int it = 0; it < min(nkb, args.stages); ++it) {
-      load_w(it);
-      if constexpr (XMODE == kXRows) load_x(it);
+      load_w(it, it);
+      if constexpr (XMODE == kXRows) load_x(it, it);
     }
   }
   if (warp == 1) {
@@ -336,16 +350,17 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      int it = min(nkb, args.stages);
+      const int first = min(nkb, args.stages);
       if constexpr (XMODE == kXDigits) {
-        for (int j = 0; j < it; ++j) load_x(j);
+        for (int j = 0; j < first; ++j) load_x(j, j);
       }
+      int it = first;
+      RingPlace at;  // stage it's, whose previous load is of phase at.phase
       for (; it < nkb; ++it) {
-        if (!wait_or_abort(&empty[it % args.stages], (static_cast<uint32_t>(it / args.stages) & 1u) ^ 1u,
-                           &abort_flag, args.status))
-          break;
-        load_w(it);
-        if constexpr (XMODE != kXInline) load_x(it);
+        if (!wait_or_abort(&empty[at.s], at.phase, &abort_flag, args.status)) break;
+        load_w(it, at.s);
+        if constexpr (XMODE != kXInline) load_x(it, at.s);
+        at.advance(1, args.stages);
       }
       // No load stays in flight after an abort either: each barrier of the last
       // round is in the phase that it was armed for.
@@ -358,9 +373,10 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     if (lane == 0) {
       const uint64_t desc_const = smem_desc(0, 16, 8 * kBlockBytes, 2u);
       const uint32_t smem0 = smem_addr(smem) >> 4;
-      for (int it = 0; it < nkb; ++it) {
-        const int s = it % args.stages;
-        const uint32_t phase = static_cast<uint32_t>(it / args.stages) & 1u;
+      RingPlace at;
+      for (int it = 0; it < nkb; ++it, at.advance(1, args.stages)) {
+        const int s = at.s;
+        const uint32_t phase = at.phase;
         // `full` follows `loaded` (and `digits`) in the scale writers, which have
         // waited for both.
         if (!wait_or_abort(&loaded[s], phase, &abort_flag, args.status)) break;
@@ -388,9 +404,10 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   } else if (warp < 6) {
     // ------------------------------------------------------ scale writers
     const uint32_t lane_base = tsf + ((32u * (warp & 3)) << 16);
-    for (int it = 0; it < nkb; ++it) {
-      const int s = it % args.stages;
-      const uint32_t phase = static_cast<uint32_t>(it / args.stages) & 1u;
+    RingPlace at;
+    for (int it = 0; it < nkb; ++it, at.advance(1, args.stages)) {
+      const int s = at.s;
+      const uint32_t phase = at.phase;
       bool ok = wait_or_abort(&loaded[s], phase, &abort_flag, args.status);
       if (XMODE == kXInline) ok = ok && wait_or_abort(&digits[s], phase, &abort_flag, args.status);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;  // tcgen05.st needs the whole warp
@@ -406,10 +423,11 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     // -------------------------------------------------------------- X warps
     // One warp a stage: digit d of token i is row 8 i + d of the X tile, whose
     // 16-byte chunk c lies at c ^ d (the 128-byte swizzle).
-    for (int it = warp - 6; it < nkb; it += kXWarps) {
-      const int s = it % args.stages;
-      const bool ok = wait_or_abort(&empty[s], (static_cast<uint32_t>(it / args.stages) & 1u) ^ 1u,
-                                    &abort_flag, args.status);
+    RingPlace at;
+    at.advance(warp - 6, args.stages);
+    for (int it = warp - 6; it < nkb; it += kXWarps, at.advance(kXWarps, args.stages)) {
+      const int s = at.s;
+      const bool ok = wait_or_abort(&empty[s], at.phase ^ 1u, &abort_flag, args.status);
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       uint8_t* xt = smem + s * args.stage_bytes + kWBytes;
       uint8_t* sx = xt + x_bytes + kScaleBlock;
@@ -538,12 +556,6 @@ template <int XMODE>
 int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, const DeviceFacts& facts, cudaStream_t stream) {
   const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile;
   args.stage_bytes = kWBytes + args.cols * kBlockBytes + 2 * kScaleBlock;
-  constexpr int kSumBytes = kEarlyTokens * (kRowTile + kMaxSplit) * 4;  // a share is rounded up
-  args.stages = (kSmemBudget - 1024 - kSumBytes) / args.stage_bytes;
-  if (args.stages > kMaxStages) args.stages = kMaxStages;
-  const int acc_cols = (args.cols + 31) / 32 * 32;
-  while (acc_cols + args.stages * kSfStageCols > kCtaTmemCols) --args.stages;
-  const int smem = args.stages * args.stage_bytes + kSumBytes + 1024;
   // A power of two of CTAs to a row tile, each with at least one K block, such
   // that all fit at once: clusters of four pack two CTAs on every SM, clusters of
   // seven or eight leave SMs of a GPC over (5000 x 4136, 1 row: 8.5 us with four,
@@ -552,6 +564,12 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   for (int split = 2; split <= kMaxSplit; split *= 2)
     if (split <= args.kblocks && tiles * split <= (split < 8 ? 2ll : 1ll) * facts.sm_count) args.split = split;
   if (tiles * args.split > INT_MAX) return TCB_ERR_RESOURCE;
+  constexpr int kSumBytes = kEarlyTokens * (kRowTile + kMaxSplit) * 4;  // a share is rounded up
+  args.stages = (kSmemBudget - 1024 - kSumBytes) / args.stage_bytes;
+  if (args.stages > kMaxStages) args.stages = kMaxStages;
+  const int acc_cols = (args.cols + 31) / 32 * 32;
+  while (acc_cols + args.stages * kSfStageCols > kCtaTmemCols) --args.stages;
+  const int smem = args.stages * args.stage_bytes + kSumBytes + 1024;
   // N of the instruction; M = 128, E2M1 x E2M1, E8M0 scales as the pair MMA.
   args.idesc = (gemm_pair_idesc() & ~(0x3Fu << 17 | 0x1Fu << 24)) |
                static_cast<uint32_t>(args.cols >> 3) << 17 | static_cast<uint32_t>(kRowTile >> 4) << 24;
