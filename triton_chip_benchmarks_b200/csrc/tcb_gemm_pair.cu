@@ -185,18 +185,14 @@ struct PairOut<kPairBf16> { using type = __nv_bfloat16; };
 template <>
 struct PairOut<kPairFp16> { using type = __half; };
 
-// acc += bias over this warp's 64 columns from `col0` (all lanes hold the same
-// columns, so every load is a broadcast).
-template <typename T>
-__device__ __forceinline__ void add_bias(uint32_t (&r)[2][32], const T* __restrict__ bias, int col0,
-                                         int n) {
+// acc += bias over this warp's 64 columns; lane l holds the bias of columns l and
+// 32 + l (asked for before the accumulator was ready).
+__device__ __forceinline__ void add_bias(uint32_t (&r)[2][32], float lo, float hi) {
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (col0 + 32 * q + e < n)
-        r[q][e] = __float_as_uint(__uint_as_float(r[q][e]) +
-                                  mx_detail::to_float(bias[col0 + 32 * q + e]));
+  for (int e = 0; e < 32; ++e) {
+    r[0][e] = __float_as_uint(__uint_as_float(r[0][e]) + __shfl_sync(0xffffffffu, lo, e));
+    r[1][e] = __float_as_uint(__uint_as_float(r[1][e]) + __shfl_sync(0xffffffffu, hi, e));
+  }
 }
 
 // 64 fp32 columns as 32 words of two 16-bit values.
@@ -439,7 +435,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       return true;
     };
+    using Out = typename PairOut<OUT>::type;
     for (int ti = 0; ti < my_tiles; ++ti) {
+      int row0, c;
+      auto place = [&] {
+        int tm, tn;
+        tile_coords(pair + ti * pairs, args.tiles_m, args.tiles_n, &tm, &tn);
+        row0 = tm * 2 * kPairRows + static_cast<int>(rank) * kPairRows + 32 * quarter;
+        c = tn * kTileN + col0;
+      };
+      [[maybe_unused]] float bias_lo = 0.0f, bias_hi = 0.0f;
+      if constexpr (BIAS) {
+        place();
+        const Out* bias = static_cast<const Out*>(args.bias);
+        if (c + lane < args.n) bias_lo = mx_detail::to_float(bias[c + lane]);
+        if (c + 32 + lane < args.n) bias_hi = mx_detail::to_float(bias[c + 32 + lane]);
+      }
       // Warp-uniform exits: tcgen05.ld and .st need the whole warp.
       if (!__all_sync(0xffffffffu, pair_wait(&acc_full, static_cast<uint32_t>(ti) & 1u,
                                               kPairIdleSleepNs)))
@@ -450,19 +461,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
-      using Out = typename PairOut<OUT>::type;
+      if constexpr (!BIAS) place();
       // A 16-bit slice is one 4 KB staging chunk (64 columns), an fp32 slice two.
       constexpr int kChunks = OUT == kPairFp32 ? 2 : 1;
-      int tm, tn;
-      tile_coords(pair + ti * pairs, args.tiles_m, args.tiles_n, &tm, &tn);
-      const int row0 = tm * 2 * kPairRows + static_cast<int>(rank) * kPairRows + 32 * quarter;
-      const int c = tn * kTileN + col0;
       if constexpr (DIGITS) {
         store_digits<Out>(args, r, row0 + lane, c);
         __syncwarp();
         continue;
       }
-      if constexpr (BIAS) add_bias(r, static_cast<const Out*>(args.bias), c, args.n);
+      if constexpr (BIAS) add_bias(r, bias_lo, bias_hi);
       auto stage_slice = [&](uint8_t* buf, int q) {
         if constexpr (OUT == kPairFp32) {
           stage_chunk(buf, lane, r[q]);

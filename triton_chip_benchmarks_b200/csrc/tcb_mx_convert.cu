@@ -455,18 +455,25 @@ __global__ void __launch_bounds__(kThreads)
                      ? __ldg(reinterpret_cast<const uint32_t*>(args.codes + r * pitch + at))
                      : 0u;
     }
+    // ... and scale i is that of row (lane + 32 i) / 4, group lane % 4.
+    float scales[kRows / 8];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int lr = warp * kRows + i;
-      const long long r = r0 + lr;
-      const uint32_t scales = *reinterpret_cast<const uint32_t*>(s_scales + (lr & 31) * 16 + (lr >> 5) * 4);
-      T* dst = static_cast<T*>(args.y) + r * args.ld + c0;
+    for (int i = 0; i < kRows / 8; ++i) {
+      const int lr = warp * kRows + 8 * i + (lane >> 2);
+      scales[i] = scale_value(s_scales[(lr & 31) * 16 + (lr >> 5) * 4 + (lane & 3)]);
+    }
+    const int shift = 4 * (lane & 7);
+    const int rows = static_cast<int>(min(static_cast<long long>(kRows), args.rows - r0 - warp * kRows));
+    const int cols = static_cast<int>(min(static_cast<long long>(kTile), args.cols - c0));
+    T* dst = static_cast<T*>(args.y) + (r0 + warp * kRows) * args.ld + c0 + lane;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i, dst += args.ld) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int c = 32 * g + lane;
         const uint32_t word = __shfl_sync(0xFFFFFFFFu, codes[i / 2], (i & 1) * 16 + 4 * g + (lane >> 3));
-        const float v = decode1(word >> (4 * (lane & 7)) & 15u) * scale_value((scales >> (8 * g)) & 255u);
-        if (r < args.rows && c0 + c < args.cols) dst[c] = from_float<T>(v);
+        const float scale = __shfl_sync(0xFFFFFFFFu, scales[i / 8], (i & 7) * 4 + g);
+        const float v = decode1(word >> shift & 15u) * scale;
+        if (i < rows && 32 * g + lane < cols) dst[32 * g] = from_float<T>(v);
       }
     }
   }
