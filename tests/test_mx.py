@@ -17,7 +17,7 @@ import torch
 
 from oracle import mx as oracle_mx
 from oracle import tensor as oracle_tensor
-from triton_chip_benchmarks_b200 import mx
+from triton_chip_benchmarks_b200 import _native, mx
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 gpu = pytest.mark.gpu
@@ -587,3 +587,57 @@ def test_two_streams_at_once_give_the_same_results(cuda):
         torch.cuda.synchronize()
         for (y, z), a, p in zip(got, alone, products):
             assert same(y, a) and same(z, p)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_products_follow_the_kernels_before_them(cuda, m):
+    """A weight written right before the product that reads it, a workspace and outputs
+    that the next call reuses: results as with everything waited for."""
+    n = k = 4096
+    raw = [torch.randn(n, k, device=cuda, dtype=FP32) for _ in range(3)]
+    xs = [activations((m, k), BF16, seed).to(cuda) for seed in range(3)]
+    waited = []
+    for i in range(9):
+        w = mx.quantize(raw[i % 3])
+        torch.cuda.synchronize()
+        waited.append(mx.linear(xs[i // 3], w))
+        torch.cuda.synchronize()
+    w = mx.MxTensor.empty_on(raw[0], n, k)
+    got = []
+    for i in range(9):
+        _native.mx_quantize(_native.T_FP32, raw[i % 3], n, k, k, _native.MX_FLOOR, w.codes, w.scales)
+        got.append(mx.linear(xs[i // 3], w))
+    for a, b in zip(got, waited):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_offsets_past_32_bits(cuda):
+    """More than 2^32 values and 2^31 bytes of codes: the last rows are as those of a
+    small tensor."""
+    rows, cols, tail = 140000, 32768, 200
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB of device memory")
+    x = torch.zeros(rows, cols, dtype=BF16, device=cuda)
+    x[-tail:] = torch.randn(tail, cols, device=cuda).to(BF16)
+    q = mx.quantize(x)
+    small = mx.quantize(x[-tail:].contiguous())
+    assert torch.equal(q.codes[-tail:], small.codes)
+    assert (q.codes[-tail - 100:-tail] == 0).all()
+    y = torch.full_like(x, 9.0)
+    del x
+    mx.dequantize(q, out=y)
+    assert torch.equal(y[-tail:], mx.dequantize(small))
+    assert (y[rows // 2:-tail] == 0).all()
+    del y
+    # The sums may be split otherwise over K in the small product: both are held to the
+    # exact one.
+    values = f64(mx.dequantize(small, FP32))
+    for m in (1, 5, 20):
+        a = activations((m, cols), BF16, m).to(cuda)
+        check_product(mx.linear(a, q)[:, -tail:], f64(a), values)
+    a = mx.quantize(activations((3, cols), BF16, 9).to(cuda))
+    va = f64(mx.dequantize(a, FP32))
+    check_product(mx.matmul(a, q)[:, -tail:], va, values)
+    check_product(mx.matmul(q, a)[-tail:], values, va)
