@@ -92,13 +92,22 @@ __device__ __forceinline__ uint32_t encode8(const float (&v)[8]) {
   return w;
 }
 
-// The two bf16 values of a word times the bf16 power of two `factor`, in fp32:
-// one instruction a value (adding -0 keeps the sign of zeros).
-__device__ __forceinline__ void scale2(uint32_t w, uint16_t factor, float& lo, float& hi) {
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-      "fma.rn.f32.bf16 %0, l, %3, 0f80000000;\n\tfma.rn.f32.bf16 %1, h, %3, 0f80000000;\n\t}"
-      : "=f"(lo), "=f"(hi)
-      : "r"(w), "h"(factor));
+// The two 16-bit values of a word times powers of two, in fp32.  bf16: one
+// instruction a value (adding -0 keeps the sign of zeros).
+template <typename T>
+__device__ __forceinline__ void scale2(uint32_t w, float inv_lo, float inv_hi, float& lo, float& hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    unpack2<T>(w, lo, hi);
+    lo *= inv_lo;
+    hi *= inv_hi;
+  } else {
+    const uint16_t a = static_cast<uint16_t>(__float_as_uint(inv_lo) >> 16);
+    const uint16_t b = static_cast<uint16_t>(__float_as_uint(inv_hi) >> 16);
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "fma.rn.f32.bf16 %0, l, %3, 0f80000000;\n\tfma.rn.f32.bf16 %1, h, %4, 0f80000000;\n\t}"
+        : "=f"(lo), "=f"(hi)
+        : "r"(w), "h"(a), "h"(b));
+  }
 }
 
 // One E2M1 code (0..15) as fp32: |code| 0 and 1 are 0 and 1/2, the others

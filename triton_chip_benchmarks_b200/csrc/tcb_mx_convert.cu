@@ -133,13 +133,7 @@ __device__ __forceinline__ uint32_t encode_words(const uint32_t* w, uint32_t e8)
     if constexpr (sizeof(T) == 4) {
       v[i] = __uint_as_float(w[i]) * inv;
     } else if (i % 2 == 0) {
-      if constexpr (std::is_same_v<T, __half>) {
-        unpack2<T>(w[i / 2], v[i], v[i + 1]);
-        v[i] *= inv;
-        v[i + 1] *= inv;
-      } else {
-        scale2(w[i / 2], static_cast<uint16_t>(__float_as_uint(inv) >> 16), v[i], v[i + 1]);
-      }
+      scale2<T>(w[i / 2], inv, inv, v[i], v[i + 1]);
     }
   }
   return e8 == 255 ? 0u : encode8(v);
@@ -283,27 +277,28 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : CO
         w[i] = *reinterpret_cast<const uint32_t*>(src + i * kTile * sizeof(T));
         top = top_of<T>(top, w[i]);
       }
+      uint32_t e8[kColsPerWord], codes[kColsPerWord][4];
+#pragma unroll
+      for (int k = 0; k < kColsPerWord; ++k) e8[k] = scale_code(top_bits<T>(magnitude<T>(top, k)), args.up);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if constexpr (sizeof(T) == 4) {
+          codes[0][q] = encode_words<T>(w + 8 * q, e8[0]);
+        } else {
+          float lo[8], hi[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            scale2<T>(w[8 * q + i], inverse_scale(e8[0]), inverse_scale(e8[1]), lo[i], hi[i]);
+          codes[0][q] = e8[0] == 255 ? 0u : encode8(lo);
+          codes[1][q] = e8[1] == 255 ? 0u : encode8(hi);
+        }
+      }
 #pragma unroll
       for (int k = 0; k < kColsPerWord; ++k) {
-        const uint32_t e8 = scale_code(top_bits<T>(magnitude<T>(top, k)), args.up);
-        uint32_t codes[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (sizeof(T) == 4) {
-            codes[q] = encode_words<T>(w + 8 * q, e8);
-          } else {
-            // This column's values of eight rows, two a word.
-            uint32_t pairs[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              pairs[i] = __byte_perm(w[8 * q + 2 * i], w[8 * q + 2 * i + 1], k ? 0x7632 : 0x5410);
-            codes[q] = encode_words<T>(pairs, e8);
-          }
-        }
         const int c = word * kColsPerWord + k;
         *reinterpret_cast<uint4*>(s_codes_t + c * kCodesPitch + group * 16) =
-            make_uint4(codes[0], codes[1], codes[2], codes[3]);
-        s_scales_t[(c & 31) * 16 + (c >> 5) * 4 + group] = static_cast<uint8_t>(e8);
+            make_uint4(codes[k][0], codes[k][1], codes[k][2], codes[k][3]);
+        s_scales_t[(c & 31) * 16 + (c >> 5) * 4 + group] = static_cast<uint8_t>(e8[k]);
       }
     }
     __syncthreads();
