@@ -209,7 +209,11 @@ int tcb_mx_scales_pack(const void *src, void *dst, int rows, int groups, tcb_str
  *            row (low nibble = even column), zeros past cols;
  *   scales : E8M0 of [rows][ceil(cols/32)], in the packed layout of
  *            tcb_mx_scales_pack (tcb_mx_scales_packed_bytes bytes).
- * None of the entry points below has a counterpart in the reference. */
+ * None of the entry points below has a counterpart in the reference.  Their
+ * kernels may start while the kernels before them on `stream` still run, and wait
+ * for those before they touch memory; what a caller sees is stream order.
+ * Outputs must not overlap inputs.  status_dev (may be NULL) is for the
+ * device-side waits of the products. */
 #define TCB_MX_FLOOR 0 /* scale = 2^(floor(log2 max|v|) - 2): OCP MX, values above 6 saturate */
 #define TCB_MX_UP 1    /* least power of two with max|v| <= 6 x scale: nothing saturates */
 
@@ -243,12 +247,13 @@ int tcb_mx_gemm(const void *A, const void *SA, const void *B, const void *SB, co
 /* Y [M][N] = X [M][K] . W [N][K]^T (+ bias [N]) with X in TCB_T_BF16 or TCB_T_FP16
  * (row pitch ldx >= K elements) and only W quantised; Y and bias in `dtype` as
  * above.  X takes part as eight MX FP4 digits of three bits: within a group of 32
- * values of a row, each is taken to 2^-24 of the group's largest.  Infinities and
- * NaN propagate as in the plain product.  Up to 16 rows are bound by
- * reading W once; more cost what an MX FP4 product of eight times the rows costs.
- * workspace (256-byte aligned) holds
- * tcb_mx_linear_workspace_bytes(M, K) bytes that the call overwrites and needs
- * until its work on `stream` is done; it may be NULL where that is 0. */
+ * values of a row, each is taken to 2^-23 of the group's largest.  Infinities and
+ * NaN propagate as in the plain product.  Up to 16 rows are bound by reading W
+ * once; more cost what an MX FP4 product of eight times the rows costs.
+ * workspace (256-byte aligned) holds tcb_mx_linear_workspace_bytes(M, K) bytes
+ * (about 4 M K) that the call overwrites and needs until its work on `stream` is
+ * done; it may be NULL where that is 0.  Calls whose work overlaps need a
+ * workspace each. */
 int tcb_mx_linear(int x_dtype, const void *X, long long ldx, const void *W, const void *SW,
                   const void *bias, int dtype, void *Y, long long ldy, int M, int N, int K,
                   void *workspace, long long workspace_bytes, int *status_dev, tcb_stream_t stream);

@@ -408,8 +408,8 @@ def test_linear_of_activations(cuda, m, n, k, x_dtype):
     w = mx.quantize((activations((n, k), FP32, seed=2) * 0.02).to(cuda))
     vw = f64(mx.dequantize(w, FP32))
     for dtype in (x_dtype, FP32):
-        # A value is off by at most 2^-24 of its group's largest, on average below
-        # the 2^-23 of |x| that the bound has for each of the K terms.
+        # A value is off by at most 2^-23 of its group's largest, which the bound
+        # holds K times over for every term.
         check_product(mx.linear(x.to(cuda), w, dtype=dtype), f64(x), vw)
 
 

@@ -64,6 +64,14 @@
 // barrier set-up and precedes teardown, so neither CTA exits while its peer
 // may still signal its barriers or read its shared memory.
 //
+// C's type (tcb_mx_gemm).  The epilogue rounds a 64-column slice once to 16 bits
+// (one staging chunk instead of two) and adds the bias in fp32 before that; a
+// lane asks for two bias values ahead of the accumulator and the columns get
+// theirs by shuffle (64 broadcast loads after it: 12.9 instead of 12.0 us at
+// 1000 x 4104 x 2072 fp32).  DIGITS: B's rows are the MX FP4 digits of 16-bit rows
+// (tcb_mx_linear with many rows), whose columns the epilogue adds eight by eight.
+// Measured (captured, back to back): 4096^3 to bf16 31 us, 4.4 PFLOP/s; 1024^3 6.6.
+//
 // Counterpart in the reference suite: none (FP4 GEMM is refused at
 // bench_tensor.py:1406-1407); same contract as the single-CTA tcb_gemm path.
 #include <cudaTypedefs.h>

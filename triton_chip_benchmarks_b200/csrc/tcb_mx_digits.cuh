@@ -5,10 +5,11 @@
 // into E2M1 digits,
 //   u_0 = x * 2^-e (|u_0| < 4),  d_i = RNE_E2M1(u_i),  u_{i+1} = 8 (u_i - d_i),
 //   x = sum_i d_i 2^(e - 3i):  |u_i| <= 4 keeps the rounding below 1/2, so each
-// digit gives three bits more.  Eight digits hold a value to 2^-24 of its
-// group's largest: bf16 values down to 2^-16 of it (fp16: 2^-13) without any
-// error, smaller ones as a 24-bit fixed-point number, the precision that an
-// fp32 sum holding the largest has.  The digits are eight rows of an MX tensor
+// digit gives three bits more.  Eight digits hold a value to 2^-23 of its
+// group's largest (half of 8^-7 in units of 2^e, the largest being at least two
+// of them): bf16 values down to 2^-15 of it (fp16: 2^-12) without any error,
+// smaller ones as a fixed-point number of about the precision that an fp32 sum
+// holding the largest has.  The digits are eight rows of an MX tensor
 // whose scales differ by 2^3: a block-scaled MMA multiplies them as it does any
 // rows, and the epilogue adds a token's eight results, smallest first.
 // Infinities and NaN have no digits: they count as zero there, and the NaN scale

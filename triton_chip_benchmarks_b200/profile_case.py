@@ -12,6 +12,8 @@ those launches (CUDA events).
   python -m triton_chip_benchmarks_b200.profile_case tensor --dtype bf16 --tile 256x256x64
   python -m triton_chip_benchmarks_b200.profile_case vector --dtype fp32
   python -m triton_chip_benchmarks_b200.profile_case gemm --dtype fp4 --size 4096
+  python -m triton_chip_benchmarks_b200.profile_case mx --op quantize_pair --shape 0x8192x4096
+  python -m triton_chip_benchmarks_b200.profile_case mx --op linear --shape 1x16384x8192
 """
 
 from __future__ import annotations
@@ -149,6 +151,44 @@ def case_gemm(args) -> dict:
             "teraops": 2 * m * n * k / (ms * 1e9)}
 
 
+def case_mx(args) -> dict:
+    """One MX FP4 operator on random data of m x n x k (quantisation: n x k), checked on
+    the values that its quantised operands stand for."""
+    from . import mx
+    m, n, k = (int(v) for v in args.shape.split("x"))
+    dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}[args.dtype]
+    gen = torch.Generator(device="cuda").manual_seed(0)
+
+    def data(rows, scale=1.0):
+        return (torch.randn(rows, k, device="cuda", generator=gen) * scale).to(dtype)
+
+    w = data(n, 0.02)
+    wq = mx.quantize(w)
+    flops = 0
+    if args.op in ("quantize", "quantize_pair", "dequantize"):
+        run = {"quantize": lambda: mx.quantize(w), "quantize_pair": lambda: mx.quantize_pair(w)[1],
+               "dequantize": lambda: mx.dequantize(wq, dtype)}[args.op]
+        got = run()
+        values = got if args.op == "dequantize" else mx.dequantize(got, dtype)
+        exact = w.t() if args.op == "quantize_pair" else w
+        assert (values.float() - exact.float()).norm() < 0.2 * exact.float().norm(), "values"
+    else:
+        x = data(m)
+        flops = 2 * m * n * k
+        if args.op == "matmul":
+            xq = mx.quantize(x)
+            run, left = (lambda: mx.matmul(xq, wq, dtype=dtype)), mx.dequantize(xq, torch.float32)
+        else:
+            run, left = (lambda: mx.linear(x, wq)), x.float()
+        torch.testing.assert_close(run().float(), left @ mx.dequantize(wq, torch.float32).t(), rtol=2e-2,
+                                   atol=2e-2)
+    run()
+    torch.cuda.synchronize()
+    ms = _time(run, args.launches)
+    return {"case": "mx", "op": args.op, "dtype": args.dtype, "shape": args.shape, "ms_per_launch": ms,
+            **({"teraops": flops / (ms * 1e9)} if flops else {})}
+
+
 def main(argv=None):
     parser = argparse.ArgumentParser(description=__doc__,
                                      formatter_class=argparse.RawDescriptionHelpFormatter)
@@ -163,6 +203,12 @@ def main(argv=None):
     p.add_argument("--mib", type=int, default=1024)
     p.add_argument("--block", type=int, default=4096, help="elements summed per CTA")
     p.add_argument("--threads", type=int, default=256)
+    p.add_argument("--launches", type=int, default=3)
+    p = sub.add_parser("mx")
+    p.add_argument("--op", default="linear",
+                   choices=("quantize", "quantize_pair", "dequantize", "matmul", "linear"))
+    p.add_argument("--shape", default="1x4096x4096", help="m x n x k")
+    p.add_argument("--dtype", default="bf16", choices=("bf16", "fp16", "fp32"))
     p.add_argument("--launches", type=int, default=3)
     p = sub.add_parser("tensor")
     p.add_argument("--dtype", default="bf16", choices=sorted(NATIVE))
@@ -188,7 +234,7 @@ def main(argv=None):
     args = parser.parse_args(argv)
     torch.cuda.set_device(0)
     result = {"copy": case_copy, "read": case_read, "tensor": case_tensor,
-              "vector": case_vector, "gemm": case_gemm}[args.case](args)
+              "vector": case_vector, "gemm": case_gemm, "mx": case_mx}[args.case](args)
     print(json.dumps(result))
 
 
