@@ -641,3 +641,17 @@ def test_offsets_past_32_bits(cuda):
     va = f64(mx.dequantize(a, FP32))
     check_product(mx.matmul(a, q)[:, -tail:], va, values)
     check_product(mx.matmul(q, a)[-tail:], values, va)
+
+
+def test_call_module_refuses_what_the_library_does_not_take(native):
+    calls = native.calls()
+    p = 0x1000  # never dereferenced
+    assert calls.tcb_mx_quantize(0, p, 4, 4, 3, 0, p, p, None, None, None) == native.ERR_INVALID_ARGUMENT
+    assert calls.tcb_mx_gemm(p, p, p, p, None, 0, p, 8, 1 << 32, 8, 32, None, None) == \
+        native.ERR_INVALID_ARGUMENT  # a size past int is not cut off
+    with pytest.raises(TypeError):
+        calls.tcb_mx_dequantize(0, p, p)
+    with pytest.raises(TypeError):
+        calls.tcb_mx_quantize(0, "x", 4, 4, 4, 0, p, p, None, None, None)
+    with pytest.raises(OverflowError):
+        calls.tcb_mx_quantize(0, 1 << 70, 4, 4, 4, 0, p, p, None, None, None)

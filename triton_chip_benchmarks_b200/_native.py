@@ -165,6 +165,30 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_calls = None
+_bound_to: ctypes.CDLL | None = None
+
+
+def calls():
+    """The module of the MX FP4 entry points (integers in, status out), bound to the
+    loaded library; raises NativeLibraryError when it has not been built."""
+    global _calls, _bound_to
+    lib = load()
+    if _bound_to is lib:
+        return _calls
+    with _lock:
+        try:
+            from . import _tcb_calls
+        except ImportError as exc:
+            raise NativeLibraryError(
+                f"cannot import _tcb_calls ({exc}); build it with "
+                "`python -m triton_chip_benchmarks_b200.build`") from exc
+        _tcb_calls.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "tcb_mx_quantize", "tcb_mx_dequantize", "tcb_mx_gemm", "tcb_mx_linear")))
+        _calls, _bound_to = _tcb_calls, lib
+    return _calls
+
+
 def strerror(status: int) -> str:
     try:
         return load().tcb_strerror(status).decode()

@@ -3,7 +3,8 @@
 Compiles every ``csrc/*.cu`` for ``sm_100a`` with nvcc (object files in
 ``_build/`` beside this file, incremental on source/header timestamps) and
 links them, with the CUDA runtime linked statically, into
-``triton_chip_benchmarks_b200/libtcb.so``.  Run ``python -m
+``triton_chip_benchmarks_b200/libtcb.so``; compiles ``csrc/tcb_pycalls.c`` into the
+Python module ``_tcb_calls`` beside it.  Run ``python -m
 triton_chip_benchmarks_b200.build`` or call :func:`build`.
 """
 
@@ -15,6 +16,7 @@ from pathlib import Path
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_DIR = PACKAGE_DIR.parent
@@ -22,6 +24,7 @@ CSRC = PACKAGE_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 BUILD_DIR = PACKAGE_DIR / "_build"
 LIBRARY = PACKAGE_DIR / "libtcb.so"
+CALLS = PACKAGE_DIR / "_tcb_calls.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -67,6 +70,21 @@ def _compile(nvcc: str, source: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_calls() -> None:
+    """The Python module of the MX FP4 entry points (no CUDA in it)."""
+    source = CSRC / "tcb_pycalls.c"
+    if not _stale(CALLS, [source, *_headers()]):
+        return
+    cc = shutil.which("cc") or shutil.which("gcc")
+    if cc is None:
+        raise RuntimeError("no C compiler on PATH")
+    cmd = [cc, "-O2", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"], "-I", str(INCLUDE),
+           "-o", str(CALLS), str(source)]
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"cc failed for {source.name}:\n{result.stdout}\n{result.stderr}")
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     """Compile and link libtcb.so; returns its path."""
     nvcc = nvcc_path()
@@ -74,6 +92,7 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     sources = sorted(CSRC.glob("*.cu"))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs or os.cpu_count() or 4) as pool:
         objects = list(pool.map(lambda src: _compile(nvcc, src, verbose), sources))
+    _build_calls()
     if _stale(LIBRARY, objects):
         cmd = [nvcc, *ARCH_FLAGS, "-shared", "-cudart", "static", "-o", str(LIBRARY),
                *map(str, objects)]

@@ -21,6 +21,7 @@ library itself refuses raises :class:`_native.TcbError`.
 from __future__ import annotations
 
 from dataclasses import dataclass
+import functools
 
 import torch
 
@@ -123,7 +124,7 @@ class MxTensor:
 
 def _call(name: str, index: int, *args) -> None:
     """The library's entry point on the current stream of device `index`, with it current."""
-    fn = getattr(_native.load(), name)
+    fn = getattr(_native.calls(), name)
     if index == _current_device():
         status = fn(*args, _raw_stream(index))
     else:
@@ -282,6 +283,10 @@ def matmul(a: MxTensor, b: MxTensor, *, bias: torch.Tensor | None = None,
     return y
 
 
+# A size for a size: worked out by the library once per pair.
+_workspace_bytes = functools.lru_cache(maxsize=1024)(_native.mx_linear_workspace_bytes)
+
+
 def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
            dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
            status: torch.Tensor | None = None) -> torch.Tensor:
@@ -308,7 +313,7 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
     y, code, pitch = _output(out, w, m, n, x_dtype if dtype is None else dtype)
     bias_ptr = _bias(bias, n, y)
     if m and n:
-        need = _native.mx_linear_workspace_bytes(m, k)
+        need = _workspace_bytes(m, k)
         space = flat.new_empty(need, dtype=torch.uint8) if need else None
         _call("tcb_mx_linear", w.index, _DTYPES[x_dtype], flat.data_ptr(), x_pitch, w.codes_ptr,
               w.scales_ptr, bias_ptr, code, y.data_ptr(), pitch, m, n, k, _native._ptr(space), need,
