@@ -232,33 +232,28 @@ __global__ void __launch_bounds__(256)
 }
 
 // The last step of a CTA: its rows' sums over the ranks in order, the bias, one
-// rounding.  A warp takes every kth token, eight at a time, a lane one row.
-struct Finish {
-  const float* sums;  // [split][tokens][share], shared memory
-  int split, tokens, share, rows;
-  int warp, warps, lane;
-
-  template <typename T>
-  __device__ __forceinline__ void run(const T* bias, long long n0, T* y, long long ldy) const {
-    constexpr int kBatch = 8;
-    for (int row = lane; row < rows; row += 32) {
-      const float b = bias == nullptr ? 0.0f : to_float(bias[n0 + row]);
-      for (int first = warp; first < tokens; first += kBatch * warps) {
-        float v[kBatch] = {};
-        for (int q = 0; q < split; ++q) {
-          const float* s = sums + q * tokens * share + row;
+// rounding.  Item i is row i % share of token i / share (share a power of two).
+template <typename T, int kThreads>
+__device__ __forceinline__ void finish(const float* sums, int split, int tokens, int share_log2, int rows,
+                                       const T* bias, T* y, long long ldy) {
+  constexpr int kBatch = 4;  // loads in flight
+  const int items = tokens << share_log2;
+  for (int first = static_cast<int>(threadIdx.x); first < items; first += kBatch * kThreads) {
+    float v[kBatch] = {};
+    for (int q = 0; q < split; ++q) {
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) v[i] += s[min(first + i * warps, tokens - 1) * share];
-        }
+      for (int u = 0; u < kBatch; ++u)
+        if (first + u * kThreads < items) v[u] += sums[q * items + first + u * kThreads];
+    }
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int token = first + i * warps;
-          if (token < tokens) y[token * ldy + row] = from_float<T>(v[i] + b);
-        }
-      }
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = first + u * kThreads;
+      const int token = i >> share_log2, row = i & ((1 << share_log2) - 1);
+      if (i < items && row < rows)
+        y[token * ldy + row] = from_float<T>(v[u] + (bias == nullptr ? 0.0f : to_float(bias[row])));
     }
   }
-};
+}
 
 template <int XMODE>
 __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
@@ -472,7 +467,8 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   const bool aborted = abort_flag != 0;
   // Row r of the tile belongs to the cluster's rank r / share; the sums of its
   // rows lie in that CTA as [rank of origin][token][r % share].
-  const int share = (kRowTile + args.split - 1) / args.split;
+  const int share_log2 = 31 - __clz(kRowTile / args.split);  // split is a power of two
+  const int share = 1 << share_log2;
   const bool early = tokens <= kEarlyTokens;
   float* sums = reinterpret_cast<float*>(smem + (early ? args.stages * args.stage_bytes : 0));
   if (!early) cluster_sync_all();
@@ -480,7 +476,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     tc_fence_after();
     const int row = 32 * (warp & 3) + lane;
     const uint32_t taddr = tbase + ((32u * (warp & 3)) << 16);
-    const int owner = row / share;
+    const int owner = row >> share_log2;
     const uint32_t to =
         mapa_shared(smem_addr(sums + rank * tokens * share + (row - owner * share)), owner);
     auto send = [&](int token, float v) {
@@ -515,15 +511,19 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     const long long n0 = static_cast<long long>(tile) * kRowTile + rank * share;
     const int rows = static_cast<int>(min(static_cast<long long>(min(share, kRowTile - rank * share)),
                                           args.n - n0));
-    constexpr int kWarps = 6 + (XMODE == kXInline ? kXWarps : 0);
-    const Finish f{sums, args.split, tokens, share, rows, warp, kWarps, lane};
+    constexpr int kThreads = (6 + (XMODE == kXInline ? kXWarps : 0)) * 32;
+    auto run = [&](auto* y) {
+      using T = std::remove_pointer_t<decltype(y)>;
+      const T* bias = static_cast<const T*>(args.bias);
+      finish<T, kThreads>(sums, args.split, tokens, share_log2, rows, bias == nullptr ? bias : bias + n0,
+                          y + n0, args.ldy);
+    };
     if (args.y_type == kRowsFp32)
-      f.run(static_cast<const float*>(args.bias), n0, static_cast<float*>(args.y) + n0, args.ldy);
+      run(static_cast<float*>(args.y));
     else if (args.y_type == kRowsBf16)
-      f.run(static_cast<const __nv_bfloat16*>(args.bias), n0, static_cast<__nv_bfloat16*>(args.y) + n0,
-            args.ldy);
+      run(static_cast<__nv_bfloat16*>(args.y));
     else
-      f.run(static_cast<const __half*>(args.bias), n0, static_cast<__half*>(args.y) + n0, args.ldy);
+      run(static_cast<__half*>(args.y));
   }
   if (warp == 1) {
     tc_fence_after();
@@ -568,7 +568,7 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   for (int split = 2; split <= kMaxSplit; split *= 2)
     if (split <= args.kblocks && tiles * split <= (split < 8 ? 2ll : 1ll) * facts.sm_count) args.split = split;
   if (tiles * args.split > INT_MAX) return TCB_ERR_RESOURCE;
-  constexpr int kSumBytes = kEarlyTokens * (kRowTile + kMaxSplit) * 4;  // a share is rounded up
+  constexpr int kSumBytes = kEarlyTokens * kRowTile * 4;
   args.stages = (kSmemBudget - 1024 - kSumBytes) / args.stage_bytes;
   if (args.stages > kMaxStages) args.stages = kMaxStages;
   const int acc_cols = (args.cols + 31) / 32 * 32;
