@@ -655,3 +655,29 @@ def test_call_module_refuses_what_the_library_does_not_take(native):
         calls.tcb_mx_quantize(0, "x", 4, 4, 4, 0, p, p, None, None, None)
     with pytest.raises(OverflowError):
         calls.tcb_mx_quantize(0, 1 << 70, 4, 4, 4, 0, p, p, None, None, None)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+@pytest.mark.parametrize("n,pitch", [(4096, 4096), (4099, 4099), (4099, 4102), (4100, 4104)])
+def test_matmul_with_more_tiles_than_pairs(cuda, n, pitch, dtype):
+    """Several tiles a CTA pair, with rows of C on and off 16-byte boundaries."""
+    m, k = 2400, 96
+    a, va = mx_random(m, k, seed=1)
+    b, vb = mx_random(n, k, seed=2)
+    bias = rounded(np.random.default_rng(3).integers(-8, 9, n) / 4.0, dtype)
+    exact = va @ vb.T
+    room = torch.full((m, pitch), 9.0, dtype=dtype, device=cuda)
+    mx.matmul(a, b, out=room[:, :n])
+    assert same(room[:, :n], rounded(exact, FP32).to(dtype)) and (room[:, n:] == 9).all()
+    mx.matmul(a, b, out=room[:, :n], bias=bias.to(cuda))
+    assert same(room[:, :n], rounded(exact + f64(bias), FP32).to(dtype)) and (room[:, n:] == 9).all()
+
+
+@gpu
+def test_linear_with_more_tiles_than_pairs(cuda):
+    m, n, k = 300, 2500, 96
+    gen = torch.Generator().manual_seed(0)
+    x = (torch.randint(-16, 17, (m, k), generator=gen) / 4).to(BF16)
+    w, vw = mx_random(n, k, seed=5)
+    assert same(mx.linear(x.to(cuda), w), rounded(f64(x) @ vw.T, FP32).to(BF16))

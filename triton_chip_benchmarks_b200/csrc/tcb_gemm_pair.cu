@@ -75,6 +75,7 @@
 // Counterpart in the reference suite: none (FP4 GEMM is refused at
 // bench_tensor.py:1406-1407); same contract as the single-CTA tcb_gemm path.
 #include <cudaTypedefs.h>
+#include <type_traits>
 
 #include "tcb_device.cuh"
 #include "tcb_gemm_common.cuh"
@@ -120,6 +121,8 @@ static_assert(kAccCols + kPairSlots * kPairSfCols <= kTmemCols, "tensor memory o
 static_assert(kPairSmem <= 227 * 1024 - 256, "shared memory overflow");
 static_assert(kPairSlotOffset % 1024 == 0 && kPairStagingOffset % 1024 == 0,
               "operand stages and staging buffers keep the 1024-byte swizzle alignment");
+constexpr int kPlainBytes = kPairEpiGroups * kEpiChunkBytes / kPairEpiWarps;  // staging of a warp
+static_assert(kPlainBytes == 512, "plain stores turn four rows of 128 bytes round");
 static_assert(kPairEpiCols == 64, "an epilogue warp drains two 32-column loads");
 static_assert(kPairEpiWarps * 2 * kEpiChunkBytes <= kPairStages * kPairStageBytes,
               "the last tile's C slices fit in the operand ring");
@@ -135,8 +138,6 @@ struct PairArgs {
   int tiles_m, tiles_n;
   int kblocks;      // 128-byte K blocks (the last may be ragged)
   int full_panels;  // whole 128-byte K blocks reachable through the 3-D maps (0: none)
-  int vec_store;    // C rows are 16-byte aligned
-  int tma_store;    // C is written through the C tensor map (requires vec_store)
   uint32_t idesc;
   const uint16_t* x;  // DIGITS kernels: the 16-bit rows, A's codes and their row bytes
   const uint8_t* a;
@@ -212,17 +213,69 @@ __device__ __forceinline__ void to_pairs(const uint32_t (&r)[2][32], uint32_t (&
                                __uint_as_float(r[i >> 4][2 * (i & 15) + 1]));
 }
 
-// Direct store of 64 16-bit columns: acc_store's counterpart.
-__device__ __forceinline__ void acc_store16(uint16_t* dst, const uint32_t (&h)[32], int col0, int n,
-                                            bool vec) {
-  if (vec && col0 + 64 <= n) {
+// 32 words of a row a lane (32 fp32 or 64 16-bit columns) to rows of C that TMA
+// cannot write.  STEP rows at a time go through shared memory of the warp's own
+// (128 bytes a row), so that a row leaves as 128 bytes side by side: lane l the word
+// l.  Where a 16-bit row starts between two words, lane l stores the aligned word
+// of columns 2l - 1 and 2l.  `rows` and `cols`: how many there are from the first
+// to C's edge (any number, negative too).  Predicated stores: branches around a
+// row's stores cost about 100 cycles a row.  (4096 x 4095 x 4096 bf16: 180 us with
+// every lane storing its own row, 88 through the two staging buffers in turns, 40
+// so; 31 through the tensor map at N = 4096.)
+template <int STEP, typename T>
+__device__ __forceinline__ void store_plain(const uint32_t (&h)[32], uint8_t* buf, T* c, long long ldc,
+                                            int rows, int cols, int lane) {
+  constexpr int kRows = 4;  // shared loads in flight
+  constexpr int kCols = 128 / static_cast<int>(sizeof(T));
+  // Chunk i of row j at i ^ swizzle(j): neither side has bank conflicts.
+  auto swizzle = [](int j) { return STEP == 4 ? (j & 3) << 1 : j & 7; };
+#pragma unroll 1
+  for (int r = 0; r < 32; r += kRows, c += kRows * ldc, rows -= kRows) {
+    if (r % STEP == 0) {
+      __syncwarp();  // the rows before these have been read
+      if (lane / STEP == r / STEP) {
+        uint8_t* mine = buf + lane % STEP * 128;
 #pragma unroll
-    for (int v = 0; v < 8; ++v)
-      st_stream_u4(dst + 8 * v, h[4 * v], h[4 * v + 1], h[4 * v + 2], h[4 * v + 3]);
-  } else {
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(mine + ((i ^ swizzle(lane)) << 4)) =
+              make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      }
+      __syncwarp();
+    }
+    uint32_t v[kRows], before[kRows];
 #pragma unroll
-    for (int e = 0; e < 64; ++e)
-      if (col0 + e < n) dst[e] = static_cast<uint16_t>(h[e >> 1] >> (16 * (e & 1)));
+    for (int j = 0; j < kRows; ++j) {
+      const int at = (r + j) % STEP;
+      v[j] = *reinterpret_cast<const uint32_t*>(buf + at * 128 + (((lane >> 2) ^ swizzle(at)) << 4) +
+                                                (lane & 3) * 4);
+      if constexpr (sizeof(T) == 2) before[j] = __shfl_up_sync(0xffffffffu, v[j], 1);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < kRows; ++j)
+        if (j < rows && lane < cols) *reinterpret_cast<uint32_t*>(c + j * ldc + lane) = v[j];
+    } else {
+      const bool whole = cols >= kCols;
+#pragma unroll
+      for (int j = 0; j < kRows; ++j) {
+        uint16_t* row = reinterpret_cast<uint16_t*>(c + j * ldc);
+        const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1;
+        const uint32_t w = odd ? __byte_perm(before[j], v[j], 0x5432) : v[j];
+        const bool in = j < rows && whole;
+        if (in && lane >= odd) *reinterpret_cast<uint32_t*>(row + 2 * lane - odd) = w;
+        // The two halves that no whole word holds: column 0 and the last.
+        const uint16_t half = static_cast<uint16_t>(lane == 0 ? v[j] : v[j] >> 16);
+        if (in && odd && (lane == 0 || lane == 31)) row[lane == 0 ? 0 : kCols - 1] = half;
+      }
+      if (!whole) {  // C's right edge
+#pragma unroll
+        for (int j = 0; j < kRows; ++j) {
+          uint16_t* row = reinterpret_cast<uint16_t*>(c + j * ldc) + 2 * lane;
+          if (j < rows && 2 * lane < cols) row[0] = static_cast<uint16_t>(v[j]);
+          if (j < rows && 2 * lane + 1 < cols) row[1] = static_cast<uint16_t>(v[j] >> 16);
+        }
+      }
+    }
   }
 }
 
@@ -250,7 +303,12 @@ __device__ __forceinline__ void store_digits(const PairArgs& args, const uint32_
   }
 }
 
-template <int OUT, bool BIAS, bool DIGITS>
+// How C leaves: through the C tensor map (rows on 16-byte boundaries), by plain
+// stores through the same shared memory, or as a digit product.  A kernel each:
+// the epilogue has 64 of 80 registers in the accumulator slice.
+enum StoreMode : int { kStoreTma = 0, kStorePlain = 1, kStoreDigits = 2 };
+
+template <int OUT, bool BIAS, int STORE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_pair_mxf4_kernel(const __grid_constant__ CUtensorMap map_a,
                           const __grid_constant__ CUtensorMap map_b,
@@ -272,8 +330,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __shared__ volatile int abort_flag;
   __shared__ volatile int store_turn[kPairEpiGroups];     // next staging turn of each group
 
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // An offset from smem_raw, so that the compiler still knows it for shared memory.
+  uint8_t* smem = smem_raw + (-smem_addr(smem_raw) & 1023u);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -292,7 +350,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       prefetch_tensormap(&map_a3);
       prefetch_tensormap(&map_b3);
     }
-    if (args.tma_store) prefetch_tensormap(&map_c);
+    if (STORE == kStoreTma) prefetch_tensormap(&map_c);
     for (int g = 0; g < kPairEpiGroups; ++g) store_turn[g] = 0;
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&loaded[s], 1);
@@ -472,12 +530,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if constexpr (!BIAS) place();
       // A 16-bit slice is one 4 KB staging chunk (64 columns), an fp32 slice two.
       constexpr int kChunks = OUT == kPairFp32 ? 2 : 1;
-      if constexpr (DIGITS) {
+      if constexpr (STORE == kStoreDigits) {
         store_digits<Out>(args, r, row0 + lane, c);
         __syncwarp();
         continue;
       }
       if constexpr (BIAS) add_bias(r, bias_lo, bias_hi);
+      if constexpr (STORE == kStorePlain) {
+        Out* dst = static_cast<Out*>(args.c) + static_cast<long long>(row0) * args.ldc + c;
+        auto store_slice = [&](auto step, uint8_t* own) {
+          constexpr int kStep = decltype(step)::value;
+          if constexpr (OUT == kPairFp32) {
+            store_plain<kStep>(r[0], own, dst, args.ldc, args.m - row0, args.n - c, lane);
+            store_plain<kStep>(r[1], own, dst + 32, args.ldc, args.m - row0, args.n - c - 32, lane);
+          } else {
+            uint32_t h[32];
+            to_pairs<Out>(r, h);
+            store_plain<kStep>(h, own, dst, args.ldc, args.m - row0, args.n - c, lane);
+          }
+        };
+        // The operand ring is idle behind the last tile (see below).
+        if (ti + 1 == my_tiles)
+          store_slice(std::integral_constant<int, 32>{}, smem + (warp - 2) * kEpiChunkBytes);
+        else
+          store_slice(std::integral_constant<int, 4>{},
+                      smem + kPairStagingOffset + (warp - 2) * kPlainBytes);
+        __syncwarp();
+        continue;
+      }
       auto stage_slice = [&](uint8_t* buf, int q) {
         if constexpr (OUT == kPairFp32) {
           stage_chunk(buf, lane, r[q]);
@@ -487,7 +567,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           stage_chunk(buf, lane, h);
         }
       };
-      if (args.tma_store && ti + 1 == my_tiles) {
+      if (ti + 1 == my_tiles) {
         // Last tile: every MMA has finished reading the operand ring (acc_full
         // follows their completion) and no load refills it, so each warp
         // stages its whole slice in 8 KB of the ring of its own and stores it
@@ -505,7 +585,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           bulk_commit_group();
         }
         __syncwarp();
-      } else if (args.tma_store) {
+      } else {
         const int mine = ti * kPairEpiGroupWarps + slot;
         if (!__all_sync(0xffffffffu, turn_wait(mine))) break;
         __threadfence_block();
@@ -522,15 +602,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           __syncwarp();
         }
         if (lane == 0) store_turn[group] = mine + 1;
-      } else if (row0 + lane < args.m) {
-        Out* dst = static_cast<Out*>(args.c) + static_cast<long long>(row0 + lane) * args.ldc + c;
-        if constexpr (OUT == kPairFp32) {
-          acc_store<2>(reinterpret_cast<uint32_t*>(dst), r, c, args.n, args.vec_store);
-        } else {
-          uint32_t h[32];
-          to_pairs<Out>(r, h);
-          acc_store16(reinterpret_cast<uint16_t*>(dst), h, c, args.n, args.vec_store);
-        }
       }
     }
     if (lane == 0) bulk_wait_group_all();  // C stores complete before the CTA retires
@@ -665,17 +736,19 @@ int pair_map_c(CUtensorMap* map, void* base, int rows, int cols, long long ldc, 
 using PairFn = void (*)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, PairArgs);
 
 template <int OUT>
-PairFn pair_fn_of(bool bias, bool digits) {
-  if (digits) return gemm_pair_mxf4_kernel<OUT, false, true>;
-  return bias ? gemm_pair_mxf4_kernel<OUT, true, false> : gemm_pair_mxf4_kernel<OUT, false, false>;
+PairFn pair_fn_of(bool bias, int store) {
+  if (store == kStoreDigits) return gemm_pair_mxf4_kernel<OUT, false, kStoreDigits>;
+  if (store == kStorePlain)
+    return bias ? gemm_pair_mxf4_kernel<OUT, true, kStorePlain> : gemm_pair_mxf4_kernel<OUT, false, kStorePlain>;
+  return bias ? gemm_pair_mxf4_kernel<OUT, true, kStoreTma> : gemm_pair_mxf4_kernel<OUT, false, kStoreTma>;
 }
 
-PairFn pair_fn(int out, bool bias, bool digits) {
+PairFn pair_fn(int out, bool bias, int store) {
   switch (out) {
-    case kPairBf16: return pair_fn_of<kPairBf16>(bias, digits);
-    case kPairFp16: return pair_fn_of<kPairFp16>(bias, digits);
+    case kPairBf16: return pair_fn_of<kPairBf16>(bias, store);
+    case kPairFp16: return pair_fn_of<kPairFp16>(bias, store);
   }
-  return pair_fn_of<kPairFp32>(bias, digits);
+  return pair_fn_of<kPairFp32>(bias, store);
 }
 
 }  // namespace
@@ -708,7 +781,6 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
   args.pitch = kbytes;
   args.x_k = p.digits_k;
   args.x_bf16 = p.digits_bf16;
-  args.vec_store = !digits && p.ldc * elem_bytes % 16 == 0 && aligned(p.c, 16);
   args.idesc = p.idesc;
   CUtensorMap map_a, map_b, map_a3, map_b3;
   int panels_a = static_cast<int>(kbytes / kBlockBytes), panels_b = panels_a;
@@ -717,11 +789,15 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
   if ((rc = pair_maps(&map_b, &map_b3, p.b, p.n, kbytes, &panels_b)) != TCB_OK) return rc;
   args.full_panels = panels_a < panels_b ? panels_a : panels_b;
   CUtensorMap map_c{};
-  args.tma_store =
-      args.vec_store && pair_map_c(&map_c, p.c, p.m, p.n, p.ldc, elem_bytes) == TCB_OK;
-  const PairFn fn = pair_fn(p.out, p.bias != nullptr, digits);
-  static DeviceIntCache cap_cache[3][3], resident_cache;
-  const int cap = cap_cache[p.out][digits ? 2 : p.bias != nullptr].get(facts.device, [&] {
+  // A row's end has to be on a 16-byte boundary too: the store clips whole 16-byte
+  // units at C's edge, and would write zeros between it and the next boundary.
+  const bool tma = p.ldc * elem_bytes % 16 == 0 && static_cast<long long>(p.n) * elem_bytes % 16 == 0 &&
+                   aligned(p.c, 16) && !digits &&
+                   pair_map_c(&map_c, p.c, p.m, p.n, p.ldc, elem_bytes) == TCB_OK;
+  const int store = digits ? kStoreDigits : tma ? kStoreTma : kStorePlain;
+  const PairFn fn = pair_fn(p.out, p.bias != nullptr, store);
+  static DeviceIntCache cap_cache[3][2][3], resident_cache;
+  const int cap = cap_cache[p.out][p.bias != nullptr][store].get(facts.device, [&] {
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
   });
   if (cap < kPairSmem) return TCB_ERR_RESOURCE;
@@ -762,7 +838,7 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
 
 int gemm_pair_info(tcb_kernel_info_t* out) {
   cudaFuncAttributes attr;
-  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(pair_fn(kPairFp32, false, false))) !=
+  if (cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(pair_fn(kPairFp32, false, kStoreTma))) !=
       cudaSuccess)
     return TCB_ERR_DEVICE;
   fill_kernel_info(attr, out);

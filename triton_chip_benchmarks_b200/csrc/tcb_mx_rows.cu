@@ -268,8 +268,8 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
 
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // An offset from smem_raw, so that the compiler still knows it for shared memory.
+  uint8_t* smem = smem_raw + (-smem_addr(smem_raw) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / args.split, rank = blockIdx.x % args.split;
   const int kb0 = static_cast<int>(static_cast<long long>(args.kblocks) * rank / args.split);
