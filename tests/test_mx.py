@@ -265,6 +265,24 @@ def test_quantize_strides_offsets_and_leading_axes(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("start", range(8))
+def test_quantize_rows_off_the_16_byte_boundaries(cuda, dtype, start):
+    """Several tiles, from every start; the last value of X is the storage's last."""
+    gen = torch.Generator().manual_seed(start)
+    for pitch in (385, 390 + start, 404):
+        rows, cols = 300, pitch - start
+        base = torch.randn(rows * pitch, generator=gen).to(dtype)
+        host = base.view(rows, pitch)[:, start:]
+        x = base.cuda().view(rows, pitch)[:, start:]
+        check_quantized(mx.quantize(x), f64(host), "floor")
+        a, b = mx.quantize_pair(x)
+        check_quantized(a, f64(host), "floor")
+        check_quantized(b, f64(host).T, "floor")
+        check_quantized(mx.quantize(x[:, :257]), f64(host[:, :257]), "floor")
+
+
+@gpu
 def test_quantize_nothing(cuda):
     for shape in ((0, 64), (64, 0), (0, 0)):
         a, b = mx.quantize_pair(torch.zeros(shape, device=cuda))
