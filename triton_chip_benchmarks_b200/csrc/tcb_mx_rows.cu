@@ -20,7 +20,7 @@
 // cluster share a row tile, each with a part of K.  Each sends the others their
 // share of its partial sums (stores into distributed shared memory) and adds
 // its own share in rank order: no workspace, the same result every time, and
-// one cluster barrier (the sums of up to kEarlyTokens tokens have room of their
+// one cluster barrier to wait for (the sums of up to kEarlyTokens tokens have room of their
 // own; those of more go where the ring was, which all CTAs must have left).
 //
 // Roles of a CTA (one tile each):
@@ -35,7 +35,7 @@
 // 4096 7.3, 1 x 128256 x 4096 61 (4.6 TB/s), 16 MX rows at 8192 x 8192 10.4.
 // Every wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and MMAs in flight are waited for (bounded
-// too), and nothing is stored.
+// too), the CTA sends and stores nothing, and the status reports it.
 #include <cudaTypedefs.h>
 #include <type_traits>
 
@@ -341,6 +341,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  cluster_arrive_started();
   let_next_kernel_start();
   wait_for_previous_kernels();
   const uint32_t tbase = tmem_slot;
@@ -471,6 +472,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   const int share = 1 << share_log2;
   const bool early = tokens <= kEarlyTokens;
   float* sums = reinterpret_cast<float*>(smem + (early ? args.stages * args.stage_bytes : 0));
+  cluster_wait_started();  // long past by now
   if (!early) cluster_sync_all();
   if (!aborted && warp >= 2 && warp < 6) {
     tc_fence_after();
