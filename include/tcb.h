@@ -247,8 +247,10 @@ int tcb_mx_gemm(const void *A, const void *SA, const void *B, const void *SB, co
 /* Y [M][N] = X [M][K] . W [N][K]^T (+ bias [N]) with X in TCB_T_BF16 or TCB_T_FP16
  * (row pitch ldx >= K elements) and only W quantised; Y and bias in `dtype` as
  * above.  X takes part as eight MX FP4 digits of three bits: within a group of 32
- * values of a row, each is taken to 2^-23 of the group's largest.  Infinities and
- * NaN propagate as in the plain product.  Up to 16 rows are bound by reading W
+ * values of a row, each is taken to 2^-23 of the group's largest.  The first digit
+ * may be a seventh larger than its value, so partial sums that come within that
+ * of fp32's largest number may be infinite.  Infinities and NaN propagate as in
+ * the plain product.  Up to 16 rows are bound by reading W
  * once; more cost what an MX FP4 product of eight times the rows costs.
  * workspace (256-byte aligned) holds tcb_mx_linear_workspace_bytes(M, K) bytes
  * (about 4 M K) that the call overwrites and needs until its work on `stream` is

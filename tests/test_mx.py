@@ -283,6 +283,19 @@ def test_quantize_rows_off_the_16_byte_boundaries(cuda, dtype, start):
 
 
 @gpu
+def test_status_words_are_refused_off_the_device(cuda):
+    w, x = mx.quantize(torch.ones(8, 64, device="cuda")), torch.ones(2, 64, device="cuda", dtype=BF16)
+    for call in (lambda s: mx.matmul(w, w, status=s), lambda s: mx.linear(x, w, status=s)):
+        with pytest.raises(ValueError, match="status"):
+            call(torch.zeros(1, dtype=torch.int32))
+        with pytest.raises(TypeError, match="status"):
+            call(torch.zeros(1, dtype=torch.int64, device="cuda"))
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        call(status)
+        assert status.item() == 0
+
+
+@gpu
 def test_quantize_nothing(cuda):
     for shape in ((0, 64), (64, 0), (0, 0)):
         a, b = mx.quantize_pair(torch.zeros(shape, device=cuda))
@@ -628,6 +641,46 @@ def test_products_follow_the_kernels_before_them(cuda, m):
         got.append(mx.linear(xs[i // 3], w))
     for a, b in zip(got, waited):
         assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 4, 40, 130])
+@pytest.mark.parametrize("k", [512, 2048])
+def test_chains_of_layers_that_reuse_two_buffers(cuda, m, k):
+    """Each call reads what the one before wrote, in a buffer that the one before that
+    read: as with everything waited for, eagerly and in a graph."""
+    weights = [mx.quantize(torch.randn(k, k, device=cuda) * k ** -0.5) for _ in range(3)]
+    start = activations((m, k), BF16, m).to(cuda)
+
+    def chain(waiting):
+        buffers = [start.clone(), torch.empty_like(start)]
+        codes = mx.MxTensor.empty_on(start, m, k)
+        for i in range(24):
+            x, y = buffers[i % 2], buffers[1 - i % 2]
+            if i % 3 == 2:
+                _native.mx_quantize(_native.T_BF16, x, m, k, k, _native.MX_FLOOR, codes.codes, codes.scales)
+                if waiting:
+                    torch.cuda.synchronize()
+                mx.matmul(codes, weights[i % 3], out=y)
+            elif m <= 40:
+                mx.linear(x, weights[i % 3], out=y)
+            else:
+                mx.matmul(mx.quantize(x), weights[i % 3], out=y)
+            if waiting:
+                torch.cuda.synchronize()
+        return buffers[0]
+
+    waited = chain(True)
+    assert waited.isfinite().all() and waited.abs().max() > 0
+    for _ in range(3):
+        assert torch.equal(chain(False), waited)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = chain(False)
+    for _ in range(5):
+        graph.replay()
+    assert torch.equal(captured, waited)
 
 
 @gpu

@@ -279,8 +279,19 @@ def matmul(a: MxTensor, b: MxTensor, *, bias: torch.Tensor | None = None,
     bias_ptr = _bias(bias, n, y)
     if m and n:
         _call("tcb_mx_gemm", a.index, a.codes_ptr, a.scales_ptr, b.codes_ptr, b.scales_ptr, bias_ptr,
-              code, y.data_ptr(), pitch, m, n, k, _native._ptr(status))
+              code, y.data_ptr(), pitch, m, n, k, _status(status, a.index))
     return y
+
+
+def _status(status: torch.Tensor | None, index: int) -> int | None:
+    """Address of a status word on device `index`."""
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() < 1:
+        raise TypeError(f"status is an int32 word, got {status.dtype} {list(status.shape)}")
+    if status.get_device() != index:
+        raise ValueError(f"status is on {status.device}, the operands are on cuda:{index}")
+    return status.data_ptr()
 
 
 # A size for a size: worked out by the library once per pair.
@@ -294,7 +305,9 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
 
     Only the weight is rounded to MX FP4: x takes part as eight MX digits, so up to
     16 rows cost what reading w costs, and many rows eight times as many of
-    :func:`matmul` (quantise x too where that matters).  ``out`` is a matrix [rows][N].
+    :func:`matmul` (quantise x too where that matters).  The first digit may be a
+    seventh larger than its value, so sums that come within that of fp32's largest
+    number may be infinite.  ``out`` is a matrix [rows][N].
     """
     x_dtype = x.dtype
     if x_dtype != torch.bfloat16 and x_dtype != torch.float16:
@@ -317,7 +330,7 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
         space = flat.new_empty(need, dtype=torch.uint8) if need else None
         _call("tcb_mx_linear", w.index, _DTYPES[x_dtype], flat.data_ptr(), x_pitch, w.codes_ptr,
               w.scales_ptr, bias_ptr, code, y.data_ptr(), pitch, m, n, k, _native._ptr(space), need,
-              _native._ptr(status))
+              _status(status, w.index))
     return y if out is not None or flat is x else y.view(*x.shape[:-1], n)
 
 
