@@ -9,13 +9,23 @@
 namespace tcb {
 namespace {
 
-// Up to here the weight's bytes bound the product and the few-row kernel, which
-// spreads them over every SM, is faster than tiles of 256 rows.  Measured
-// (us, few-row / CTA pairs, M = 8, 64, 128): N = K = 4096 6.7/9.4, 9.9/9.8,
-// 13.4/10.3; N = K = 8192 10.6/16.7, 12.8/16.6, 15.4/17.2; N = 4096, K = 1024
-// 4.2/6.0, 6.0/6.4, 7.5/6.8.
-constexpr int kFewRows = 64;
-static_assert(kFewRows <= kRowsMostMx, "one column tile of the few-row kernel");
+// Up to so many rows of A the weight's bytes bound the product, and the few-row
+// kernel, which spreads them over every SM, is faster than tiles of 256 rows:
+// fewest where the tiles of 256 columns keep half of the SMs busy, most where K is
+// long too.  Measured (us, few-row / CTA pairs, M = 8, 48, 64, 96, 128):
+//   N x K   4096 x 4096   5.2/9.2   6.6/9.3   7.0/9.4   7.8/9.6   8.8/9.8
+//           8192 x 8192   9.9/16.5 11.4/16.4 12.3/16.5 13.9/16.7 15.2/17.0
+//           4096 x 1024   3.3/5.7   4.7/5.9   5.2/5.9   6.1/6.1   7.1/6.3
+//           8192 x 1024             6.2/6.0   6.7/6.1   8.2/6.2
+//          12288 x 4096          10.5/13.0 11.9/11.5 13.5/11.7
+//          16384 x 4096   9.8/13.1 11.8/13.0 13.0/12.5 14.5/12.8 16.2/13.0
+int few_rows(int n, int k, const DeviceFacts& facts) {
+  const long long pairs = (static_cast<long long>(n) + 255) / 256;  // with work
+  if (4 * pairs > facts.sm_count) return 48;
+  const int most = 96;
+  static_assert(most <= kRowsMostMx, "one column tile of the few-row kernel");
+  return k >= 2048 ? most : 64;
+}
 
 bool out_type(int dtype, int* rows, int* pair, int* bytes) {
   switch (dtype) {
@@ -49,7 +59,7 @@ extern "C" int tcb_mx_gemm(const void* A, const void* SA, const void* B, const v
   if (rc != TCB_OK) return rc;
   if (facts.major != 10) return TCB_ERR_UNSUPPORTED;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (M <= kFewRows) {
+  if (M <= few_rows(N, K, facts)) {
     const RowsProblem p{A, SA, B, SB, bias, C, 0, ldc, M, N, K, kRowsMx, rows_type};
     return mx_rows_run(p, nullptr, status_dev, facts, s);
   }

@@ -20,8 +20,8 @@
 // cluster share a row tile, each with a part of K.  Each sends the others their
 // share of its partial sums (stores into distributed shared memory) and adds
 // its own share in rank order: no workspace, the same result every time, and
-// one cluster barrier to wait for (the sums of up to kEarlyTokens tokens have room of their
-// own; those of more go where the ring was, which all CTAs must have left).
+// one cluster barrier to wait for (the sums of up to kEarlyTokens tokens have room
+// of their own; those of more go where the ring was, which all CTAs must have left).
 //
 // Roles of a CTA (one tile each):
 //   warp 0      producer: per 256 K values, TMA loads of W (128 rows x 128 B) and X
@@ -31,8 +31,9 @@
 //   warps 6-9   X warps (inline digits only).
 // What bounds it: HBM while the weights stream (25 B/clk per SM at two CTAs), and
 // about 5 us around that: start, first loads, the cluster's join, the end.
-// Captured and back to back: 1 x 16384 x 8192 17.0 us (71 MB, 4.2 TB/s), 1 x 4096 x
-// 4096 7.3, 1 x 128256 x 4096 61 (4.6 TB/s), 16 MX rows at 8192 x 8192 10.4.
+// Captured and back to back: 1 x 16384 x 8192 15.7 us (71 MB, 4.5 TB/s), 1 x 4096 x
+// 4096 6.7, 1 x 128256 x 4096 61 (4.6 TB/s), 16 MX rows at 8192 x 8192 10.0, 16 x
+// 16384 x 8192 19.6 with the digits' kernel.
 // Every wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and MMAs in flight are waited for (bounded
 // too), the CTA sends and stores nothing, and the status reports it.
@@ -563,12 +564,20 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile;
   args.stage_bytes = kWBytes + args.cols * kBlockBytes + 2 * kScaleBlock;
   // A power of two of CTAs to a row tile, each with at least one K block, such
-  // that all fit at once: clusters of four pack two CTAs on every SM, clusters of
-  // seven or eight leave SMs of a GPC over (5000 x 4136, 1 row: 8.5 us with four,
-  // 13.4 with seven; 4096 x 4096, 16 rows: 9.8 with four, 12.2 with eight).
+  // that all run at once, two on an SM: a cluster left over for a second round costs
+  // more than the split saves.  Clusters of four and eight leave places of a GPC
+  // over: of the 296 places of 148 SMs they fill 284 and 264 at most (16 MX rows, K
+  // = 4096: 71 tiles as clusters of four 6.6 us, 72 tiles 10.6, 72 as pairs 7.4; 33
+  // tiles as clusters of eight 5.6, 34 tiles 8.3, 34 as fours 5.4).  Clusters of
+  // eight stop a little earlier, where their join costs more than they save (30
+  // tiles: 5.0 with eight, 5.3 with four; 32 tiles: 5.6 and 5.3), and more CTAs of
+  // them than SMs want two K blocks each (K = 2048, 30 tiles: 4.4 and 4.0).
+  const long long places = 2ll * facts.sm_count;
+  const long long most_in_eights = args.kblocks >= 2 * kMaxSplit ? places - 56 : places / 2;
   args.split = 1;
-  for (int split = 2; split <= kMaxSplit; split *= 2)
-    if (split <= args.kblocks && tiles * split <= (split < 8 ? 2ll : 1ll) * facts.sm_count) args.split = split;
+  if (args.kblocks >= 2 && tiles * 2 <= places) args.split = 2;
+  if (args.kblocks >= 4 && tiles * 4 <= places - 16) args.split = 4;
+  if (args.kblocks >= kMaxSplit && tiles * kMaxSplit <= most_in_eights) args.split = kMaxSplit;
   if (tiles * args.split > INT_MAX) return TCB_ERR_RESOURCE;
   constexpr int kSumBytes = kEarlyTokens * kRowTile * 4;
   args.stages = (kSmemBudget - 1024 - kSumBytes) / args.stage_bytes;
