@@ -44,6 +44,13 @@ def _packed_bytes(rows: int, cols: int) -> int:
     return (rows + 255) // 256 * 256 * ((cols + 255) // 256 * 8)
 
 
+@functools.lru_cache(maxsize=4096)
+def _places(rows: int, cols: int) -> tuple[int, int]:
+    """Where the scales begin behind the codes, and where they end (multiples of 256)."""
+    scales = (_code_bytes(rows, cols) + 255) // 256 * 256
+    return scales, scales + _packed_bytes(rows, cols)
+
+
 class MxTensor:
     """A [rows][cols] MX FP4 matrix.
 
@@ -74,13 +81,32 @@ class MxTensor:
     @classmethod
     def empty_on(cls, other: torch.Tensor, rows: int, cols: int) -> "MxTensor":
         """Uninitialised, codes and scales in one allocation on another tensor's device."""
+        offset, size = _places(rows, cols)
+        held = other.new_empty(size, dtype=torch.uint8)
         t = cls.__new__(cls)
-        offset = (_code_bytes(rows, cols) + 255) // 256 * 256
-        held = other.new_empty(offset + _packed_bytes(rows, cols), dtype=torch.uint8)
         t.rows, t.cols, t.index, t._held = rows, cols, held.get_device(), held
-        t.codes_ptr = held.data_ptr()
-        t.scales_ptr = t.codes_ptr + offset
+        t.codes_ptr = start = held.data_ptr()
+        t.scales_ptr = start + offset
         return t
+
+    @classmethod
+    def two_on(cls, other: torch.Tensor, first: tuple[int, int],
+               second: tuple[int, int]) -> "tuple[MxTensor, MxTensor]":
+        """Two in one allocation, which lives as long as either (an allocation takes
+        the host 1.7 us)."""
+        a, b = cls.__new__(cls), cls.__new__(cls)
+        offset, size = _places(*first)
+        offset_b, size_b = _places(*second)
+        held = other.new_empty(size + size_b, dtype=torch.uint8)
+        a.rows, a.cols = first
+        b.rows, b.cols = second
+        a._held = b._held = held
+        a.index = b.index = held.get_device()
+        a.codes_ptr = start = held.data_ptr()
+        a.scales_ptr = start + offset
+        b.codes_ptr = start + size
+        b.scales_ptr = start + size + offset_b
+        return a, b
 
     @classmethod
     def from_rows(cls, codes: torch.Tensor, scales: torch.Tensor, cols: int) -> "MxTensor":
@@ -106,17 +132,21 @@ class MxTensor:
     def _any(self) -> torch.Tensor:
         return self._held[0] if isinstance(self._held, tuple) else self._held
 
+    def _part(self, address: int, size: int) -> torch.Tensor:
+        return self._held.narrow(0, address - self._held.data_ptr(), size)
+
     @property
     def codes(self) -> torch.Tensor:
         if isinstance(self._held, tuple):
             return self._held[0]
-        return self._held[:_code_bytes(self.rows, self.cols)].view(self.rows, (self.cols + 31) // 32 * 16)
+        return self._part(self.codes_ptr, _code_bytes(self.rows, self.cols)).view(
+            self.rows, (self.cols + 31) // 32 * 16)
 
     @property
     def scales(self) -> torch.Tensor:
         if isinstance(self._held, tuple):
             return self._held[1]
-        return self._held[self.scales_ptr - self.codes_ptr:]
+        return self._part(self.scales_ptr, _packed_bytes(self.rows, self.cols))
 
     def __repr__(self) -> str:
         return f"MxTensor({self.rows} x {self.cols}, {self.device})"
@@ -139,12 +169,6 @@ def _dtype_code(dtype: torch.dtype, what: str) -> int:
     if code is None:
         raise TypeError(f"{what} is bf16, fp16 or fp32, got {dtype}")
     return code
-
-
-def _rule_code(rule: str) -> int:
-    if rule not in RULES:
-        raise ValueError(f"rule is one of {sorted(RULES)}, got {rule!r}")
-    return RULES[rule]
 
 
 def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
@@ -182,26 +206,27 @@ def _device_index(x: torch.Tensor, what: str) -> int:
     return index
 
 
-def _quantize(x: torch.Tensor, rule: str, rows: bool, cols: bool):
-    dtype = _dtype_code(x.dtype, "x")
-    code = _rule_code(rule)
-    index = _device_index(x, "x")
-    if x.dim() != 2:
-        x = _matrix(x, "x")
+def _quantizable(x: torch.Tensor, rule: str) -> torch.Tensor:
+    """x as a matrix, once its type, its device and the rule are known to be quantize's."""
+    _dtype_code(x.dtype, "x")
+    if rule not in RULES:
+        raise ValueError(f"rule is one of {sorted(RULES)}, got {rule!r}")
+    _device_index(x, "x")
+    return x if x.dim() == 2 else _matrix(x, "x")
+
+
+def _quantize(x: torch.Tensor, rule: str, by_row: MxTensor | None, by_col: MxTensor | None) -> None:
+    """The matrix x into by_row (as it is), by_col (transposed) or both."""
     r, c, pitch = _layout(x)
-    swap = pitch is None
-    if swap:  # a transposed view: its rows are the columns of what lies in memory
-        rows, cols = cols, rows
+    if pitch is None:  # a transposed view: its rows are the columns of what lies in memory
+        by_row, by_col = by_col, by_row
         r, c, pitch = _layout(x.t())
         if pitch is None:
             raise ValueError("one axis of x has to be contiguous and its rows must not overlap")
-    by_row = MxTensor.empty_on(x, r, c) if rows else None
-    by_col = MxTensor.empty_on(x, c, r) if cols else None
     if r and c:
-        _call("tcb_mx_quantize", index, dtype, x.data_ptr(), r, c, pitch, code,
-              by_row.codes_ptr if rows else None, by_row.scales_ptr if rows else None,
-              by_col.codes_ptr if cols else None, by_col.scales_ptr if cols else None)
-    return (by_col, by_row) if swap else (by_row, by_col)
+        _call("tcb_mx_quantize", x.get_device(), _DTYPES[x.dtype], x.data_ptr(), r, c, pitch, RULES[rule],
+              by_row and by_row.codes_ptr, by_row and by_row.scales_ptr,
+              by_col and by_col.codes_ptr, by_col and by_col.scales_ptr)
 
 
 def quantize(x: torch.Tensor, *, rule: str = "floor") -> MxTensor:
@@ -213,12 +238,19 @@ def quantize(x: torch.Tensor, *, rule: str = "floor") -> MxTensor:
     with an infinity or a NaN becomes NaN as a whole.  A transposed view is read in
     place.
     """
-    return _quantize(x, rule, True, False)[0]
+    x = _quantizable(x, rule)
+    rows = MxTensor.empty_on(x, *x.shape)
+    _quantize(x, rule, rows, None)
+    return rows
 
 
 def quantize_pair(x: torch.Tensor, *, rule: str = "floor") -> tuple[MxTensor, MxTensor]:
     """quantize(x) and quantize(x^T) (x as a matrix [rows][cols]) in one read of x."""
-    return _quantize(x, rule, True, True)
+    x = _quantizable(x, rule)
+    r, c = x.shape
+    rows, cols = MxTensor.empty_on(x, r, c), MxTensor.empty_on(x, c, r)  # either may outlive the other
+    _quantize(x, rule, rows, cols)
+    return rows, cols
 
 
 def dequantize(q: MxTensor, dtype: torch.dtype = torch.bfloat16, *,
@@ -357,8 +389,14 @@ def linear_forward(x: torch.Tensor, w: torch.Tensor, *,
         raise ValueError(f"x is [..., in] and w [out][in], got {list(x.shape)} and {list(w.shape)}")
     if x.get_device() != w.get_device():
         raise ValueError(f"x is on {x.device} and w on {w.device}")
-    x_rows, x_cols = quantize_pair(x, rule=rule)
-    w_rows, w_cols = quantize_pair(w, rule=rule)
+    flat = _quantizable(x, rule)
+    _quantizable(w, rule)
+    tokens, inner = flat.shape
+    outer = w.shape[0]
+    x_rows, w_rows = MxTensor.two_on(w, (tokens, inner), (outer, inner))
+    x_cols, w_cols = MxTensor.two_on(w, (inner, tokens), (inner, outer))
+    _quantize(flat, rule, x_rows, x_cols)
+    _quantize(w, rule, w_rows, w_cols)
     y = matmul(x_rows, w_rows, dtype=x.dtype)
     saved = LinearSaved(x_cols, w_cols, tuple(x.shape), x.dtype, w.dtype, rule)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0]), saved
@@ -377,9 +415,17 @@ def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = Tru
         raise ValueError(f"dy is {list(shape)}, got {list(dy.shape)}")
     if dy.get_device() != saved.x.index:
         raise ValueError(f"dy is on {dy.device}, the forward pass was on {saved.x.device}")
-    dy_rows, dy_cols = _quantize(dy, saved.rule, need_dx, need_dw) \
-        if need_dx or need_dw else (None, None)
-    dx = dw = None
+    dx = dw = dy_rows = dy_cols = None
+    if need_dx or need_dw:
+        flat = _quantizable(dy, saved.rule)
+        tokens = flat.shape[0]
+        if need_dx and need_dw:
+            dy_rows, dy_cols = MxTensor.two_on(flat, (tokens, out_features), (out_features, tokens))
+        elif need_dx:
+            dy_rows = MxTensor.empty_on(flat, tokens, out_features)
+        else:
+            dy_cols = MxTensor.empty_on(flat, out_features, tokens)
+        _quantize(flat, saved.rule, dy_rows, dy_cols)
     if need_dx:
         dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype)
         if len(saved.x_shape) != 2:
