@@ -752,3 +752,50 @@ def test_linear_with_more_tiles_than_pairs(cuda):
     x = (torch.randint(-16, 17, (m, k), generator=gen) / 4).to(BF16)
     w, vw = mx_random(n, k, seed=5)
     assert same(mx.linear(x.to(cuda), w), rounded(f64(x) @ vw.T, FP32).to(BF16))
+
+
+@gpu
+@pytest.mark.parametrize("x_dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n,k", [(17, 1, 40), (32, 130, 257), (33, 513, 300), (130, 1000, 130),  # column tiles
+                                   (17, 19001, 70), (33, 18945, 300), (130, 2200, 130)])  # CTA pairs
+def test_linear_of_more_rows_than_a_column_tile(cuda, m, n, k, x_dtype):
+    gen = torch.Generator().manual_seed(m + n + k)
+    x = (torch.randint(-16, 17, (m, k), generator=gen) / 4).to(x_dtype)
+    w, vw = mx_random(n, k, seed=n + k, low=125, high=130)
+    # Terms are multiples of 2^-5; their absolute values sum to below 2^19.
+    assert (np.abs(f64(x)) @ np.abs(vw).T).max() < 2.0**24 * 2.0**-5
+    exact = f64(x) @ vw.T
+    for dtype in (x_dtype, FP32):
+        bias = rounded(np.random.default_rng(m).integers(-8, 9, n) / 4.0, dtype)
+        got = mx.linear(x.to(cuda), w, bias=bias.to(cuda), dtype=dtype)
+        assert same(got, rounded(exact + f64(bias), FP32).to(dtype))
+    # Into a pitched output, whose gap stays as it is.
+    wide = torch.full((m, n + 5), 7.0, dtype=x_dtype, device=cuda)
+    mx.linear(x.to(cuda), w, out=wide[:, :n])
+    assert same(wide[:, :n], rounded(exact, FP32).to(x_dtype)) and (wide[:, n:] == 7).all()
+    # Infinities and NaN in their rows alone.
+    x[0, 1], x[m - 1, k - 1], x[16, 5] = float("inf"), -float("inf"), float("nan")
+    with np.errstate(invalid="ignore"):
+        exact = f64(x) @ vw.T
+    assert same(mx.linear(x.to(cuda), w, dtype=FP32), rounded(exact, FP32))
+
+
+@gpu
+def test_linear_of_many_rows_follows_the_kernels_before_it(cuda):
+    """Column tiles, and pairs, whose weight and workspace the calls before have just written."""
+    for m, n, k in ((40, 1024, 2048), (40, 19200, 512)):
+        raw = [torch.randn(n, k, device=cuda) for _ in range(2)]
+        xs = [activations((m, k), BF16, seed).to(cuda) for seed in range(2)]
+        waited = []
+        for i in range(6):
+            w = mx.quantize(raw[i % 2])
+            torch.cuda.synchronize()
+            waited.append(mx.linear(xs[i // 3], w))
+            torch.cuda.synchronize()
+        w = mx.MxTensor.empty_on(raw[0], n, k)
+        got = []
+        for i in range(6):
+            _native.mx_quantize(_native.T_FP32, raw[i % 2], n, k, k, _native.MX_FLOOR, w.codes, w.scales)
+            got.append(mx.linear(xs[i // 3], w))
+        for a, b in zip(got, waited):
+            assert torch.equal(a, b)

@@ -14,7 +14,9 @@
 // the digits of its K slice into shared memory on the way; for more rows a
 // kernel of their own writes them once (into the caller's workspace), and the
 // product starts beside it: its weight loads are under way before the digits
-// are there.  More than kRowsMostDigits rows become columns of the CTA-pair GEMM.
+// are there.  16 rows fill the 128 columns of a tile; column tiles share the weight
+// through L2 while there is an SM for each, and more digits than that become
+// columns of the CTA-pair GEMM.
 //
 // Split over K.  With fewer row tiles than CTAs fit, up to eight CTAs of a
 // cluster share a row tile, each with a part of K.  Each sends the others their
@@ -98,6 +100,7 @@ struct RowsArgs {
   int split;             // CTAs of a cluster
   int stages, stage_bytes;
   int cols;              // columns of the MMA (a multiple of 8, at most 128)
+  int col_tiles;         // of 128 columns each, if there are more than one
   int x_bf16;
   int y_type;            // RowsType of y and the bias
   uint32_t idesc;
@@ -272,12 +275,15 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   // An offset from smem_raw, so that the compiler still knows it for shared memory.
   uint8_t* smem = smem_raw + (-smem_addr(smem_raw) & 1023u);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tile = blockIdx.x / args.split, rank = blockIdx.x % args.split;
+  // Column tiles of the same weight rows side by side: the weight comes from L2.
+  const int rank = blockIdx.x % args.split, both = blockIdx.x / args.split;
+  const int tile = both / args.col_tiles, col_tile = both % args.col_tiles;
   const int kb0 = static_cast<int>(static_cast<long long>(args.kblocks) * rank / args.split);
   const int kb1 = static_cast<int>(static_cast<long long>(args.kblocks) * (rank + 1) / args.split);
   const int nkb = kb1 - kb0;
   constexpr int kPerToken = XMODE == kXRows ? 1 : kDigits;  // columns of a token
-  const int tokens = args.m;
+  const int token0 = col_tile * (kRowTile / kPerToken);
+  const int tokens = min(args.m - token0, kRowTile / kPerToken);
   const int x_bytes = args.cols * kBlockBytes;
 
   auto load_w = [&](int it, int s) {
@@ -294,9 +300,10 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     uint8_t* stage = smem + s * args.stage_bytes;
     uint64_t* bar = &loaded[s];
     const int kb = kb0 + it;
-    tma_load_2d(stage + kWBytes, &map_x, kb * kBlockBytes, 0, bar);
+    tma_load_2d(stage + kWBytes, &map_x, kb * kBlockBytes, col_tile * kRowTile, bar);
     bulk_load_1d(stage + kWBytes + x_bytes + kScaleBlock,
-                 args.sx + static_cast<long long>(kb) * kScaleBlock, kScaleBlock, bar);
+                 args.sx + (static_cast<long long>(col_tile) * args.kblocks + kb) * kScaleBlock, kScaleBlock,
+                 bar);
   };
   // An X warp's next values (inline digits): asked for one round ahead, the first
   // ones before the weights, behind whose bytes they would otherwise queue.
@@ -499,7 +506,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
         float sum = sum_digits(r, &odd);
         const long long n = static_cast<long long>(tile) * kRowTile + row;
         if (odd && n < args.n)
-          sum += odd_products(static_cast<const uint16_t*>(args.x) + token * args.ldx, args.x_bf16, args.w,
+          sum += odd_products(static_cast<const uint16_t*>(args.x) + (token0 + token) * args.ldx, args.x_bf16, args.w,
                               args.pitch, args.sw, args.kblocks, n, kb0 * kBlockK,
                               static_cast<int>(min(static_cast<long long>(kb1) * kBlockK,
                                                    static_cast<long long>(args.k))));
@@ -519,7 +526,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
       using T = std::remove_pointer_t<decltype(y)>;
       const T* bias = static_cast<const T*>(args.bias);
       finish<T, kThreads>(sums, args.split, tokens, share_log2, rows, bias == nullptr ? bias : bias + n0,
-                          y + n0, args.ldy);
+                          y + token0 * args.ldy + n0, args.ldy);
     };
     if (args.y_type == kRowsFp32)
       run(static_cast<float*>(args.y));
@@ -561,7 +568,9 @@ struct DigitSpace {
 
 template <int XMODE>
 int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, const DeviceFacts& facts, cudaStream_t stream) {
-  const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile;
+  args.col_tiles = (args.cols + kRowTile - 1) / kRowTile;
+  if (args.cols > kRowTile) args.cols = kRowTile;
+  const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile * args.col_tiles;
   args.stage_bytes = kWBytes + args.cols * kBlockBytes + 2 * kScaleBlock;
   // A power of two of CTAs to a row tile, each with at least one K block, such
   // that all run at once, two on an SM: a cluster left over for a second round costs
@@ -631,7 +640,7 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
   if (rc != TCB_OK) return rc;
   if (p.x_type == kRowsMx) {
     args.cols = (p.m + 7) / 8 * 8;
-    if ((rc = rows_map(&map_x, p.x, p.m, args.pitch, args.cols)) != TCB_OK) return rc;
+    if ((rc = rows_map(&map_x, p.x, p.m, args.pitch, args.cols < kRowTile ? args.cols : kRowTile)) != TCB_OK) return rc;
     return launch_rows<kXRows>(map_w, map_x, args, facts, stream);
   }
   if (p.m <= kInlineTokens) {
@@ -647,7 +656,13 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
                           static_cast<int>(aligned(p.x, 16) && p.ldx % 8 == 0), args.x_bf16,
                           base + space.codes_at, base);
   if (rc != TCB_OK) return rc;
-  if (p.m > kRowsMostDigits) {
+  args.cols = p.m * kDigits;
+  // Measured (us, here / pairs, 24, 33, 48 and 64 rows): N x K = 4096 x 4096 10.8/11.6
+  // 11.6/12.0 12.3/12.6 12.8/12.9; 1024 x 4096 7.7/11.5 9.2/11.6 9.3/11.8 9.9/11.8; 5000 x
+  // 4136 11.8/12.3 12.8/13.1 13.0/13.4, 160 tiles 16.6/14.2; 16384 x 4096, 384 tiles
+  // 26.8/24.5; 256 x 8192, 256 rows 16.6/22.3.
+  const long long row_tiles = (static_cast<long long>(p.n) + kRowTile - 1) / kRowTile;
+  if (args.cols > kRowTile && (args.cols + kRowTile - 1) / kRowTile * row_tiles > facts.sm_count) {
     // Columns of the CTA-pair GEMM, whose M side is the weight.
     PairProblem q = {};
     q.a = p.w;
@@ -670,8 +685,7 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
     return gemm_pair_run(q, 0, status, facts, stream);
   }
   args.sx = base;
-  args.cols = p.m * kDigits;
-  if ((rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols)) != TCB_OK) return rc;
+  if ((rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols < kRowTile ? args.cols : kRowTile)) != TCB_OK) return rc;
   return launch_rows<kXDigits>(map_w, map_x, args, facts, stream);
 }
 

@@ -9,11 +9,8 @@ namespace tcb {
 
 enum RowsType : int { kRowsFp32 = 0, kRowsBf16 = 1, kRowsFp16 = 2, kRowsMx = 3 };
 
-// MX rows of a call at most, and 16-bit rows that the few-row kernel takes itself
-// (of more it makes columns of the CTA-pair GEMM; us, few-row / pair: 4096 x 4096
-// 9.7/11.5 for 16 rows, 14.2/12.9 for 64; 16384 x 8192 20.8/23.6 and 51/36).
+// MX rows of a call at most (one column tile).
 constexpr int kRowsMostMx = 128;
-constexpr int kRowsMostDigits = 16;
 
 struct RowsProblem {
   const void* x;     // [m] rows of x_type, pitch ldx elements (MX: codes, whole groups)
