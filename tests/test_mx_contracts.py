@@ -1,0 +1,23 @@
+"""What the MX FP4 operators promise beside their values: how their kernels read memory,
+and what happens at the edges of the calls."""
+
+import re
+
+from conftest import REPO
+
+CSRC = REPO / "triton_chip_benchmarks_b200" / "csrc"
+
+
+def code(path) -> str:
+    """A source without its comments."""
+    return re.sub(r"//[^\n]*", "", re.sub(r"/\*.*?\*/", "", path.read_text(), flags=re.S))
+
+
+def test_kernels_that_start_early_read_with_ordinary_loads():
+    """A kernel launched beside the writers of its inputs must not use the read-only
+    path, which is for memory that nobody writes while the kernel runs."""
+    early = [p for p in sorted(CSRC.glob("*.cu")) if "wait_for_previous_kernels" in code(p)]
+    assert {p.name for p in early} >= {"tcb_mx_convert.cu", "tcb_mx_rows.cu", "tcb_gemm_pair.cu"}
+    for path in [*early, *sorted(CSRC.glob("tcb_mx*.cuh"))]:
+        for word in ("__ldg", "__restrict__", "ld.global.nc", "__ldca", "__ldcg"):
+            assert word not in code(path), (path.name, word)

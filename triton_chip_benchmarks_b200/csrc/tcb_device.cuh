@@ -77,7 +77,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
 
 // Programmatic dependent launch.  A kernel launched with the attribute may start
 // while the kernels before it in the stream still run: it waits for them (and
-// their memory) here, before it touches global memory.  A no-op otherwise.
+// their memory) here, before it touches global memory.  A no-op otherwise.  Its
+// inputs may be written while it runs, so they are read with ordinary loads: the
+// read-only path (ld.global.nc: __ldg, const __restrict__ pointers) is for memory
+// that nobody writes during the kernel's life.
 __device__ __forceinline__ void wait_for_previous_kernels() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

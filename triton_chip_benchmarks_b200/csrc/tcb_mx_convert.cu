@@ -70,9 +70,9 @@ constexpr int kWords = kVec * static_cast<int>(sizeof(T)) / 4;
 
 // 16 bytes of a row, zero past its end; `valid` values are in the matrix.
 template <typename T>
-__device__ __forceinline__ uint4 load_edge(const T* __restrict__ p, int valid) {
+__device__ __forceinline__ uint4 load_edge(const T* p, int valid) {
   constexpr int kPer = 16 / sizeof(T);
-  if (valid >= kPer) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (valid >= kPer) return *reinterpret_cast<const uint4*>(p);
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : CO
       for (int i = 0; i < kPasses; ++i)
 #pragma unroll
         for (int q = 0; q < kChunks; ++q)
-          raw[i][q] = __ldg(reinterpret_cast<const uint4*>(p + i * kRowsPerPass * args.ld) + q);
+          raw[i][q] = reinterpret_cast<const uint4*>(p + i * kRowsPerPass * args.ld)[q];
     } else {
       const long long left = args.cols - c0 - col;
 #pragma unroll
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? (COLS ? 3 : 2) : CO
           const char* p = reinterpret_cast<const char*>(x + (r0 + lr0 + (i + j) * kStep) * args.ld + at);
           m[j] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
           const uint4* q = reinterpret_cast<const uint4*>(p - m[j]);
-          lo[j] = __ldg(q);
-          hi[j] = __ldg(q + 1);
+          lo[j] = q[0];
+          hi[j] = q[1];
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j)
@@ -437,13 +437,13 @@ __global__ void __launch_bounds__(kThreads)
     for (int p = 0; p < kDeqPasses; ++p) {
       const long long r = r0 + row + p * kDeqRows;
       w[p] = valid > 0 && r < args.rows
-                 ? __ldg(reinterpret_cast<const uint32_t*>(args.codes + r * pitch + (c0 + col) / 2))
+                 ? *reinterpret_cast<const uint32_t*>(args.codes + r * pitch + (c0 + col) / 2)
                  : 0u;
     }
   }
   if (tid < kHalfBytes / 16)
-    reinterpret_cast<uint4*>(s_scales)[tid] = __ldg(
-        reinterpret_cast<const uint4*>(args.scales + (ty * mx_tiles(args.cols) + tx) * kHalfBytes) + tid);
+    reinterpret_cast<uint4*>(s_scales)[tid] =
+        reinterpret_cast<const uint4*>(args.scales + (ty * mx_tiles(args.cols) + tx) * kHalfBytes)[tid];
   __syncthreads();
   if constexpr (VEC) {
 #pragma unroll
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kThreads)
       const long long r = r0 + warp * kRows + 2 * i + (lane >> 4);
       const long long at = c0 / 2 + (lane & 15) * 4;
       codes[i] = r < args.rows && at < pitch
-                     ? __ldg(reinterpret_cast<const uint32_t*>(args.codes + r * pitch + at))
+                     ? *reinterpret_cast<const uint32_t*>(args.codes + r * pitch + at)
                      : 0u;
     }
     // ... and scale i is that of row (lane + 32 i) / 4, group lane % 4.

@@ -140,11 +140,11 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
 
 // The 16-bit values x[k..k+7] of a row, zeros past the end.
 __device__ __forceinline__ uint4 load_values(const uint16_t* row, int k, int end, bool vec) {
-  if (vec && k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (vec && k + 8 <= end) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (k + i < end) w[i / 2] |= static_cast<uint32_t>(__ldg(row + k + i)) << (16 * (i & 1));
+    if (k + i < end) w[i / 2] |= static_cast<uint32_t>(row[k + i]) << (16 * (i & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -202,9 +202,8 @@ __device__ __forceinline__ uint32_t next_digit(float (&u)[8]) {
 // Digits of all tokens as rows of an MX tensor, one warp per token and K block:
 // digit i of token j is row 8 j + i.
 __global__ void __launch_bounds__(256)
-    mx_digits_kernel(const uint16_t* __restrict__ x, long long ldx, int m, int k, long long pitch,
-                     int kblocks, int vec, int bf16, uint8_t* __restrict__ codes,
-                     uint8_t* __restrict__ scales) {
+    mx_digits_kernel(const uint16_t* x, long long ldx, int m, int k, long long pitch, int kblocks, int vec,
+                     int bf16, uint8_t* codes, uint8_t* scales) {
   // The product may start once the kernels before this one are done: its weight
   // may be theirs.
   wait_for_previous_kernels();
