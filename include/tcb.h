@@ -246,14 +246,15 @@ int tcb_mx_gemm(const void *A, const void *SA, const void *B, const void *SB, co
 
 /* Y [M][N] = X [M][K] . W [N][K]^T (+ bias [N]) with X in TCB_T_BF16 or TCB_T_FP16
  * (row pitch ldx >= K elements) and only W quantised; Y and bias in `dtype` as
- * above.  X takes part as eight MX FP4 digits of three bits: within a group of 32
- * values of a row, each is taken to 2^-23 of the group's largest.  The first digit
- * may be a seventh larger than its value, so partial sums that come within that
- * of fp32's largest number may be infinite.  Infinities and NaN propagate as in
- * the plain product.  Up to 16 rows are bound by reading W
- * once; more cost what an MX FP4 product of eight times the rows costs.
+ * above.  X is not rounded: it takes part as MX FP4 digits of three bits, and what they
+ * leave of a value (small ones beside a large one in a group of 32, groups below about
+ * 2^-105, values from 2^126 on) as products in fp32, so products and sums are those of
+ * fp32.  The first digit may be a seventh larger than its value, so partial sums that
+ * come within that of fp32's largest number may be infinite.  Infinities and NaN propagate
+ * as in the plain product.  Rows that leave much (a large value in every group) take
+ * longer.
  * workspace (256-byte aligned) holds tcb_mx_linear_workspace_bytes(M, K) bytes
- * (about 4 M K) that the call overwrites and needs until its work on `stream` is
+ * (about 5 M K) that the call overwrites and needs until its work on `stream` is
  * done; it may be NULL where that is 0.  Calls whose work overlaps need a
  * workspace each. */
 int tcb_mx_linear(int x_dtype, const void *X, long long ldx, const void *W, const void *SW,

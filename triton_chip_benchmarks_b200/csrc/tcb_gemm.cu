@@ -543,7 +543,7 @@ extern "C" int tcb_gemm(int dtype, const void* A, const void* B, const void* SA,
   if (kind == gMXF4 && M > 128) {
     // CTA pairs: 256 x 256 tiles, each CTA loading 128 rows of A and of B.
     const PairProblem p{A, B, SA, SB, nullptr, C, N, M, N, K, kPairFp32, gemm_pair_idesc(),
-                        false, nullptr, 0, 0, 0};
+                        false, nullptr, nullptr};
     return gemm_pair_run(p, blocks, status_dev, facts, reinterpret_cast<cudaStream_t>(stream));
   }
   const int halves = gemm_halves(kind, M, N, facts.sm_count);

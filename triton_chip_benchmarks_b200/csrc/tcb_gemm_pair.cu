@@ -69,7 +69,8 @@
 // lane asks for two bias values ahead of the accumulator and the columns get
 // theirs by shuffle (64 broadcast loads after it: 12.9 instead of 12.0 us at
 // 1000 x 4104 x 2072 fp32).  DIGITS: B's rows are the MX FP4 digits of 16-bit rows
-// (tcb_mx_linear with many rows), whose columns the epilogue adds eight by eight.
+// (tcb_mx_linear with many rows), whose columns the epilogue adds nine by nine; while a
+// tile's MMAs run its warps multiply what the digits leave.
 // Measured (captured, back to back): 4096^3 to bf16 31 us, 4.4 PFLOP/s; 1024^3 6.6.
 //
 // Counterpart in the reference suite: none (FP4 GEMM is refused at
@@ -124,6 +125,7 @@ static_assert(kPairSlotOffset % 1024 == 0 && kPairStagingOffset % 1024 == 0,
 constexpr int kPlainBytes = kPairEpiGroups * kEpiChunkBytes / kPairEpiWarps;  // staging of a warp
 static_assert(kPlainBytes == 512, "plain stores turn four rows of 128 bytes round");
 static_assert(kPairEpiCols == 64, "an epilogue warp drains two 32-column loads");
+static_assert(mx_detail::SliceDigits::kRows == kPairEpiCols, "a slice is a list's tokens");
 static_assert(kPairEpiWarps * 2 * kEpiChunkBytes <= kPairStages * kPairStageBytes,
               "the last tile's C slices fit in the operand ring");
 
@@ -139,10 +141,10 @@ struct PairArgs {
   int kblocks;      // 128-byte K blocks (the last may be ragged)
   int full_panels;  // whole 128-byte K blocks reachable through the 3-D maps (0: none)
   uint32_t idesc;
-  const uint16_t* x;  // DIGITS kernels: the 16-bit rows, A's codes and their row bytes
-  const uint8_t* a;
-  long long ldx, pitch;
-  int x_k, x_bf16;
+  mx_detail::ValueRows x;            // DIGITS kernels: the 16-bit rows,
+  const mx_detail::LeftList* lists;  // what their digits leave,
+  const uint8_t* a;                  // A's codes and their row bytes
+  long long pitch;
 };
 
 __device__ __forceinline__ void pair_mma_mxf4(uint32_t d, uint64_t adesc, uint64_t bdesc,
@@ -279,26 +281,28 @@ __device__ __forceinline__ void store_plain(const uint32_t (&h)[32], uint8_t* bu
   }
 }
 
-// DIGITS: B's rows are eight digits a token.  A lane (a row n of A) adds the eight
-// columns of each of its slice's eight tokens and stores C[token][n]: 32
-// neighbours a store.
+// DIGITS: a slice of 64 columns is the digits of seven tokens.  A lane (a row n of A)
+// adds each token's columns, and what the digits leave (null: nothing), and stores
+// C[token][n]: 32 neighbours a store.
 template <typename T>
-__device__ __forceinline__ void store_digits(const PairArgs& args, const uint32_t (&r)[2][32], int n, int c) {
+__device__ __forceinline__ void store_digits(const PairArgs& args, const uint32_t (&r)[2][32], int n, int token0,
+                                             const float* left) {
+  using mx_detail::SliceDigits;
   if (n >= args.m) return;
   const T* bias = static_cast<const T*>(args.bias);
   const float b = bias == nullptr ? 0.0f : mx_detail::to_float(bias[n]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float v[8];
+  for (int i = 0; i < SliceDigits::kTokens; ++i) {
+    float v[SliceDigits::kDigits];
 #pragma unroll
-    for (int d = 0; d < 8; ++d) v[d] = __uint_as_float(r[i >> 2][8 * (i & 3) + d]);
-    bool odd;
-    float sum = mx_detail::sum_digits(v, &odd);
-    const int token = c / mx_detail::kDigits + i;
-    if (token * mx_detail::kDigits >= args.n) break;
-    if (odd)
-      sum += mx_detail::odd_products(args.x + token * args.ldx, args.x_bf16, args.a, args.pitch, args.sa,
-                                     args.kblocks, n, 0, args.x_k);
+    for (int d = 0; d < SliceDigits::kDigits; ++d) {
+      const int column = i * SliceDigits::kDigits + d;
+      v[d] = __uint_as_float(r[column >> 5][column & 31]);
+    }
+    float sum = mx_detail::sum_digits<SliceDigits::kDigits>(v);
+    const int token = token0 + i;
+    if (token >= args.x.m) break;
+    if (left != nullptr) sum += left[i];
     static_cast<T*>(args.c)[token * args.ldc + n] = mx_detail::from_float<T>(sum + b);
   }
 }
@@ -517,6 +521,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (c + lane < args.n) bias_lo = mx_detail::to_float(bias[c + lane]);
         if (c + 32 + lane < args.n) bias_hi = mx_detail::to_float(bias[c + 32 + lane]);
       }
+      // What the digits leave, while the tile's MMAs run.
+      [[maybe_unused]] float left[mx_detail::SliceDigits::kTokens];
+      [[maybe_unused]] bool any_left = false;
+      [[maybe_unused]] int token0 = 0;
+      if constexpr (STORE == kStoreDigits) {
+        place();
+        const int list = c / mx_detail::SliceDigits::kRows;
+        token0 = list * mx_detail::SliceDigits::kTokens;
+        if (token0 < args.x.m && row0 < args.m)
+          any_left = mx_detail::left_products<mx_detail::SliceDigits>(
+              args.lists + static_cast<long long>(list) * args.kblocks, args.x, token0,
+              mx_detail::MxRows{args.a, args.pitch, args.sa, args.kblocks, args.m}, row0 + lane, left);
+      }
       // Warp-uniform exits: tcgen05.ld and .st need the whole warp.
       if (!__all_sync(0xffffffffu, pair_wait(&acc_full, static_cast<uint32_t>(ti) & 1u,
                                               kPairIdleSleepNs)))
@@ -531,7 +548,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // A 16-bit slice is one 4 KB staging chunk (64 columns), an fp32 slice two.
       constexpr int kChunks = OUT == kPairFp32 ? 2 : 1;
       if constexpr (STORE == kStoreDigits) {
-        store_digits<Out>(args, r, row0 + lane, c);
+        store_digits<Out>(args, r, row0 + lane, token0, any_left ? left : nullptr);
         __syncwarp();
         continue;
       }
@@ -775,12 +792,10 @@ int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFac
   args.tiles_n = static_cast<int>(tiles_n);
   args.kblocks = static_cast<int>((kbytes + kBlockBytes - 1) / kBlockBytes);
   const bool digits = p.digits_of != nullptr;
-  args.x = static_cast<const uint16_t*>(p.digits_of);
+  args.x = digits ? *p.digits_of : mx_detail::ValueRows{};
+  args.lists = p.digits_left;
   args.a = static_cast<const uint8_t*>(p.a);
-  args.ldx = p.digits_ld;
   args.pitch = kbytes;
-  args.x_k = p.digits_k;
-  args.x_bf16 = p.digits_bf16;
   args.idesc = p.idesc;
   CUtensorMap map_a, map_b, map_a3, map_b3;
   int panels_a = static_cast<int>(kbytes / kBlockBytes), panels_b = panels_a;

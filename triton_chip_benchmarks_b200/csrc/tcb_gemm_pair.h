@@ -9,6 +9,11 @@
 
 namespace tcb {
 
+namespace mx_detail {
+struct ValueRows;
+struct LeftList;
+}  // namespace mx_detail
+
 enum PairOutType : int { kPairFp32 = 0, kPairBf16 = 1, kPairFp16 = 2 };
 
 struct PairProblem {
@@ -23,12 +28,10 @@ struct PairProblem {
   int out;           // PairOutType
   uint32_t idesc;
   bool overlap;      // may start while the kernels before it still run (launch_overlapping)
-  // Non-null: b's rows are the MX FP4 digits of these 16-bit rows of digits_k
-  // values, and c is their product with a's rows, transposed: [n / 8][m].
-  const void* digits_of;
-  long long digits_ld;
-  int digits_k;
-  int digits_bf16;
+  // Non-null: b's rows are the MX FP4 digits of these 16-bit rows (SliceDigits), which
+  // leave digits_left, and c is the product of the rows with a's, transposed.
+  const mx_detail::ValueRows* digits_of;
+  const mx_detail::LeftList* digits_left;
 };
 
 int gemm_pair_run(const PairProblem& p, int blocks, int* status, const DeviceFacts& facts,

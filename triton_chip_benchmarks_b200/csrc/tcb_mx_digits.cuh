@@ -1,19 +1,32 @@
 // 16-bit rows as MX FP4 digits: what the few-row kernel and the CTA-pair GEMM
 // share.
 //
-// A group of 32 values with the largest in [2^(e+1), 2^(e+2)) is split exactly
-// into E2M1 digits,
+// A group of 32 values with the largest in [2^(e+1), 2^(e+2)) is split into E2M1
+// digits,
 //   u_0 = x * 2^-e (|u_0| < 4),  d_i = RNE_E2M1(u_i),  u_{i+1} = 8 (u_i - d_i),
-//   x = sum_i d_i 2^(e - 3i):  |u_i| <= 4 keeps the rounding below 1/2, so each
-// digit gives three bits more.  Eight digits hold a value to 2^-23 of its
-// group's largest (half of 8^-7 in units of 2^e, the largest being at least two
-// of them): bf16 values down to 2^-15 of it (fp16: 2^-12) without any error,
-// smaller ones as a fixed-point number of about the precision that an fp32 sum
-// holding the largest has.  The digits are eight rows of an MX tensor
+//   x = sum_i d_i 2^(e - 3i) + u_8 2^(e - 24):  |u_i| <= 4 keeps the rounding below
+// 1/2, so each digit gives three bits more.  The digits are eight rows of an MX tensor
 // whose scales differ by 2^3: a block-scaled MMA multiplies them as it does any
 // rows, and the epilogue adds a token's eight results, smallest first.
-// Infinities and NaN have no digits: they count as zero there, and the NaN scale
-// on their group's last digit tells the epilogue (odd_products).
+//
+// What is left.  Eight digits hold a value to 2^-23 of its group's largest: bf16
+// values down to 2^-15 of it (fp16: 2^-12) without any error.  Smaller ones may leave
+// something, and the largest value's weight may be zero (E2M1 has that code), so it
+// counts.  All of the following take part as fp32 products beside the MMA, so that x is
+// not rounded at all:
+//   * u_8 2^(e - 24), exact in fp32 (a multiple of the value's last bit);
+//   * digits whose scale would be below 2^-127 (groups below about 2^-105): the digit is
+//     zero, and u goes on without it;
+//   * values from 2^126 on, infinities and NaN, which count as zero in the digits (the
+//     first digit may be a seventh larger than its value, which must not overflow).
+// Few values leave anything: of 8192 normal ones whose channels have log-normal sizes,
+// 0.8 in bf16 and 5.6 in fp16.  They are listed by token and place, a list for a few
+// tokens and 256 values of K; a list that is too short only counts, and its readers
+// split the rows again (right for any rows, fast for those that leave little).  The
+// few-row kernel takes its lists along with a stage and finds the weights in shared
+// memory.  The CTA-pair GEMM's spare warps gather them from L2, 32 bytes for half of
+// one (1024 x 8192 x 8192: 194 us became 258 in bf16, 755 in fp16), so rows for it have
+// nine digits, which leave a tenth: seven tokens to a slice of 64 columns.
 #pragma once
 
 #include "tcb_mx.cuh"
@@ -21,16 +34,32 @@
 namespace tcb {
 namespace mx_detail {
 
-constexpr int kDigits = 8;
 constexpr int kDigitBits = 3;
+
+// How tokens lie in an MX tensor of digits: digit d of token j of list i is row
+// i * kRows + j * kDigits + d.  A list covers kTokens tokens and 256 values of K;
+// kPerTile lists (of neighbouring tokens) lie side by side.
+template <int DIGITS, int TOKENS, int ROWS, int PER_TILE>
+struct DigitLayout {
+  static constexpr int kDigits = DIGITS, kTokens = TOKENS, kRows = ROWS, kPerTile = PER_TILE;
+  static_assert(DIGITS * TOKENS <= ROWS, "rows of a list");
+  static __host__ __device__ long long lists(long long m) { return (m + TOKENS - 1) / TOKENS; }
+  static __host__ __device__ long long rows(long long m) { return lists(m) * ROWS; }
+  static __host__ __device__ long long index(long long list, int kb, int kblocks) {
+    return (list / PER_TILE * kblocks + kb) * PER_TILE + list % PER_TILE;
+  }
+};
+using TileDigits = DigitLayout<8, 4, 32, 4>;    // few-row kernel: 16 tokens a tile of 128 columns
+using SliceDigits = DigitLayout<9, 7, 64, 1>;   // CTA-pair GEMM: 7 tokens a slice of 64 columns
 
 __device__ __forceinline__ float value16(uint16_t bits, bool bf16) {
   return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
               : __half2float(__ushort_as_half(bits));
 }
 
-__device__ __forceinline__ bool is_odd(float v) {
-  return (__float_as_uint(v) & 0x7FFFFFFFu) >= 0x7F800000u;
+// No digits: at least 2^126, infinite or not a number.
+__device__ __forceinline__ bool is_large(float v) {
+  return (__float_as_uint(v) & 0x7FFFFFFFu) >= 0x7E800000u;
 }
 
 // Packed E8M0 code of (row, group).
@@ -39,28 +68,252 @@ __device__ __forceinline__ uint32_t packed_scale(const uint8_t* scales, int kblo
                 ((row & 127) >> 5) * 4 + (group & 3)];
 }
 
-// The products of a row's infinities and NaN in [k0, k1) with weight row n: what
-// its result is when it has any, whatever the rest sums to.
-static __device__ __noinline__ float odd_products(const uint16_t* x, bool bf16, const uint8_t* w,
-                                                  long long pitch, const uint8_t* sw, int kblocks,
-                                                  long long n, int k0, int k1) {
+// 16-bit rows [m][k], pitch ld elements; vec: every row starts on a 16-byte boundary.
+struct ValueRows {
+  const uint16_t* x;
+  long long ld;
+  int m, k;
+  int bf16, vec;
+};
+
+// MX rows [n], of pitch code bytes, with packed scales.
+struct MxRows {
+  const uint8_t* codes;
+  long long pitch;
+  const uint8_t* scales;
+  int kblocks;
+  long long n;
+  __device__ __forceinline__ float scale(long long row, int group) const {
+    return scale_value(packed_scale(scales, kblocks, row, group));
+  }
+};
+
+// The lane's eight of 256 values from k on, zeros past the end.
+__device__ __forceinline__ uint4 load_values(const ValueRows& rows, long long token, int k) {
+  const uint16_t* row = rows.x + token * rows.ld;
+  if (rows.vec && k + 8 <= rows.k) return *reinterpret_cast<const uint4*>(row + k);
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < rows.k) w[i / 2] |= static_cast<uint32_t>(row[k + i]) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Value i of a lane's eight.
+__device__ __forceinline__ float lane_value(uint4 raw, bool bf16, int i) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  return value16(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))), bf16);
+}
+
+// A lane's eight values (four lanes a group) as digits: put(d, code, words) for digit
+// d, with the E8M0 code of its scale.  Returns whether the lane's values leave
+// anything; u[] (u_DIGITS) and e8 are for left_of.
+template <int DIGITS, typename Put>
+__device__ __forceinline__ bool split_digits(uint4 raw, bool bf16, float (&u)[8], int& e8, Put put) {
+  uint32_t top = 0, any = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    u[i] = lane_value(raw, bf16, i);
+    if (is_large(u[i])) {
+      u[i] = 0.0f;
+      any = 1;
+    }
+    top = max(top, __float_as_uint(u[i]) & 0x7FFFFFFFu);
+  }
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+  // The first digit's code; a group of zeros has one that makes all of them valid.
+  e8 = top == 0 ? 127 + (DIGITS - 1) * kDigitBits : max(static_cast<int>(top >> 23) - 1, 0);
+  const float inv = inverse_scale(static_cast<uint32_t>(e8));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] *= inv;
+#pragma unroll
+  for (int d = 0; d < DIGITS; ++d) {
+    const int code = e8 - kDigitBits * d;
+    const uint32_t codes = code >= 0 ? encode8(u) : 0u;
+    uint32_t h[4];
+    decode8(codes, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo, hi;
+      unpack2<__half>(h[i], lo, hi);
+      u[2 * i] = (u[2 * i] - lo) * static_cast<float>(1 << kDigitBits);
+      u[2 * i + 1] = (u[2 * i + 1] - hi) * static_cast<float>(1 << kDigitBits);
+    }
+    put(d, static_cast<uint8_t>(max(code, 0)), codes);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) any |= __float_as_uint(u[i]) << 1;  // but for signs of zeros
+  return any != 0;
+}
+
+// What split_digits leaves of the lane's values: u becomes that.
+template <int DIGITS>
+__device__ __forceinline__ void left_of(uint4 raw, bool bf16, float (&u)[8], int e8) {
+  // Two exact products: the last digit's scale over eight alone may be too small a number.
+  constexpr float kPast = 1.0f / (1 << DIGITS * kDigitBits);
+  const float unit = scale_value(static_cast<uint32_t>(e8));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = lane_value(raw, bf16, i);
+    u[i] = is_large(v) ? v : u[i] * kPast * unit;
+  }
+}
+
+// How many of the lane's values leave something.
+__device__ __forceinline__ int count_left(const float (&left)[8]) {
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) n += left[i] != 0.0f;  // NaN too
+  return n;
+}
+
+// The sum of left . weight row n over K block kb, `left` being spread over the
+// warp's `lanes`.
+__device__ __forceinline__ float left_block(const float (&left)[8], uint32_t lanes, int kb, const MxRows& w,
+                                            long long n) {
   float sum = 0.0f;
-  for (int k = k0; k < k1; ++k) {
-    const float v = value16(x[k], bf16);
-    if (!is_odd(v)) continue;
-    const uint32_t code = w[n * pitch + k / 2] >> (4 * (k & 1)) & 15u;
-    sum += v * (decode1(code) * scale_value(packed_scale(sw, kblocks, n, k / 32)));
+  while (lanes != 0) {
+    const int from = __ffs(lanes) - 1;
+    lanes &= lanes - 1;
+    const bool in = n < w.n;
+    const uint32_t codes = in ? *reinterpret_cast<const uint32_t*>(w.codes + n * w.pitch + kb * 128ll + from * 4) : 0u;
+    const float scale = in ? w.scale(n, kb * 8 + from / 4) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = __shfl_sync(0xFFFFFFFFu, left[i], from);
+      if (v != 0.0f) sum += v * (decode1(codes >> (4 * i) & 15u) * scale);
+    }
   }
   return sum;
 }
 
-// A token's result from its eight columns r[0..7]; `*odd` where odd_products has
-// to be added (the last digit is not a number).
-__device__ __forceinline__ float sum_digits(const float* r, bool* odd) {
-  *odd = isnan(r[kDigits - 1]);
-  float sum = *odd ? 0.0f : r[kDigits - 1];
+// What the digits of a list's tokens leave in 256 values of K, in order.  More than
+// kLeftEntries are counted, not listed.
+constexpr int kLeftEntries = 7;
+struct LeftList {
+  uint32_t count;
+  uint32_t unused;
+  uint2 entries[kLeftEntries];  // a LeftEntry; the fp32 value
+};
+// A place in a block of 256 values of K and a token, as its reader wants them: the byte
+// and nibble of the code, and where the scale lies in the row's 1 KB of packed scales.
+struct LeftEntry {
+  uint32_t bits;
+  static __device__ __forceinline__ uint32_t token(uint32_t t) { return t << 24; }
+  static __device__ __forceinline__ LeftEntry of(uint32_t t, uint32_t place) {
+    return {token(t) | ((place >> 7) * 512 + (place >> 5 & 3u)) << 11 | (place & 1u) << 10 | place >> 1};
+  }
+  __device__ __forceinline__ uint32_t byte() const { return bits & 127u; }
+  __device__ __forceinline__ uint32_t shift() const { return bits >> 8 & 4u; }
+  __device__ __forceinline__ uint32_t scale() const { return bits >> 11 & 1023u; }
+  __device__ __forceinline__ uint32_t token() const { return bits >> 24; }
+};
+static_assert(sizeof(LeftList) == 64, "a bulk copy of whole 16 bytes; eight lanes read one");
+
+// Appends a warp's values to a list whose first `at` entries are other tokens'; a lane
+// has `mine`.
+__device__ __forceinline__ void append_left(LeftList* list, uint32_t at, uint32_t mine, uint32_t token,
+                                            const float (&left)[8]) {
+  const int lane = threadIdx.x & 31;
+  uint32_t end = mine;
 #pragma unroll
-  for (int d = kDigits - 2; d >= 0; --d) sum += r[d];
+  for (int step = 1; step < 32; step *= 2) {
+    const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, end, step);
+    if (lane >= step) end += before;
+  }
+  at += end - mine;
+  if (mine == 0) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (left[i] != 0.0f && at < kLeftEntries)
+      list->entries[at++] = make_uint2(LeftEntry::of(token, lane * 8 + i).bits, __float_as_uint(left[i]));
+}
+
+// What the digits of a token leave in K block kb, split again, times weight row n (a
+// row a lane).
+template <int DIGITS>
+__device__ __forceinline__ float left_again(const ValueRows& rows, long long token, int kb, const MxRows& w,
+                                            long long n) {
+  const uint4 raw = load_values(rows, token, kb * 256 + (threadIdx.x & 31) * 8);
+  float left[8];
+  int e8;
+  const bool any = split_digits<DIGITS>(raw, rows.bf16, left, e8, [](int, uint8_t, uint32_t) {});
+  left_of<DIGITS>(raw, rows.bf16, left, e8);
+  return left_block(left, __ballot_sync(0xFFFFFFFFu, any), kb, w, n);
+}
+
+// acc[t] = the products of weight row n (a row a lane) with what the digits of token
+// first + t, t < Layout::kTokens, leave; `lists` are that list's, a K block each.
+// Returns whether there is anything (acc is not written otherwise).
+template <typename Layout>
+__device__ __noinline__ bool left_products(const LeftList* lists, const ValueRows& rows, long long first,
+                                           const MxRows& w, long long n, float* acc) {
+  constexpr int kBatch = 8;  // weights in flight
+  const int lane = threadIdx.x & 31;
+  const long long m = min(n, w.n - 1);  // rows past the end: any row
+  const uint8_t* row = w.codes + m * w.pitch;
+  const uint8_t* scales = w.scales + (m >> 7) * w.kblocks * 1024 + (m & 31) * 16 + ((m & 127) >> 5) * 4;
+  bool any = false;
+  for (int base = 0; base < w.kblocks; base += 32) {
+    const uint32_t count = base + lane < w.kblocks ? lists[base + lane].count : 0u;
+    if (!__any_sync(0xFFFFFFFFu, count != 0)) continue;
+    if (!any) {
+      for (int t = 0; t < Layout::kTokens; ++t) acc[t] = 0.0f;
+      any = true;
+    }
+    // The lists end to end, an entry a lane.
+    const uint32_t listed = count <= kLeftEntries ? count : 0u;
+    uint32_t end = listed;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) {
+      const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, end, step);
+      if (lane >= step) end += before;
+    }
+    const int total = static_cast<int>(__shfl_sync(0xFFFFFFFFu, end, 31));
+    for (int from = 0; from < total; from += 32) {
+      const uint32_t e = static_cast<uint32_t>(from + lane);
+      int at = 0;  // the list that entry e lies in: as many end at or before it
+#pragma unroll
+      for (int step = 16; step > 0; step /= 2)
+        if (__shfl_sync(0xFFFFFFFFu, end, at + step - 1) <= e) at += step;
+      const uint32_t start = __shfl_sync(0xFFFFFFFFu, end - listed, at);
+      const bool own = e < static_cast<uint32_t>(total);
+      const uint2 entry = own ? lists[base + at].entries[e - start] : make_uint2(0, 0);
+      const int kb = own ? base + at : 0;
+      const int here = min(32, total - from);
+      for (int j = 0; j < here; j += kBatch) {
+        // Straight-line loads, whether there is an entry or not.
+        uint32_t codes[kBatch], scale[kBatch];
+        LeftEntry place[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          place[u].bits = __shfl_sync(0xFFFFFFFFu, entry.x, j + u);
+          const long long block = __shfl_sync(0xFFFFFFFFu, kb, j + u);
+          codes[u] = row[block * 128 + place[u].byte()];
+          scale[u] = scales[block * 1024 + place[u].scale()];
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const float v = __uint_as_float(__shfl_sync(0xFFFFFFFFu, entry.y, j + u));
+          const float term = v * (decode1(codes[u] >> place[u].shift() & 15u) * scale_value(scale[u]));
+          if (j + u < here) acc[place[u].token()] += term;
+        }
+      }
+    }
+    for (uint32_t full = __ballot_sync(0xFFFFFFFFu, count > kLeftEntries); full != 0; full &= full - 1)
+      for (int t = 0; t < Layout::kTokens && first + t < rows.m; ++t)
+        acc[t] += left_again<Layout::kDigits>(rows, first + t, base + __ffs(full) - 1, w, n);
+  }
+  return any;
+}
+
+// A token's result from its columns r[0..DIGITS - 1], smallest first.
+template <int DIGITS>
+__device__ __forceinline__ float sum_digits(const float* r) {
+  float sum = r[DIGITS - 1];
+#pragma unroll
+  for (int d = DIGITS - 2; d >= 0; --d) sum += r[d];
   return sum;
 }
 

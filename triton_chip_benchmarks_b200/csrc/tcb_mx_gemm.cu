@@ -64,7 +64,7 @@ extern "C" int tcb_mx_gemm(const void* A, const void* SA, const void* B, const v
     return mx_rows_run(p, nullptr, status_dev, facts, s);
   }
   const PairProblem p{A, B, SA, SB, bias, C, ldc, M, N, static_cast<int>(mx_detail::mx_padded(K)),
-                      pair_type, gemm_pair_idesc(), true, nullptr, 0, 0, 0};
+                      pair_type, gemm_pair_idesc(), true, nullptr, nullptr};
   return gemm_pair_run(p, 0, status_dev, facts, s);
 }
 

@@ -7,15 +7,16 @@
 // tcgen05.mma kind::mxf4.block_scale: nothing is decoded by threads.
 //
 // 16-bit rows take part as eight MX FP4 digits each (tcb_mx_digits.cuh), columns that
-// the epilogue adds.  (Decoding W to fp16 for mma.sync instead was bound by issue
-// slots: 24 us at 1 x 16384 x 8192, 31 us for 16 MX rows at 8192 x 8192.)
+// the epilogue adds, and as products with what the digits leave.  (Decoding W to fp16 for
+// mma.sync instead was bound by issue slots: 24 us at 1 x 16384 x 8192, 31 us for 16 MX
+// rows at 8192 x 8192.)
 //
 // Where the digits come from.  Up to kInlineTokens rows, X warps of each CTA write
 // the digits of its K slice into shared memory on the way; for more rows a
 // kernel of their own writes them once (into the caller's workspace), and the
 // product starts beside it: its weight loads are under way before the digits
 // are there.  16 rows fill the 128 columns of a tile; column tiles share the weight
-// through L2 while there is an SM for each, and more digits than that become
+// through L2 while all of them run at once, and more digits than that become
 // columns of the CTA-pair GEMM.
 //
 // Split over K.  With fewer row tiles than CTAs fit, up to eight CTAs of a
@@ -29,13 +30,16 @@
 //   warp 0      producer: per 256 K values, TMA loads of W (128 rows x 128 B) and X
 //               (128-byte swizzle), bulk copies of their packed scales;
 //   warp 1      MMA issuer: four MMAs a stage into one accumulator;
-//   warps 2-5   scale writers (shared -> tensor memory), then the epilogue;
+//   warps 2-5   scale writers (shared -> tensor memory), which also multiply what a
+//               stage's digits leave, then the epilogue;
 //   warps 6-9   X warps (inline digits only).
 // What bounds it: HBM while the weights stream (25 B/clk per SM at two CTAs), and
 // about 5 us around that: start, first loads, the cluster's join, the end.
-// Captured and back to back: 1 x 16384 x 8192 15.7 us (71 MB, 4.5 TB/s), 1 x 4096 x
-// 4096 6.7, 1 x 128256 x 4096 61 (4.6 TB/s), 16 MX rows at 8192 x 8192 10.0, 16 x
-// 16384 x 8192 19.6 with the digits' kernel.
+// Captured and back to back, bf16 rows: 1 x 16384 x 8192 16.4 us (71 MB, 4.3 TB/s), 1 x
+// 4096 x 4096 7.1, 16 x 16384 x 8192 21.0 with the digits' kernel; 16 MX rows at 8192 x
+// 8192 9.7.  What the digits leave takes 0.1 to 0.7 us of that; fp16 rows leave seven
+// times as many values (16 x 4096 x 4096: bf16 9.3, fp16 10.4, integers, which leave
+// nothing, 8.6).
 // Every wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and MMAs in flight are waited for (bounded
 // too), the CTA sends and stores nothing, and the status reports it.
@@ -76,32 +80,37 @@ constexpr int kInlineTokens = 2;
 constexpr int kXWarps = 4;
 constexpr int kMaxSplit = 8;
 constexpr int kEarlyTokens = 16;
+constexpr int kSumBytes = kEarlyTokens * kRowTile * 4;
+constexpr int kTileLists = TileDigits::kPerTile, kTileTokens = kTileLists * TileDigits::kTokens;
+static_assert(kInlineTokens <= TileDigits::kTokens, "inline digits have one list a stage");
+static_assert(kTileTokens * TileDigits::kDigits == kRowTile, "a column tile");
 // Two CTAs share an SM: half of its shared memory and of its tensor memory each.
 // (One CTA with twice the stages has the same bytes in flight but one MMA thread
 // and no second tile to cover its start and end: 28.6 us instead of 17.0 at
 // 1 x 32768 x 4096.)
-constexpr int kSmemBudget = 112 * 1024;
+constexpr int kSmemBudget = 112 * 1024 + 512;  // 512 bytes below half of 228 KB less 1 KB a CTA
 constexpr int kCtaTmemCols = 256;
 
 enum XMode : int { kXRows = 0, kXDigits = 1, kXInline = 2 };
+constexpr int rows_threads(int mode) { return (6 + (mode == kXInline ? kXWarps : 0)) * 32; }
 
 struct RowsArgs {
   const uint8_t* sw;     // packed scales of W
   const uint8_t* sx;     // packed scales of X's rows or digits
-  const uint8_t* w;      // W's codes (products of infinities and NaN)
-  const void* x;         // 16-bit X
+  const uint8_t* w;      // W's codes (products with what the digits leave)
+  ValueRows x;           // 16-bit X
+  const LeftList* lists; // what its digits leave
   const void* bias;
   void* y;
   long long pitch;       // code bytes of a row of W
-  long long ldx, ldy;
+  long long ldy;
   int* status;
-  int m, n, k;
+  int m, n;
   int kblocks;
   int split;             // CTAs of a cluster
   int stages, stage_bytes;
   int cols;              // columns of the MMA (a multiple of 8, at most 128)
   int col_tiles;         // of 128 columns each, if there are more than one
-  int x_bf16;
   int y_type;            // RowsType of y and the bias
   uint32_t idesc;
 };
@@ -138,100 +147,103 @@ __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, flo
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 
-// The 16-bit values x[k..k+7] of a row, zeros past the end.
-__device__ __forceinline__ uint4 load_values(const uint16_t* row, int k, int end, bool vec) {
-  if (vec && k + 8 <= end) return *reinterpret_cast<const uint4*>(row + k);
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (k + i < end) w[i / 2] |= static_cast<uint32_t>(row[k + i]) << (16 * (i & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// A lane's eight values in fp32; infinities and NaN become zeros and set `*odd`,
-// for all four lanes of the group.
-__device__ __forceinline__ void to_values(uint4 raw, bool bf16, float (&v)[8], bool* odd) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  *odd = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = value16(static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1))), bf16);
-    if (is_odd(v[i])) {
-      v[i] = 0.0f;
-      *odd = true;
-    }
-  }
-  const uint32_t lanes = 0xFu << (threadIdx.x & 28u);
-  *odd = (__ballot_sync(0xFFFFFFFFu, *odd) & lanes) != 0;
-}
-
-// The scale code of digit d: a digit whose scale would be below 2^-127 has none.
-__device__ __forceinline__ uint8_t digit_code(int code, int d, bool odd) {
-  return d == kDigits - 1 && odd ? 255 : static_cast<uint8_t>(max(code, 0));
-}
-
-// E8M0 code of the first digit of a group (four lanes of eight values); digit i
-// has kDigitBits * i less.  127 + (kDigits - 1) * kDigitBits for a group of zeros,
-// so that its digits' codes are valid.
-__device__ __forceinline__ int digit_scale(const float (&v)[8]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-  top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-  if (top == 0) return 127 + (kDigits - 1) * kDigitBits;
-  return max(static_cast<int>(top >> 23) - 1, 0);
-}
-
-// The next digit of eight values u (times 2^e8 - 127 of the digit): its codes; u
-// becomes what is left, times 8.
-__device__ __forceinline__ uint32_t next_digit(float (&u)[8]) {
-  const uint32_t codes = encode8(u);
-  uint32_t h[4];
-  decode8(codes, h);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float lo, hi;
-    unpack2<__half>(h[i], lo, hi);
-    u[2 * i] = (u[2 * i] - lo) * static_cast<float>(1 << kDigitBits);
-    u[2 * i + 1] = (u[2 * i + 1] - hi) * static_cast<float>(1 << kDigitBits);
-  }
-  return codes;
-}
-
-// Digits of all tokens as rows of an MX tensor, one warp per token and K block:
-// digit i of token j is row 8 j + i.
-__global__ void __launch_bounds__(256)
-    mx_digits_kernel(const uint16_t* x, long long ldx, int m, int k, long long pitch, int kblocks, int vec,
-                     int bf16, uint8_t* codes, uint8_t* scales) {
+// Digits of a list's tokens in one K block, a warp a token, and the list of what they
+// leave.
+template <typename Layout>
+__global__ void __launch_bounds__(Layout::kTokens * 32)
+    mx_digits_kernel(const __grid_constant__ ValueRows rows, long long pitch, int kblocks, uint8_t* codes,
+                     uint8_t* scales, LeftList* lists) {
+  __shared__ uint32_t counts[Layout::kTokens];
   // The product may start once the kernels before this one are done: its weight
   // may be theirs.
   wait_for_previous_kernels();
   let_next_kernel_start();
-  const int lane = threadIdx.x & 31;
-  const long long task = static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + (threadIdx.x >> 5);
-  const long long token = task / kblocks;
-  const int kb = static_cast<int>(task % kblocks);
-  if (token >= m) return;
-  float u[8];
-  bool odd;
-  to_values(load_values(x + token * ldx, kb * kBlockK + lane * 8, k, vec), bf16, u, &odd);
-  const int e8 = digit_scale(u);
-  const float inv = inverse_scale(static_cast<uint32_t>(e8));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] *= inv;
-  const long long byte = static_cast<long long>(kb) * kBlockBytes + lane * 4;
-  const int group = lane >> 2;
-#pragma unroll
-  for (int d = 0; d < kDigits; ++d) {
-    const long long row = token * kDigits + d;
-    const int code = e8 - kDigitBits * d;
-    const uint32_t w = next_digit(u);
-    if (byte < pitch) *reinterpret_cast<uint32_t*>(codes + row * pitch + byte) = code >= 0 ? w : 0u;
-    if ((lane & 3) == 0)
-      scales[((row >> 7) * kblocks + kb) * kScaleBlock + (group >> 2) * 512 + (row & 31) * 16 +
-             ((row & 127) >> 5) * 4 + (group & 3)] = digit_code(code, d, odd);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int kb = static_cast<int>(blockIdx.x) % kblocks;
+  const long long at = static_cast<long long>(blockIdx.x) / kblocks;  // the list
+  const long long token = at * Layout::kTokens + warp;
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  float left[8];
+  int e8 = 0;
+  bool any = false;
+  if (token < rows.m) {
+    raw = load_values(rows, token, kb * kBlockK + lane * 8);
+    const long long byte = static_cast<long long>(kb) * kBlockBytes + lane * 4;
+    const int group = lane >> 2;
+    any = split_digits<Layout::kDigits>(raw, rows.bf16, left, e8, [&](int d, uint8_t code, uint32_t words) {
+      const long long row = at * Layout::kRows + warp * Layout::kDigits + d;
+      if (byte < pitch) *reinterpret_cast<uint32_t*>(codes + row * pitch + byte) = words;
+      if ((lane & 3) == 0)
+        scales[((row >> 7) * kblocks + kb) * kScaleBlock + (group >> 2) * 512 + (row & 31) * 16 +
+               ((row & 127) >> 5) * 4 + (group & 3)] = code;
+    });
   }
+  if (any) left_of<Layout::kDigits>(raw, rows.bf16, left, e8);
+  const uint32_t mine = any ? count_left(left) : 0u;
+  const uint32_t warp_total = __reduce_add_sync(0xFFFFFFFFu, mine);
+  if (lane == 0) counts[warp] = warp_total;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < Layout::kTokens; ++i) {
+    const uint32_t n = counts[i];
+    if (i < warp) before += n;
+    total += n;
+  }
+  LeftList* list = lists + Layout::index(at, kb, kblocks);
+  if (threadIdx.x == 0) list->count = total;
+  if (warp_total != 0) append_left(list, before, mine, static_cast<uint32_t>(warp), left);
+}
+
+// What a list that is too short counts, for one of its tokens: out of the way of the
+// stages' loop.
+__device__ __noinline__ float left_of_full_list(const RowsArgs& args, long long token, int kb, long long n) {
+  const MxRows w{args.w, args.pitch, args.sw, args.kblocks, args.n};
+  return token < args.x.m ? left_again<TileDigits::kDigits>(args.x, token, kb, w, n) : 0.0f;
+}
+
+// sums[t] += the weight row of this lane (row 0..127 of the tile) times what the lists of
+// a stage say of token t.  The warp has the lists in registers, eight lanes one: its
+// count, then the entries (zeros: no list).  codes, scales: the stage's weights in shared
+// memory.  A loop of few instructions: most of the time goes into fetching them, as the
+// code runs once in a while (two or four entries at once took longer, in registers too:
+// 33 x 5000 x 4136 fp16, three entries a stage, 16.0 us so, 16.5 and 17.9).
+__device__ __forceinline__ void add_listed(uint2 word, const uint8_t* codes, const uint8_t* scales, int row,
+                                           float* sums) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t count = __shfl_sync(0xFFFFFFFFu, word.x, lane & 24);
+  word.x += static_cast<uint32_t>(lane >> 3) * LeftEntry::token(TileDigits::kTokens);
+  const float value = decode1(lane & 15);                        // of code lane % 16
+  const uint32_t mine = smem_addr(codes) + row * kBlockBytes;    // 16-byte chunk c at c ^ (row % 8)
+  const uint32_t swizzle = (row & 7) << 4;
+  const uint32_t scale = smem_addr(scales) + (row & 31) * 16 + (row >> 5) * 4;
+  uint32_t left =
+      __ballot_sync(0xFFFFFFFFu, (lane & 7) != 0 && static_cast<uint32_t>(lane & 7) <= count && count <= kLeftEntries);
+#pragma unroll 1
+  for (; left != 0; left &= left - 1) {
+    const int from = __ffs(left) - 1;
+    const LeftEntry at{__shfl_sync(0xFFFFFFFFu, word.x, from)};
+    const float v = __uint_as_float(__shfl_sync(0xFFFFFFFFu, word.y, from));
+    uint32_t code, e8;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(mine + (at.byte() ^ swizzle)));
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e8) : "r"(scale + at.scale()));
+    // A NaN scale may pass as infinity: the row's product is not a number already.
+    sums[at.token()] += v * (__shfl_sync(0xFFFFFFFFu, value, code >> at.shift()) *
+                             __uint_as_float(max(e8 << 23, 0x00400000u)));
+  }
+}
+
+// Appends what the inline digits of a token leave to a stage's list of `listed`
+// entries; u, raw, e8 and any are split_digits' of the warp.  Returns how many there are
+// then.  Not inlined: what runs once in a while lies out of the way of what always runs
+// (which every launch fetches: 7.25 us instead of 6.7 at 1 x 4096 x 4096).
+__device__ __noinline__ uint32_t list_left(float4 u0, float4 u1, uint4 raw, bool bf16, int e8, bool any,
+                                           uint32_t token, LeftList* list, uint32_t listed) {
+  float left[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+  left_of<TileDigits::kDigits>(raw, bf16, left, e8);
+  const uint32_t mine = any ? count_left(left) : 0u;
+  append_left(list, listed, mine, token, left);
+  return listed + __reduce_add_sync(0xFFFFFFFFu, mine);
 }
 
 // The last step of a CTA: its rows' sums over the ranks in order, the bias, one
@@ -259,14 +271,14 @@ __device__ __forceinline__ void finish(const float* sums, int split, int tokens,
 }
 
 template <int XMODE>
-__global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
+__global__ void __launch_bounds__(rows_threads(XMODE), 2)
     mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ RowsArgs args) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t loaded[kMaxStages];  // operand and scale bytes landed
   __shared__ __align__(8) uint64_t digits[kMaxStages];  // X warps wrote the stage's digits
   __shared__ __align__(8) uint64_t full[kMaxStages];    // scales are in tensor memory
-  __shared__ __align__(8) uint64_t empty[kMaxStages];   // the stage's MMAs have finished
+  __shared__ __align__(8) uint64_t empty[kMaxStages];   // the stage's MMAs, and what digits leave, are done
   __shared__ __align__(8) uint64_t acc_full;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
@@ -280,16 +292,19 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   const int kb0 = static_cast<int>(static_cast<long long>(args.kblocks) * rank / args.split);
   const int kb1 = static_cast<int>(static_cast<long long>(args.kblocks) * (rank + 1) / args.split);
   const int nkb = kb1 - kb0;
-  constexpr int kPerToken = XMODE == kXRows ? 1 : kDigits;  // columns of a token
+  constexpr int kPerToken = XMODE == kXRows ? 1 : TileDigits::kDigits;  // columns of a token
   const int token0 = col_tile * (kRowTile / kPerToken);
   const int tokens = min(args.m - token0, kRowTile / kPerToken);
   const int x_bytes = args.cols * kBlockBytes;
+  const int list_count = (tokens + TileDigits::kTokens - 1) / TileDigits::kTokens;  // of a stage
+  LeftList* stage_lists = reinterpret_cast<LeftList*>(smem + args.stages * args.stage_bytes + kSumBytes);
 
   auto load_w = [&](int it, int s) {
     const int kb = kb0 + it;
     uint8_t* stage = smem + s * args.stage_bytes;
     mbar_arrive_expect_tx(&loaded[s], kWBytes + kScaleBlock +
-                                          (XMODE == kXInline ? 0 : x_bytes + kScaleBlock));
+                                          (XMODE == kXInline ? 0 : x_bytes + kScaleBlock) +
+                                          (XMODE == kXDigits ? list_count * static_cast<int>(sizeof(LeftList)) : 0));
     tma_load_2d(stage, &map_w, kb * kBlockBytes, tile * kRowTile, &loaded[s]);
     bulk_load_1d(stage + kWBytes + x_bytes,
                  args.sw + (static_cast<long long>(tile) * args.kblocks + kb) * kScaleBlock,
@@ -303,17 +318,18 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     bulk_load_1d(stage + kWBytes + x_bytes + kScaleBlock,
                  args.sx + (static_cast<long long>(col_tile) * args.kblocks + kb) * kScaleBlock, kScaleBlock,
                  bar);
+    if constexpr (XMODE == kXDigits)
+      bulk_load_1d(stage_lists + s * kTileLists,
+                   args.lists + TileDigits::index(static_cast<long long>(col_tile) * kTileLists, kb, args.kblocks),
+                   list_count * static_cast<int>(sizeof(LeftList)), bar);
   };
   // An X warp's next values (inline digits): asked for one round ahead, the first
   // ones before the weights, behind whose bytes they would otherwise queue.
   [[maybe_unused]] uint4 x_next[kInlineTokens];
   auto ask_x = [&](int it) {
-    const bool vec = (reinterpret_cast<uintptr_t>(args.x) & 15) == 0 && (args.ldx % 8 == 0 || args.m == 1);
 #pragma unroll
     for (int i = 0; i < kInlineTokens; ++i)
-      if (i < tokens && it < nkb)
-        x_next[i] = load_values(static_cast<const uint16_t*>(args.x) + i * args.ldx,
-                                (kb0 + it) * kBlockK + lane * 8, args.k, vec);
+      if (i < tokens && it < nkb) x_next[i] = load_values(args.x, i, (kb0 + it) * kBlockK + lane * 8);
   };
   if constexpr (XMODE == kXInline) {
     if (warp >= 6) {
@@ -328,7 +344,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
       mbar_init(&loaded[s], 1);
       mbar_init(&digits[s], 1);
       mbar_init(&full[s], 4);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], XMODE == kXRows ? 1 : 5);
     }
     mbar_init(&acc_full, 1);
     abort_flag = 0;
@@ -353,6 +369,11 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   wait_for_previous_kernels();
   const uint32_t tbase = tmem_slot;
   const uint32_t tsf = tbase + static_cast<uint32_t>((args.cols + 31) & ~31);
+  const int row_of_lane = 32 * (warp & 3) + lane;
+  // A scale writer's sums of what the digits leave: its lane's row, a token each.
+  constexpr int kStageLists = XMODE == kXInline ? 1 : kTileLists, kStageTokens = kStageLists * TileDigits::kTokens;
+  [[maybe_unused]] float left_sums[kStageTokens] = {};
+  [[maybe_unused]] bool any_left = false;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -425,6 +446,23 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
+      if constexpr (XMODE != kXRows) {
+        uint2 word = make_uint2(0, 0);
+        if (lane < 8 * list_count) word = reinterpret_cast<const uint2*>(stage_lists + s * kStageLists)[lane];
+        if (__any_sync(0xFFFFFFFFu, (lane & 7) == 0 && word.x != 0)) {
+          any_left = true;
+          add_listed(word, smem + s * args.stage_bytes, sw - lane * 16, row_of_lane, left_sums);
+          uint32_t full = __ballot_sync(0xFFFFFFFFu, (lane & 7) == 0 && word.x > kLeftEntries);
+          for (; full != 0; full &= full - 1) {
+            const int first = (__ffs(full) - 1) / 8 * TileDigits::kTokens;
+            for (int t = first; t < first + TileDigits::kTokens; ++t)
+              left_sums[t] += left_of_full_list(args, token0 + t, kb0 + it,
+                                                static_cast<long long>(tile) * kRowTile + row_of_lane);
+          }
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
     }
   } else if (XMODE == kXInline) {
     // -------------------------------------------------------------- X warps
@@ -438,32 +476,25 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
       if (!__all_sync(0xFFFFFFFFu, ok)) break;
       uint8_t* xt = smem + s * args.stage_bytes + kWBytes;
       uint8_t* sx = xt + x_bytes + kScaleBlock;
-      uint4 x_now[kInlineTokens];
-#pragma unroll
-      for (int i = 0; i < kInlineTokens; ++i) x_now[i] = x_next[i];
+      uint32_t listed = 0;
 #pragma unroll
       for (int token = 0; token < kInlineTokens; ++token) {
         if (token >= tokens) break;
-        float u[8];
-        bool odd;
-        to_values(x_now[token], args.x_bf16, u, &odd);
-        const int e8 = digit_scale(u);
-        const float inv = inverse_scale(static_cast<uint32_t>(e8));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] *= inv;
         const int group = lane >> 2;
-#pragma unroll
-        for (int d = 0; d < kDigits; ++d) {
-          const int row = token * kDigits + d;
-          const int code = e8 - kDigitBits * d;
-          const uint32_t w = next_digit(u);
-          *reinterpret_cast<uint32_t*>(xt + row * kBlockBytes + ((group ^ d) << 4) + (lane & 3) * 4) =
-              code >= 0 ? w : 0u;
-          if ((lane & 3) == 0)
-            sx[(group >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (group & 3)] =
-                digit_code(code, d, odd);
-        }
+        float u[8];
+        int e8;
+        const bool any = split_digits<TileDigits::kDigits>(
+            x_next[token], args.x.bf16, u, e8, [&](int d, uint8_t code, uint32_t words) {
+              const int row = token * TileDigits::kDigits + d;
+              *reinterpret_cast<uint32_t*>(xt + row * kBlockBytes + ((group ^ d) << 4) + (lane & 3) * 4) = words;
+              if ((lane & 3) == 0)
+                sx[(group >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (group & 3)] = code;
+            });
+        if (__any_sync(0xFFFFFFFFu, any))
+          listed = list_left(make_float4(u[0], u[1], u[2], u[3]), make_float4(u[4], u[5], u[6], u[7]), x_next[token],
+                             args.x.bf16, e8, any, token, stage_lists + s, listed);
       }
+      if (lane == 0) stage_lists[s].count = listed;
       fence_proxy_async_smem();  // the MMA reads the tile through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(&digits[s]);
@@ -483,7 +514,16 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
   if (!early) cluster_sync_all();
   if (!aborted && warp >= 2 && warp < 6) {
     tc_fence_after();
-    const int row = 32 * (warp & 3) + lane;
+    const int row = row_of_lane;
+    float* left_in_ring = reinterpret_cast<float*>(smem);  // [token][row]
+    if constexpr (XMODE != kXRows) {
+      // Sixteen local loads side by side instead of one a token, each of them slow (9.3
+      // instead of 10.7 us at 16 x 4096 x 4096).
+      if (any_left) {
+#pragma unroll
+        for (int t = 0; t < kStageTokens; ++t) left_in_ring[t * kRowTile + row] = left_sums[t];
+      }
+    }
     const uint32_t taddr = tbase + ((32u * (warp & 3)) << 16);
     const int owner = row >> share_log2;
     const uint32_t to =
@@ -500,15 +540,9 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
         for (int i = 0; i < 8; ++i)
           if (c + i < tokens) send(c + i, r[i]);
       } else {
-        const int token = c / kDigits;
-        bool odd;
-        float sum = sum_digits(r, &odd);
-        const long long n = static_cast<long long>(tile) * kRowTile + row;
-        if (odd && n < args.n)
-          sum += odd_products(static_cast<const uint16_t*>(args.x) + (token0 + token) * args.ldx, args.x_bf16, args.w,
-                              args.pitch, args.sw, args.kblocks, n, kb0 * kBlockK,
-                              static_cast<int>(min(static_cast<long long>(kb1) * kBlockK,
-                                                   static_cast<long long>(args.k))));
+        const int token = c / TileDigits::kDigits;
+        float sum = sum_digits<TileDigits::kDigits>(r);
+        if (any_left) sum += left_in_ring[token * kRowTile + row];
         send(token, sum);
       }
     }
@@ -520,7 +554,7 @@ __global__ void __launch_bounds__((6 + (XMODE == kXInline ? kXWarps : 0)) * 32)
     const long long n0 = static_cast<long long>(tile) * kRowTile + rank * share;
     const int rows = static_cast<int>(min(static_cast<long long>(min(share, kRowTile - rank * share)),
                                           args.n - n0));
-    constexpr int kThreads = (6 + (XMODE == kXInline ? kXWarps : 0)) * 32;
+    constexpr int kThreads = rows_threads(XMODE);
     auto run = [&](auto* y) {
       using T = std::remove_pointer_t<decltype(y)>;
       const T* bias = static_cast<const T*>(args.bias);
@@ -555,18 +589,33 @@ int rows_map(CUtensorMap* map, const void* base, long long rows, long long pitch
              : TCB_ERR_INVALID_ARGUMENT;
 }
 
-// The digits of m rows of k values as an MX tensor: [scales][codes].
+// The digits of m rows of k values as an MX tensor, and what they leave:
+// [scales][lists][codes].
 struct DigitSpace {
-  long long codes_at, bytes;
-  DigitSpace(long long m, long long k) {
+  long long rows, lists, lists_at, codes_at, bytes;
+  template <typename Layout>
+  DigitSpace(Layout, long long m, long long k) : rows(Layout::rows(m)), lists(Layout::lists(m)) {
     const long long kblocks = (mx_padded(k) + kBlockK - 1) / kBlockK;
-    codes_at = (m * kDigits + 255) / 256 * 2 * kScaleBlock * kblocks;
-    bytes = codes_at + m * kDigits * (mx_padded(k) / 2);
+    const long long tiles = (lists + Layout::kPerTile - 1) / Layout::kPerTile;
+    lists_at = (rows + 255) / 256 * 2 * kScaleBlock * kblocks;
+    const long long list_bytes = tiles * Layout::kPerTile * kblocks * static_cast<long long>(sizeof(LeftList));
+    codes_at = lists_at + (list_bytes + 255) / 256 * 256;
+    bytes = codes_at + rows * (mx_padded(k) / 2);
   }
 };
 
+template <typename Layout>
+int launch_digits(const RowsArgs& args, const DigitSpace& space, uint8_t* base, cudaStream_t stream) {
+  const long long blocks = space.lists * args.kblocks;
+  if (blocks > INT_MAX || space.rows > INT_MAX / 2) return TCB_ERR_RESOURCE;
+  return launch_overlapping(mx_digits_kernel<Layout>, dim3(static_cast<unsigned>(blocks)), 32 * Layout::kTokens, 0, 1,
+                            stream, args.x, args.pitch, args.kblocks, base + space.codes_at, base,
+                            reinterpret_cast<LeftList*>(base + space.lists_at));
+}
+
 template <int XMODE>
-int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, const DeviceFacts& facts, cudaStream_t stream) {
+int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, const DeviceFacts& facts,
+                cudaStream_t stream) {
   args.col_tiles = (args.cols + kRowTile - 1) / kRowTile;
   if (args.cols > kRowTile) args.cols = kRowTile;
   const long long tiles = (static_cast<long long>(args.n) + kRowTile - 1) / kRowTile * args.col_tiles;
@@ -587,14 +636,15 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   if (args.kblocks >= 4 && tiles * 4 <= places - 16) args.split = 4;
   if (args.kblocks >= kMaxSplit && tiles * kMaxSplit <= most_in_eights) args.split = kMaxSplit;
   if (tiles * args.split > INT_MAX) return TCB_ERR_RESOURCE;
-  constexpr int kSumBytes = kEarlyTokens * kRowTile * 4;
-  args.stages = (kSmemBudget - 1024 - kSumBytes) / args.stage_bytes;
+  constexpr int kLists = XMODE == kXRows ? 0 : XMODE == kXInline ? 1 : kTileLists;
+  constexpr int list_bytes = kLists * static_cast<int>(sizeof(LeftList));
+  args.stages = (kSmemBudget - 1024 - kSumBytes) / (args.stage_bytes + list_bytes);
   if (args.stages > kMaxStages) args.stages = kMaxStages;
   const int acc_cols = (args.cols + 31) / 32 * 32;
   while (acc_cols + args.stages * kSfStageCols > kCtaTmemCols) --args.stages;
   // The ring's places: X warps step kXWarps of them at a time.
   if (args.stages < (XMODE == kXInline ? kXWarps : 2)) return TCB_ERR_RESOURCE;
-  const int smem = args.stages * args.stage_bytes + kSumBytes + 1024;
+  const int smem = args.stages * (args.stage_bytes + list_bytes) + kSumBytes + 1024;
   // N of the instruction; M = 128, E2M1 x E2M1, E8M0 scales as the pair MMA.
   args.idesc = (gemm_pair_idesc() & ~(0x3Fu << 17 | 0x1Fu << 24)) |
                static_cast<uint32_t>(args.cols >> 3) << 17 | static_cast<uint32_t>(kRowTile >> 4) << 24;
@@ -605,14 +655,19 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   });
   if (cap < smem) return TCB_ERR_RESOURCE;
   return launch_overlapping(fn, dim3(static_cast<unsigned>(tiles * args.split)),
-                            (6 + (XMODE == kXInline ? kXWarps : 0)) * 32, static_cast<size_t>(smem),
-                            args.split, stream, map_w, map_x, args);
+                            rows_threads(XMODE), static_cast<size_t>(smem), args.split, stream, map_w, map_x,
+                            args);
 }
 
 }  // namespace
 
+// Column tiles of the few-row kernel or columns of the CTA-pair GEMM, which N decides.
 long long mx_rows_workspace(long long m, long long k) {
-  return m <= kInlineTokens ? 0 : DigitSpace(m, k).bytes;
+  if (m <= kInlineTokens) return 0;
+  const long long tile = DigitSpace(TileDigits{}, m, k).bytes;
+  if (m <= kTileTokens) return tile;
+  const long long slice = DigitSpace(SliceDigits{}, m, k).bytes;
+  return tile > slice ? tile : slice;
 }
 
 int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const DeviceFacts& facts,
@@ -621,18 +676,16 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
   args.sw = static_cast<const uint8_t*>(p.sw);
   args.sx = static_cast<const uint8_t*>(p.sx);
   args.w = static_cast<const uint8_t*>(p.w);
-  args.x = p.x;
+  args.x = {static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, p.x_type == kRowsBf16,
+            aligned(p.x, 16) && (p.ldx % 8 == 0 || p.m == 1)};
   args.bias = p.bias;
   args.y = p.y;
   args.pitch = mx_padded(p.k) / 2;
-  args.ldx = p.ldx;
   args.ldy = p.ldy;
   args.status = status;
   args.m = p.m;
   args.n = p.n;
-  args.k = p.k;
   args.kblocks = static_cast<int>((args.pitch + kBlockBytes - 1) / kBlockBytes);
-  args.x_bf16 = p.x_type == kRowsBf16;
   args.y_type = p.y_type;
   CUtensorMap map_w, map_x{};
   int rc = rows_map(&map_w, p.w, p.n, args.pitch, kRowTile);
@@ -643,26 +696,20 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
     return launch_rows<kXRows>(map_w, map_x, args, facts, stream);
   }
   if (p.m <= kInlineTokens) {
-    args.cols = p.m * kDigits;
+    args.cols = p.m * TileDigits::kDigits;
     return launch_rows<kXInline>(map_w, map_x, args, facts, stream);
   }
-  const DigitSpace space(p.m, p.k);
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  const long long warps = static_cast<long long>(p.m) * args.kblocks;
-  if ((warps + 7) / 8 > INT_MAX || p.m > INT_MAX / (2 * kDigits)) return TCB_ERR_RESOURCE;
-  rc = launch_overlapping(mx_digits_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, 1, stream,
-                          static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, args.pitch, args.kblocks,
-                          static_cast<int>(aligned(p.x, 16) && p.ldx % 8 == 0), args.x_bf16,
-                          base + space.codes_at, base);
-  if (rc != TCB_OK) return rc;
-  args.cols = p.m * kDigits;
-  // Measured (us, here / pairs, 24, 33, 48 and 64 rows): N x K = 4096 x 4096 10.8/11.6
-  // 11.6/12.0 12.3/12.6 12.8/12.9; 1024 x 4096 7.7/11.5 9.2/11.6 9.3/11.8 9.9/11.8; 5000 x
-  // 4136 11.8/12.3 12.8/13.1 13.0/13.4, 160 tiles 16.6/14.2; 16384 x 4096, 384 tiles
-  // 26.8/24.5; 256 x 8192, 256 rows 16.6/22.3.
+  // Column tiles while two of them fit an SM and all run at once.  Measured (us, column
+  // tiles / pairs, bf16 activations): 128 x 4096 x 4096 (256 tiles) 22.3/24.1, 48 x 12288 x
+  // 4096 (288) 20.9/25.1; 64 x 12288 x 4096 (384) 29.3/26.4, 33 x 16384 x 8192 (384)
+  // 45.0/36.7, 20 x 32768 x 4096 (512) 31.8/26.9.
   const long long row_tiles = (static_cast<long long>(p.n) + kRowTile - 1) / kRowTile;
-  if (args.cols > kRowTile && (args.cols + kRowTile - 1) / kRowTile * row_tiles > facts.sm_count) {
+  const long long col_tiles = (static_cast<long long>(p.m) + kTileTokens - 1) / kTileTokens;
+  if (col_tiles > 1 && col_tiles * row_tiles > 2ll * facts.sm_count) {
     // Columns of the CTA-pair GEMM, whose M side is the weight.
+    const DigitSpace space(SliceDigits{}, p.m, p.k);
+    if ((rc = launch_digits<SliceDigits>(args, space, base, stream)) != TCB_OK) return rc;
     PairProblem q = {};
     q.a = p.w;
     q.b = base + space.codes_at;
@@ -672,19 +719,22 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
     q.c = p.y;
     q.ldc = p.ldy;
     q.m = p.n;
-    q.n = p.m * kDigits;
+    q.n = static_cast<int>(space.rows);
     q.k = static_cast<int>(mx_padded(p.k));
     q.out = p.y_type == kRowsFp32 ? kPairFp32 : p.y_type == kRowsBf16 ? kPairBf16 : kPairFp16;
     q.idesc = gemm_pair_idesc();
     q.overlap = true;
-    q.digits_of = p.x;
-    q.digits_ld = p.ldx;
-    q.digits_k = p.k;
-    q.digits_bf16 = args.x_bf16;
+    q.digits_of = &args.x;
+    q.digits_left = reinterpret_cast<const LeftList*>(base + space.lists_at);
     return gemm_pair_run(q, 0, status, facts, stream);
   }
+  const DigitSpace space(TileDigits{}, p.m, p.k);
+  if ((rc = launch_digits<TileDigits>(args, space, base, stream)) != TCB_OK) return rc;
+  args.cols = p.m * TileDigits::kDigits;
   args.sx = base;
-  if ((rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols < kRowTile ? args.cols : kRowTile)) != TCB_OK) return rc;
+  args.lists = reinterpret_cast<const LeftList*>(base + space.lists_at);
+  rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols < kRowTile ? args.cols : kRowTile);
+  if (rc != TCB_OK) return rc;
   return launch_rows<kXDigits>(map_w, map_x, args, facts, stream);
 }
 

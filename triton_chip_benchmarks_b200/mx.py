@@ -335,11 +335,13 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
            status: torch.Tensor | None = None) -> torch.Tensor:
     """x [..., K] . w [N][K]^T (+ bias [N]) with bf16 or fp16 x, in `dtype` (default x's).
 
-    Only the weight is rounded to MX FP4: x takes part as eight MX digits, so up to
-    16 rows cost what reading w costs, and many rows eight times as many of
-    :func:`matmul` (quantise x too where that matters).  The first digit may be a
-    seventh larger than its value, so sums that come within that of fp32's largest
-    number may be infinite.  ``out`` is a matrix [rows][N].
+    Only the weight is rounded to MX FP4: x takes part as MX digits of three bits and
+    fp32 products with what these leave, so small values count in full beside large
+    ones.  Rows that leave much (a value 2^14 times the others, 2^11 in fp16, in every
+    group of 32) take longer.  The first digit may be a seventh larger than its value, so
+    sums that come within that of fp32's largest number may be infinite.  A few rows
+    cost little more than reading w once, a prompt's several products of MX rows
+    (quantise x too where that matters).  ``out`` is a matrix [rows][N].
     """
     x_dtype = x.dtype
     if x_dtype != torch.bfloat16 and x_dtype != torch.float16:
