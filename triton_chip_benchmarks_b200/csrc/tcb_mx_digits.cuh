@@ -4,29 +4,32 @@
 // A group of 32 values with the largest in [2^(e+1), 2^(e+2)) is split into E2M1
 // digits,
 //   u_0 = x * 2^-e (|u_0| < 4),  d_i = RNE_E2M1(u_i),  u_{i+1} = 8 (u_i - d_i),
-//   x = sum_i d_i 2^(e - 3i) + u_8 2^(e - 24):  |u_i| <= 4 keeps the rounding below
-// 1/2, so each digit gives three bits more.  The digits are eight rows of an MX tensor
+//   x = sum_{i<D} d_i 2^(e - 3i) + u_D 2^(e - 3D):  |u_i| <= 4 keeps the rounding below
+// 1/2, so each digit gives three bits more.  The digits are D rows of an MX tensor
 // whose scales differ by 2^3: a block-scaled MMA multiplies them as it does any
-// rows, and the epilogue adds a token's eight results, smallest first.
+// rows, and the epilogue adds a token's D results, smallest first.
 //
 // What is left.  Eight digits hold a value to 2^-23 of its group's largest: bf16
 // values down to 2^-15 of it (fp16: 2^-12) without any error.  Smaller ones may leave
 // something, and the largest value's weight may be zero (E2M1 has that code), so it
 // counts.  All of the following take part as fp32 products beside the MMA, so that x is
 // not rounded at all:
-//   * u_8 2^(e - 24), exact in fp32 (a multiple of the value's last bit);
+//   * u_D 2^(e - 3D), exact in fp32 (a multiple of the value's last bit);
 //   * digits whose scale would be below 2^-127 (groups below about 2^-105): the digit is
 //     zero, and u goes on without it;
 //   * values from 2^126 on, infinities and NaN, which count as zero in the digits (the
 //     first digit may be a seventh larger than its value, which must not overflow).
 // Few values leave anything: of 8192 normal ones whose channels have log-normal sizes,
-// 0.8 in bf16 and 5.6 in fp16.  They are listed by token and place, a list for a few
-// tokens and 256 values of K; a list that is too short only counts, and its readers
-// split the rows again (right for any rows, fast for those that leave little).  The
-// few-row kernel takes its lists along with a stage and finds the weights in shared
+// with eight digits 0.8 in bf16 and 5.6 in fp16, with nine a thirteenth of that.  They are
+// listed by token and place, a list for a few tokens and 256 values of K; a list that is
+// too short only counts, and its readers split the rows again (right for any rows, fast
+// for those that leave little: 16 x 4096 x 4096 bf16 takes 9.0 us for normal rows, 10.8 with
+// six channels and 12.3 with 24 a thousand times larger; 16 x 8192 x 8192 with a value
+// 2^20 times larger in every group 2.6 ms).
+// The few-row kernel takes its lists along with a stage and finds the weights in shared
 // memory.  The CTA-pair GEMM's spare warps gather them from L2, 32 bytes for half of
-// one (1024 x 8192 x 8192: 194 us became 258 in bf16, 755 in fp16), so rows for it have
-// nine digits, which leave a tenth: seven tokens to a slice of 64 columns.
+// one (1024 x 8192 x 8192 with eight digits: 194 us became 258 in bf16, 755 in fp16), so
+// rows for it have nine digits (230, 250).
 #pragma once
 
 #include "tcb_mx.cuh"
@@ -48,9 +51,18 @@ struct DigitLayout {
   static __host__ __device__ long long index(long long list, int kb, int kblocks) {
     return (list / PER_TILE * kblocks + kb) * PER_TILE + list % PER_TILE;
   }
+  static constexpr int kTileTokens = PER_TILE * TOKENS;
+  // First column of token t of a tile; columns of m tokens, in eights.
+  static __host__ __device__ int column(int t) { return t / TOKENS * ROWS + t % TOKENS * DIGITS; }
+  static __host__ __device__ int columns(int m) { return (column(m - 1) + DIGITS + 7) / 8 * 8; }
 };
-using TileDigits = DigitLayout<8, 4, 32, 4>;    // few-row kernel: 16 tokens a tile of 128 columns
-using SliceDigits = DigitLayout<9, 7, 64, 1>;   // CTA-pair GEMM: 7 tokens a slice of 64 columns
+// Few-row kernel, a tile of 128 columns: 16 bf16 or 14 fp16 tokens.  fp16 values have three
+// bits more, and with a ninth digit leave as little as bf16 values do with eight (33 x 5000
+// x 4136: 16.0 us with eight, 13.9 with nine; 16 x 16384 x 8192, two tiles, 24.5 and 26.4).
+using Bf16Tile = DigitLayout<8, 4, 32, 4>;
+using Fp16Tile = DigitLayout<9, 7, 64, 2>;
+// CTA-pair GEMM: seven tokens a slice of 64 columns.
+using SliceDigits = DigitLayout<9, 7, 64, 1>;
 
 __device__ __forceinline__ float value16(uint16_t bits, bool bf16) {
   return bf16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16)
@@ -190,8 +202,8 @@ __device__ __forceinline__ float left_block(const float (&left)[8], uint32_t lan
 
 // What the digits of a list's tokens leave in 256 values of K, in order.  More than
 // kLeftEntries are counted, not listed.
-constexpr int kLeftEntries = 7;
-struct LeftList {
+constexpr int kLeftEntries = 15;
+struct __align__(16) LeftList {
   uint32_t count;
   uint32_t unused;
   uint2 entries[kLeftEntries];  // a LeftEntry; the fp32 value
@@ -209,7 +221,7 @@ struct LeftEntry {
   __device__ __forceinline__ uint32_t scale() const { return bits >> 11 & 1023u; }
   __device__ __forceinline__ uint32_t token() const { return bits >> 24; }
 };
-static_assert(sizeof(LeftList) == 64, "a bulk copy of whole 16 bytes; eight lanes read one");
+static_assert(sizeof(LeftList) == 128, "eight lanes read 16 bytes each");
 
 // Appends a warp's values to a list whose first `at` entries are other tokens'; a lane
 // has `mine`.

@@ -6,7 +6,7 @@
 // SMs busy -- and X the N side, 8 to 128 columns of
 // tcgen05.mma kind::mxf4.block_scale: nothing is decoded by threads.
 //
-// 16-bit rows take part as eight MX FP4 digits each (tcb_mx_digits.cuh), columns that
+// 16-bit rows take part as eight or nine MX FP4 digits each (tcb_mx_digits.cuh), columns that
 // the epilogue adds, and as products with what the digits leave.  (Decoding W to fp16 for
 // mma.sync instead was bound by issue slots: 24 us at 1 x 16384 x 8192, 31 us for 16 MX
 // rows at 8192 x 8192.)
@@ -15,8 +15,8 @@
 // the digits of its K slice into shared memory on the way; for more rows a
 // kernel of their own writes them once (into the caller's workspace), and the
 // product starts beside it: its weight loads are under way before the digits
-// are there.  16 rows fill the 128 columns of a tile; column tiles share the weight
-// through L2 while all of them run at once, and more digits than that become
+// are there.  16 bf16 or 14 fp16 rows fill the 128 columns of a tile; column tiles share
+// the weight through L2 while all of them run at once, and more digits than that become
 // columns of the CTA-pair GEMM.
 //
 // Split over K.  With fewer row tiles than CTAs fit, up to eight CTAs of a
@@ -35,11 +35,9 @@
 //   warps 6-9   X warps (inline digits only).
 // What bounds it: HBM while the weights stream (25 B/clk per SM at two CTAs), and
 // about 5 us around that: start, first loads, the cluster's join, the end.
-// Captured and back to back, bf16 rows: 1 x 16384 x 8192 16.4 us (71 MB, 4.3 TB/s), 1 x
-// 4096 x 4096 7.1, 16 x 16384 x 8192 21.0 with the digits' kernel; 16 MX rows at 8192 x
-// 8192 9.7.  What the digits leave takes 0.1 to 0.7 us of that; fp16 rows leave seven
-// times as many values (16 x 4096 x 4096: bf16 9.3, fp16 10.4, integers, which leave
-// nothing, 8.6).
+// Captured and back to back, bf16 rows: 1 x 16384 x 8192 16.5 us (71 MB, 4.3 TB/s), 1 x
+// 4096 x 4096 6.8, 16 x 16384 x 8192 21.2 with the digits' kernel (19.9 where they leave
+// nothing); 16 MX rows at 8192 x 8192 9.7.
 // Every wait is bounded; a wait that runs out raises the CTA's abort flag, all
 // roles leave their loops, copies and MMAs in flight are waited for (bounded
 // too), the CTA sends and stores nothing, and the status reports it.
@@ -81,9 +79,10 @@ constexpr int kXWarps = 4;
 constexpr int kMaxSplit = 8;
 constexpr int kEarlyTokens = 16;
 constexpr int kSumBytes = kEarlyTokens * kRowTile * 4;
-constexpr int kTileLists = TileDigits::kPerTile, kTileTokens = kTileLists * TileDigits::kTokens;
-static_assert(kInlineTokens <= TileDigits::kTokens, "inline digits have one list a stage");
-static_assert(kTileTokens * TileDigits::kDigits == kRowTile, "a column tile");
+static_assert(Bf16Tile::kPerTile * Bf16Tile::kRows == kRowTile && Fp16Tile::kPerTile * Fp16Tile::kRows == kRowTile,
+              "a column tile");
+static_assert(Bf16Tile::kTileTokens <= kEarlyTokens && Fp16Tile::kTileTokens <= kEarlyTokens,
+              "what the digits leave goes where the ring was, beside the sums");
 // Two CTAs share an SM: half of its shared memory and of its tensor memory each.
 // (One CTA with twice the stages has the same bytes in flight but one MMA thread
 // and no second tile to cover its start and end: 28.6 us instead of 17.0 at
@@ -143,6 +142,10 @@ __device__ __forceinline__ void tmem_ld_8cols(uint32_t taddr, float (&r)[8]) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld_1col(uint32_t taddr, float& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(r) : "r"(taddr) : "memory");
+}
+
 __device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
@@ -197,39 +200,45 @@ __global__ void __launch_bounds__(Layout::kTokens * 32)
 
 // What a list that is too short counts, for one of its tokens: out of the way of the
 // stages' loop.
+template <typename Layout>
 __device__ __noinline__ float left_of_full_list(const RowsArgs& args, long long token, int kb, long long n) {
   const MxRows w{args.w, args.pitch, args.sw, args.kblocks, args.n};
-  return token < args.x.m ? left_again<TileDigits::kDigits>(args.x, token, kb, w, n) : 0.0f;
+  return token < args.x.m ? left_again<Layout::kDigits>(args.x, token, kb, w, n) : 0.0f;
 }
 
 // sums[t] += the weight row of this lane (row 0..127 of the tile) times what the lists of
-// a stage say of token t.  The warp has the lists in registers, eight lanes one: its
-// count, then the entries (zeros: no list).  codes, scales: the stage's weights in shared
+// a stage say of token t.  The warp has the lists in registers, eight lanes one (zeros: no
+// list).  codes, scales: the stage's weights in shared
 // memory.  A loop of few instructions: most of the time goes into fetching them, as the
 // code runs once in a while (two or four entries at once took longer, in registers too:
-// 33 x 5000 x 4136 fp16, three entries a stage, 16.0 us so, 16.5 and 17.9).
-__device__ __forceinline__ void add_listed(uint2 word, const uint8_t* codes, const uint8_t* scales, int row,
+// 33 x 5000 x 4136, three entries a stage, 16.0 us so, 16.5 and 17.9).
+template <typename Layout>
+__device__ __forceinline__ void add_listed(uint4 word, const uint8_t* codes, const uint8_t* scales, int row,
                                            float* sums) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t count = __shfl_sync(0xFFFFFFFFu, word.x, lane & 24);
-  word.x += static_cast<uint32_t>(lane >> 3) * LeftEntry::token(TileDigits::kTokens);
+  const int lane = threadIdx.x & 31, first = 2 * (lane & 7);  // of the list's 16 words: the count, 15 entries
+  const int count = static_cast<int>(__shfl_sync(0xFFFFFFFFu, word.x, lane & 24));
+  const uint32_t list = static_cast<uint32_t>(lane >> 3) * LeftEntry::token(Layout::kTokens);
   const float value = decode1(lane & 15);                        // of code lane % 16
   const uint32_t mine = smem_addr(codes) + row * kBlockBytes;    // 16-byte chunk c at c ^ (row % 8)
   const uint32_t swizzle = (row & 7) << 4;
   const uint32_t scale = smem_addr(scales) + (row & 31) * 16 + (row >> 5) * 4;
-  uint32_t left =
-      __ballot_sync(0xFFFFFFFFu, (lane & 7) != 0 && static_cast<uint32_t>(lane & 7) <= count && count <= kLeftEntries);
 #pragma unroll 1
-  for (; left != 0; left &= left - 1) {
-    const int from = __ffs(left) - 1;
-    const LeftEntry at{__shfl_sync(0xFFFFFFFFu, word.x, from)};
-    const float v = __uint_as_float(__shfl_sync(0xFFFFFFFFu, word.y, from));
-    uint32_t code, e8;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(mine + (at.byte() ^ swizzle)));
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e8) : "r"(scale + at.scale()));
-    // A NaN scale may pass as infinity: the row's product is not a number already.
-    sums[at.token()] += v * (__shfl_sync(0xFFFFFFFFu, value, code >> at.shift()) *
-                             __uint_as_float(max(e8 << 23, 0x00400000u)));
+  for (int half = 0; half < 2; ++half) {
+    const int at_word = first + half;
+    uint32_t left = __ballot_sync(0xFFFFFFFFu, at_word > 0 && at_word <= count && count <= kLeftEntries);
+#pragma unroll 1
+    for (; left != 0; left &= left - 1) {
+      const int from = __ffs(left) - 1;
+      const LeftEntry at{__shfl_sync(0xFFFFFFFFu, word.x + list, from)};
+      const float v = __uint_as_float(__shfl_sync(0xFFFFFFFFu, word.y, from));
+      uint32_t code, e8;
+      asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(mine + (at.byte() ^ swizzle)));
+      asm volatile("ld.shared.u8 %0, [%1];" : "=r"(e8) : "r"(scale + at.scale()));
+      // A NaN scale may pass as infinity: the row's product is not a number already.
+      sums[at.token()] += v * (__shfl_sync(0xFFFFFFFFu, value, code >> at.shift()) *
+                               __uint_as_float(max(e8 << 23, 0x00400000u)));
+    }
+    word.x = word.z, word.y = word.w;
   }
 }
 
@@ -237,10 +246,11 @@ __device__ __forceinline__ void add_listed(uint2 word, const uint8_t* codes, con
 // entries; u, raw, e8 and any are split_digits' of the warp.  Returns how many there are
 // then.  Not inlined: what runs once in a while lies out of the way of what always runs
 // (which every launch fetches: 7.25 us instead of 6.7 at 1 x 4096 x 4096).
+template <int DIGITS>
 __device__ __noinline__ uint32_t list_left(float4 u0, float4 u1, uint4 raw, bool bf16, int e8, bool any,
                                            uint32_t token, LeftList* list, uint32_t listed) {
   float left[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-  left_of<TileDigits::kDigits>(raw, bf16, left, e8);
+  left_of<DIGITS>(raw, bf16, left, e8);
   const uint32_t mine = any ? count_left(left) : 0u;
   append_left(list, listed, mine, token, left);
   return listed + __reduce_add_sync(0xFFFFFFFFu, mine);
@@ -270,7 +280,8 @@ __device__ __forceinline__ void finish(const float* sums, int split, int tokens,
   }
 }
 
-template <int XMODE>
+// Layout: of the digits of 16-bit rows.
+template <int XMODE, typename Layout = Bf16Tile>
 __global__ void __launch_bounds__(rows_threads(XMODE), 2)
     mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ RowsArgs args) {
@@ -292,11 +303,11 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
   const int kb0 = static_cast<int>(static_cast<long long>(args.kblocks) * rank / args.split);
   const int kb1 = static_cast<int>(static_cast<long long>(args.kblocks) * (rank + 1) / args.split);
   const int nkb = kb1 - kb0;
-  constexpr int kPerToken = XMODE == kXRows ? 1 : TileDigits::kDigits;  // columns of a token
-  const int token0 = col_tile * (kRowTile / kPerToken);
-  const int tokens = min(args.m - token0, kRowTile / kPerToken);
+  constexpr int kTileTokens = XMODE == kXRows ? kRowTile : Layout::kTileTokens;
+  const int token0 = col_tile * kTileTokens;
+  const int tokens = min(args.m - token0, kTileTokens);
   const int x_bytes = args.cols * kBlockBytes;
-  const int list_count = (tokens + TileDigits::kTokens - 1) / TileDigits::kTokens;  // of a stage
+  const int list_count = (tokens + Layout::kTokens - 1) / Layout::kTokens;  // of a stage
   LeftList* stage_lists = reinterpret_cast<LeftList*>(smem + args.stages * args.stage_bytes + kSumBytes);
 
   auto load_w = [&](int it, int s) {
@@ -319,8 +330,8 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
                  args.sx + (static_cast<long long>(col_tile) * args.kblocks + kb) * kScaleBlock, kScaleBlock,
                  bar);
     if constexpr (XMODE == kXDigits)
-      bulk_load_1d(stage_lists + s * kTileLists,
-                   args.lists + TileDigits::index(static_cast<long long>(col_tile) * kTileLists, kb, args.kblocks),
+      bulk_load_1d(stage_lists + s * Layout::kPerTile,
+                   args.lists + Layout::index(static_cast<long long>(col_tile) * Layout::kPerTile, kb, args.kblocks),
                    list_count * static_cast<int>(sizeof(LeftList)), bar);
   };
   // An X warp's next values (inline digits): asked for one round ahead, the first
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
   const uint32_t tsf = tbase + static_cast<uint32_t>((args.cols + 31) & ~31);
   const int row_of_lane = 32 * (warp & 3) + lane;
   // A scale writer's sums of what the digits leave: its lane's row, a token each.
-  constexpr int kStageLists = XMODE == kXInline ? 1 : kTileLists, kStageTokens = kStageLists * TileDigits::kTokens;
+  constexpr int kStageLists = XMODE == kXInline ? 1 : Layout::kPerTile, kStageTokens = kStageLists * Layout::kTokens;
   [[maybe_unused]] float left_sums[kStageTokens] = {};
   [[maybe_unused]] bool any_left = false;
 
@@ -447,16 +458,16 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
       if constexpr (XMODE != kXRows) {
-        uint2 word = make_uint2(0, 0);
-        if (lane < 8 * list_count) word = reinterpret_cast<const uint2*>(stage_lists + s * kStageLists)[lane];
+        uint4 word = make_uint4(0, 0, 0, 0);
+        if (lane < 8 * list_count) word = reinterpret_cast<const uint4*>(stage_lists + s * kStageLists)[lane];
         if (__any_sync(0xFFFFFFFFu, (lane & 7) == 0 && word.x != 0)) {
           any_left = true;
-          add_listed(word, smem + s * args.stage_bytes, sw - lane * 16, row_of_lane, left_sums);
+          add_listed<Layout>(word, smem + s * args.stage_bytes, sw - lane * 16, row_of_lane, left_sums);
           uint32_t full = __ballot_sync(0xFFFFFFFFu, (lane & 7) == 0 && word.x > kLeftEntries);
           for (; full != 0; full &= full - 1) {
-            const int first = (__ffs(full) - 1) / 8 * TileDigits::kTokens;
-            for (int t = first; t < first + TileDigits::kTokens; ++t)
-              left_sums[t] += left_of_full_list(args, token0 + t, kb0 + it,
+            const int first = (__ffs(full) - 1) / 8 * Layout::kTokens;
+            for (int t = first; t < first + Layout::kTokens; ++t)
+              left_sums[t] += left_of_full_list<Layout>(args, token0 + t, kb0 + it,
                                                 static_cast<long long>(tile) * kRowTile + row_of_lane);
           }
           __syncwarp();
@@ -466,8 +477,8 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
     }
   } else if (XMODE == kXInline) {
     // -------------------------------------------------------------- X warps
-    // One warp a stage: digit d of token i is row 8 i + d of the X tile, whose
-    // 16-byte chunk c lies at c ^ d (the 128-byte swizzle).
+    // One warp a stage: digit d of token i is row i * kDigits + d of the X tile, whose
+    // 16-byte chunk c lies at c ^ (row % 8) (the 128-byte swizzle).
     RingPlace at;
     at.advance(warp - 6, args.stages);
     for (int it = warp - 6; it < nkb; it += kXWarps, at.advance(kXWarps, args.stages)) {
@@ -483,15 +494,15 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
         const int group = lane >> 2;
         float u[8];
         int e8;
-        const bool any = split_digits<TileDigits::kDigits>(
+        const bool any = split_digits<Layout::kDigits>(
             x_next[token], args.x.bf16, u, e8, [&](int d, uint8_t code, uint32_t words) {
-              const int row = token * TileDigits::kDigits + d;
-              *reinterpret_cast<uint32_t*>(xt + row * kBlockBytes + ((group ^ d) << 4) + (lane & 3) * 4) = words;
+              const int row = token * Layout::kDigits + d;
+              *reinterpret_cast<uint32_t*>(xt + row * kBlockBytes + ((group ^ (row & 7)) << 4) + (lane & 3) * 4) = words;
               if ((lane & 3) == 0)
                 sx[(group >> 2) * 512 + (row & 31) * 16 + (row >> 5) * 4 + (group & 3)] = code;
             });
         if (__any_sync(0xFFFFFFFFu, any))
-          listed = list_left(make_float4(u[0], u[1], u[2], u[3]), make_float4(u[4], u[5], u[6], u[7]), x_next[token],
+          listed = list_left<Layout::kDigits>(make_float4(u[0], u[1], u[2], u[3]), make_float4(u[4], u[5], u[6], u[7]), x_next[token],
                              args.x.bf16, e8, any, token, stage_lists + s, listed);
       }
       if (lane == 0) stage_lists[s].count = listed;
@@ -531,17 +542,24 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
     auto send = [&](int token, float v) {
       st_shared_cluster_f32(to + static_cast<uint32_t>(token * share * 4), v);
     };
-    for (int c = 0; c < tokens * kPerToken; c += 8) {
-      float r[8];
-      tmem_ld_8cols(taddr + static_cast<uint32_t>(c), r);
-      tmem_wait_ld();
-      if constexpr (XMODE == kXRows) {
+    if constexpr (XMODE == kXRows) {
+      for (int c = 0; c < tokens; c += 8) {
+        float r[8];
+        tmem_ld_8cols(taddr + static_cast<uint32_t>(c), r);
+        tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           if (c + i < tokens) send(c + i, r[i]);
-      } else {
-        const int token = c / TileDigits::kDigits;
-        float sum = sum_digits<TileDigits::kDigits>(r);
+      }
+    } else {
+      for (int token = 0; token < tokens; ++token) {
+        static_assert(Layout::kDigits == 8 || Layout::kDigits == 9, "columns of a token");
+        const uint32_t at = taddr + static_cast<uint32_t>(Layout::column(token));
+        float r[9];
+        tmem_ld_8cols(at, reinterpret_cast<float(&)[8]>(r));
+        if constexpr (Layout::kDigits == 9) tmem_ld_1col(at + 8, r[8]);
+        tmem_wait_ld();
+        float sum = sum_digits<Layout::kDigits>(r);
         if (any_left) sum += left_in_ring[token * kRowTile + row];
         send(token, sum);
       }
@@ -613,7 +631,7 @@ int launch_digits(const RowsArgs& args, const DigitSpace& space, uint8_t* base, 
                             reinterpret_cast<LeftList*>(base + space.lists_at));
 }
 
-template <int XMODE>
+template <int XMODE, typename Layout = Bf16Tile>
 int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs args, const DeviceFacts& facts,
                 cudaStream_t stream) {
   args.col_tiles = (args.cols + kRowTile - 1) / kRowTile;
@@ -636,7 +654,7 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   if (args.kblocks >= 4 && tiles * 4 <= places - 16) args.split = 4;
   if (args.kblocks >= kMaxSplit && tiles * kMaxSplit <= most_in_eights) args.split = kMaxSplit;
   if (tiles * args.split > INT_MAX) return TCB_ERR_RESOURCE;
-  constexpr int kLists = XMODE == kXRows ? 0 : XMODE == kXInline ? 1 : kTileLists;
+  constexpr int kLists = XMODE == kXRows ? 0 : XMODE == kXInline ? 1 : Layout::kPerTile;
   constexpr int list_bytes = kLists * static_cast<int>(sizeof(LeftList));
   args.stages = (kSmemBudget - 1024 - kSumBytes) / (args.stage_bytes + list_bytes);
   if (args.stages > kMaxStages) args.stages = kMaxStages;
@@ -648,7 +666,7 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
   // N of the instruction; M = 128, E2M1 x E2M1, E8M0 scales as the pair MMA.
   args.idesc = (gemm_pair_idesc() & ~(0x3Fu << 17 | 0x1Fu << 24)) |
                static_cast<uint32_t>(args.cols >> 3) << 17 | static_cast<uint32_t>(kRowTile >> 4) << 24;
-  auto fn = mx_rows_kernel<XMODE>;
+  auto fn = mx_rows_kernel<XMODE, Layout>;
   static DeviceIntCache cap_cache;
   const int cap = cap_cache.get(facts.device, [&] {
     return raise_dynamic_smem(reinterpret_cast<const void*>(fn), facts.max_smem_optin);
@@ -659,15 +677,65 @@ int launch_rows(const CUtensorMap& map_w, const CUtensorMap& map_x, RowsArgs arg
                             args);
 }
 
+// 16-bit rows.
+template <typename Layout>
+int run_16bit(const RowsProblem& p, RowsArgs args, const CUtensorMap& map_w, void* workspace, int* status,
+              const DeviceFacts& facts, cudaStream_t stream) {
+  CUtensorMap map_x{};
+  if (p.m <= kInlineTokens) {
+    args.cols = Layout::columns(p.m);
+    return launch_rows<kXInline, Layout>(map_w, map_x, args, facts, stream);
+  }
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  int rc;
+  // Column tiles while two of them fit an SM and all run at once.  Measured (us, column
+  // tiles / pairs, bf16 activations): 128 x 4096 x 4096 (256 tiles) 22.3/24.1, 48 x 12288 x
+  // 4096 (288) 20.9/25.1; 64 x 12288 x 4096 (384) 29.3/26.4, 33 x 16384 x 8192 (384)
+  // 45.0/36.7, 20 x 32768 x 4096 (512) 31.8/26.9.
+  const long long row_tiles = (static_cast<long long>(p.n) + kRowTile - 1) / kRowTile;
+  const long long col_tiles = (static_cast<long long>(p.m) + Layout::kTileTokens - 1) / Layout::kTileTokens;
+  if (col_tiles > 1 && col_tiles * row_tiles > 2ll * facts.sm_count) {
+    // Columns of the CTA-pair GEMM, whose M side is the weight.
+    const DigitSpace space(SliceDigits{}, p.m, p.k);
+    if ((rc = launch_digits<SliceDigits>(args, space, base, stream)) != TCB_OK) return rc;
+    PairProblem q = {};
+    q.a = p.w;
+    q.b = base + space.codes_at;
+    q.sa = p.sw;
+    q.sb = base;
+    q.bias = p.bias;
+    q.c = p.y;
+    q.ldc = p.ldy;
+    q.m = p.n;
+    q.n = static_cast<int>(space.rows);
+    q.k = static_cast<int>(mx_padded(p.k));
+    q.out = p.y_type == kRowsFp32 ? kPairFp32 : p.y_type == kRowsBf16 ? kPairBf16 : kPairFp16;
+    q.idesc = gemm_pair_idesc();
+    q.overlap = true;
+    q.digits_of = &args.x;
+    q.digits_left = reinterpret_cast<const LeftList*>(base + space.lists_at);
+    return gemm_pair_run(q, 0, status, facts, stream);
+  }
+  const DigitSpace space(Layout{}, p.m, p.k);
+  if ((rc = launch_digits<Layout>(args, space, base, stream)) != TCB_OK) return rc;
+  args.cols = Layout::columns(p.m);
+  args.sx = base;
+  args.lists = reinterpret_cast<const LeftList*>(base + space.lists_at);
+  rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols < kRowTile ? args.cols : kRowTile);
+  if (rc != TCB_OK) return rc;
+  return launch_rows<kXDigits, Layout>(map_w, map_x, args, facts, stream);
+}
+
 }  // namespace
 
-// Column tiles of the few-row kernel or columns of the CTA-pair GEMM, which N decides.
+// X's type decides the digits, N whether they are column tiles of the few-row kernel or
+// columns of the CTA-pair GEMM: room for any.
 long long mx_rows_workspace(long long m, long long k) {
   if (m <= kInlineTokens) return 0;
-  const long long tile = DigitSpace(TileDigits{}, m, k).bytes;
-  if (m <= kTileTokens) return tile;
+  const long long bf16 = DigitSpace(Bf16Tile{}, m, k).bytes, fp16 = DigitSpace(Fp16Tile{}, m, k).bytes;
   const long long slice = DigitSpace(SliceDigits{}, m, k).bytes;
-  return tile > slice ? tile : slice;
+  const long long most = bf16 > fp16 ? bf16 : fp16;
+  return most > slice ? most : slice;
 }
 
 int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const DeviceFacts& facts,
@@ -695,47 +763,8 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
     if ((rc = rows_map(&map_x, p.x, p.m, args.pitch, args.cols < kRowTile ? args.cols : kRowTile)) != TCB_OK) return rc;
     return launch_rows<kXRows>(map_w, map_x, args, facts, stream);
   }
-  if (p.m <= kInlineTokens) {
-    args.cols = p.m * TileDigits::kDigits;
-    return launch_rows<kXInline>(map_w, map_x, args, facts, stream);
-  }
-  uint8_t* base = static_cast<uint8_t*>(workspace);
-  // Column tiles while two of them fit an SM and all run at once.  Measured (us, column
-  // tiles / pairs, bf16 activations): 128 x 4096 x 4096 (256 tiles) 22.3/24.1, 48 x 12288 x
-  // 4096 (288) 20.9/25.1; 64 x 12288 x 4096 (384) 29.3/26.4, 33 x 16384 x 8192 (384)
-  // 45.0/36.7, 20 x 32768 x 4096 (512) 31.8/26.9.
-  const long long row_tiles = (static_cast<long long>(p.n) + kRowTile - 1) / kRowTile;
-  const long long col_tiles = (static_cast<long long>(p.m) + kTileTokens - 1) / kTileTokens;
-  if (col_tiles > 1 && col_tiles * row_tiles > 2ll * facts.sm_count) {
-    // Columns of the CTA-pair GEMM, whose M side is the weight.
-    const DigitSpace space(SliceDigits{}, p.m, p.k);
-    if ((rc = launch_digits<SliceDigits>(args, space, base, stream)) != TCB_OK) return rc;
-    PairProblem q = {};
-    q.a = p.w;
-    q.b = base + space.codes_at;
-    q.sa = p.sw;
-    q.sb = base;
-    q.bias = p.bias;
-    q.c = p.y;
-    q.ldc = p.ldy;
-    q.m = p.n;
-    q.n = static_cast<int>(space.rows);
-    q.k = static_cast<int>(mx_padded(p.k));
-    q.out = p.y_type == kRowsFp32 ? kPairFp32 : p.y_type == kRowsBf16 ? kPairBf16 : kPairFp16;
-    q.idesc = gemm_pair_idesc();
-    q.overlap = true;
-    q.digits_of = &args.x;
-    q.digits_left = reinterpret_cast<const LeftList*>(base + space.lists_at);
-    return gemm_pair_run(q, 0, status, facts, stream);
-  }
-  const DigitSpace space(TileDigits{}, p.m, p.k);
-  if ((rc = launch_digits<TileDigits>(args, space, base, stream)) != TCB_OK) return rc;
-  args.cols = p.m * TileDigits::kDigits;
-  args.sx = base;
-  args.lists = reinterpret_cast<const LeftList*>(base + space.lists_at);
-  rc = rows_map(&map_x, base + space.codes_at, args.cols, args.pitch, args.cols < kRowTile ? args.cols : kRowTile);
-  if (rc != TCB_OK) return rc;
-  return launch_rows<kXDigits>(map_w, map_x, args, facts, stream);
+  return args.x.bf16 ? run_16bit<Bf16Tile>(p, args, map_w, workspace, status, facts, stream)
+                     : run_16bit<Fp16Tile>(p, args, map_w, workspace, status, facts, stream);
 }
 
 }  // namespace tcb
