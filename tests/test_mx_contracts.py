@@ -3,7 +3,13 @@ and what happens at the edges of the calls."""
 
 import re
 
+import pytest
+import torch
+
 from conftest import REPO
+from triton_chip_benchmarks_b200 import mx
+
+gpu = pytest.mark.gpu
 
 CSRC = REPO / "triton_chip_benchmarks_b200" / "csrc"
 
@@ -21,3 +27,15 @@ def test_kernels_that_start_early_read_with_ordinary_loads():
     for path in [*early, *sorted(CSRC.glob("tcb_mx*.cuh"))]:
         for word in ("__ldg", "__restrict__", "ld.global.nc", "__ldca", "__ldcg"):
             assert word not in code(path), (path.name, word)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3, 64), (2, 3, 64)])
+def test_a_layer_without_outputs_has_zero_gradients(cuda, shape):
+    """dx sums over the outputs: over none it is zero, as dw is over no rows."""
+    x, w = torch.ones(shape, device=cuda, dtype=torch.bfloat16), torch.ones(0, 64, device=cuda)
+    y, saved = mx.linear_forward(x, w)
+    assert y.shape == (*shape[:-1], 0)
+    dx, dw = mx.linear_backward(torch.zeros(*shape[:-1], 0, device=cuda, dtype=torch.bfloat16), saved)
+    assert dx.shape == x.shape and dx.dtype == x.dtype and (dx == 0).all()
+    assert dw.shape == (0, 64) and dw.dtype == w.dtype

@@ -409,7 +409,7 @@ def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = Tru
     """(dx, dw) of y = Q(x) . Q(w)^T for the gradient dy [..., out] of y.
 
     dx = Q(dy) . Q(w^T)^T in x's type and shape, dw = Q(dy^T) . Q(x^T)^T in w's type
-    (None where not needed); with no rows dw is zero.
+    (None where not needed); with no rows dw is zero, with no outputs dx.
     """
     out_features, in_features = saved.w.cols, saved.w.rows
     shape = saved.x_shape[:-1] + (out_features,)
@@ -429,9 +429,12 @@ def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = Tru
             dy_cols = MxTensor.empty_on(flat, out_features, tokens)
         _quantize(flat, saved.rule, dy_rows, dy_cols)
     if need_dx:
-        dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype)
-        if len(saved.x_shape) != 2:
-            dx = dx.view(saved.x_shape)
+        if out_features == 0:
+            dx = torch.zeros(saved.x_shape, dtype=saved.x_dtype, device=dy.device)
+        else:
+            dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype)
+            if len(saved.x_shape) != 2:
+                dx = dx.view(saved.x_shape)
     if need_dw:
         if saved.x.cols == 0:
             dw = torch.zeros((out_features, in_features), dtype=saved.w_dtype, device=dy.device)
