@@ -13,6 +13,9 @@ tensors' device and on its current stream, allocate their outputs through torch 
   MX products (both passes quantise their operands along the axis that the
   product sums over; gradients pass the rounding unchanged).
 
+The operators are outside autograd: an output of one never requires a gradient, and
+:func:`linear_backward` is called by hand (or by a ``torch.autograd.Function``).
+
 Results are rounded once, from fp32 sums.  Arguments that an operator does not take
 raise ``TypeError`` (types) or ``ValueError`` (shapes, strides, devices); what the
 library itself refuses raises :class:`_native.TcbError`.
@@ -298,7 +301,9 @@ def matmul(a: MxTensor, b: MxTensor, *, bias: torch.Tensor | None = None,
            status: torch.Tensor | None = None) -> torch.Tensor:
     """a [M][K] . b [N][K]^T (+ bias [N]) in `dtype` (or out's type).
 
-    ``status`` (an int32 device word) receives an error of a device-side wait.
+    ``status`` (an int32 device word) receives an error of a device-side wait; without
+    one such an error is not reported, and what the wait's tiles should have held is
+    left unwritten.
     """
     m, n, k = a.rows, b.rows, a.cols
     if k != b.cols:
@@ -341,7 +346,8 @@ def linear(x: torch.Tensor, w: MxTensor, *, bias: torch.Tensor | None = None,
     group of 32) take longer.  The first digit may be a seventh larger than its value, so
     sums that come within that of fp32's largest number may be infinite.  A few rows
     cost little more than reading w once, a prompt's several products of MX rows
-    (quantise x too where that matters).  ``out`` is a matrix [rows][N].
+    (quantise x too where that matters).  ``out`` is a matrix [rows][N]; ``status`` as in
+    :func:`matmul`.
     """
     x_dtype = x.dtype
     if x_dtype != torch.bfloat16 and x_dtype != torch.float16:
@@ -381,11 +387,12 @@ class LinearSaved:
     rule: str
 
 
-def linear_forward(x: torch.Tensor, w: torch.Tensor, *,
-                   rule: str = "floor") -> tuple[torch.Tensor, LinearSaved]:
+def linear_forward(x: torch.Tensor, w: torch.Tensor, *, rule: str = "floor",
+                   status: torch.Tensor | None = None) -> tuple[torch.Tensor, LinearSaved]:
     """y = Q(x) . Q(w)^T for x [..., in], w [out][in], and what the backward pass needs.
 
-    Each of x and w is read once and quantised along both axes.
+    Each of x and w is read once and quantised along both axes.  ``status`` as in
+    :func:`matmul`.
     """
     if w.dim() != 2 or x.dim() == 0 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"x is [..., in] and w [out][in], got {list(x.shape)} and {list(w.shape)}")
@@ -399,17 +406,18 @@ def linear_forward(x: torch.Tensor, w: torch.Tensor, *,
     x_cols, w_cols = MxTensor.two_on(w, (inner, tokens), (inner, outer))
     _quantize(flat, rule, x_rows, x_cols)
     _quantize(w, rule, w_rows, w_cols)
-    y = matmul(x_rows, w_rows, dtype=x.dtype)
+    y = matmul(x_rows, w_rows, dtype=x.dtype, status=status)
     saved = LinearSaved(x_cols, w_cols, tuple(x.shape), x.dtype, w.dtype, rule)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0]), saved
 
 
-def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = True,
-                    need_dw: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = True, need_dw: bool = True,
+                    status: torch.Tensor | None = None) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """(dx, dw) of y = Q(x) . Q(w)^T for the gradient dy [..., out] of y.
 
     dx = Q(dy) . Q(w^T)^T in x's type and shape, dw = Q(dy^T) . Q(x^T)^T in w's type
     (None where not needed); with no rows dw is zero, with no outputs dx.
+    ``status`` as in :func:`matmul`, for both products.
     """
     out_features, in_features = saved.w.cols, saved.w.rows
     shape = saved.x_shape[:-1] + (out_features,)
@@ -432,12 +440,12 @@ def linear_backward(dy: torch.Tensor, saved: LinearSaved, *, need_dx: bool = Tru
         if out_features == 0:
             dx = torch.zeros(saved.x_shape, dtype=saved.x_dtype, device=dy.device)
         else:
-            dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype)
+            dx = matmul(dy_rows, saved.w, dtype=saved.x_dtype, status=status)
             if len(saved.x_shape) != 2:
                 dx = dx.view(saved.x_shape)
     if need_dw:
         if saved.x.cols == 0:
             dw = torch.zeros((out_features, in_features), dtype=saved.w_dtype, device=dy.device)
         else:
-            dw = matmul(dy_cols, saved.x, dtype=saved.w_dtype)
+            dw = matmul(dy_cols, saved.x, dtype=saved.w_dtype, status=status)
     return dx, dw
