@@ -2,11 +2,14 @@
 and what happens at the edges of the calls."""
 
 import re
+import sys
+import sysconfig
 
 import pytest
 import torch
 
 from conftest import REPO
+from triton_chip_benchmarks_b200 import build as tcb_build
 from triton_chip_benchmarks_b200 import mx
 
 gpu = pytest.mark.gpu
@@ -69,3 +72,52 @@ def test_the_products_reach_the_library_with_their_status_word(monkeypatch):
     saved.x.index = -1  # host tensors
     mx.linear_backward(torch.zeros(4, 8), saved, status=word)
     assert words == [word] * 3
+
+
+# ------------------------------------------------------- the module of entry points
+def test_the_library_is_built_where_the_python_module_cannot_be(monkeypatch, tmp_path, capsys):
+    monkeypatch.setattr(tcb_build, "CALLS", tmp_path / "_tcb_calls.so")
+    monkeypatch.setattr(sysconfig, "get_paths", lambda: {"include": str(tmp_path)})  # no Python.h
+    assert tcb_build.build() == tcb_build.LIBRARY and tcb_build.LIBRARY.exists()
+    assert not tcb_build.CALLS.exists() and "tcb_pycalls.c" in capsys.readouterr().err
+
+
+def test_the_python_module_is_named_for_its_python():
+    assert tcb_build.CALLS.name.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def without_module(native, monkeypatch):
+    """_native.calls() where _tcb_calls cannot be imported."""
+    package = native.__package__
+    monkeypatch.setitem(sys.modules, f"{package}._tcb_calls", None)
+    monkeypatch.delattr(sys.modules[package], "_tcb_calls", raising=False)
+    monkeypatch.setattr(native, "_bound_to", None)
+    monkeypatch.setattr(native, "_calls", None)
+    return native.calls()
+
+
+def test_entry_points_without_the_python_module(native, monkeypatch):
+    calls = without_module(native, monkeypatch)
+    p = 0x1000  # never dereferenced
+    assert not hasattr(calls, "bind")
+    assert calls.tcb_mx_quantize(0, p, 4, 4, 3, 0, p, p, None, None, None) == native.ERR_INVALID_ARGUMENT
+    assert calls.tcb_mx_gemm(p, p, p, p, None, 0, p, 8, 1 << 32, 8, 32, None, None) == \
+        native.ERR_INVALID_ARGUMENT  # a size past int is not cut off
+    assert calls.tcb_mx_gemm(None, None, None, None, None, 0, None, 8, 0, 8, 32, None, None) == native.OK
+    with pytest.raises(TypeError):
+        calls.tcb_mx_dequantize(0, p, p)
+    with pytest.raises(TypeError):
+        calls.tcb_mx_quantize(0, "x", 4, 4, 4, 0, p, p, None, None, None)
+    with pytest.raises(OverflowError):
+        calls.tcb_mx_quantize(0, 1 << 70, 4, 4, 4, 0, p, p, None, None, None)
+
+
+@gpu
+def test_operators_without_the_python_module(cuda, native, monkeypatch):
+    x, w = torch.randn(3, 64, device=cuda).bfloat16(), torch.randn(40, 64, device=cuda)
+    q = mx.quantize(w)
+    expected = mx.linear(x, q), mx.matmul(q, q), mx.dequantize(q)
+    without_module(native, monkeypatch)
+    again = mx.quantize(w)
+    for got, want in zip((mx.linear(x, again), mx.matmul(again, again), mx.dequantize(again)), expected):
+        assert torch.equal(got, want)

@@ -165,13 +165,44 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+# The MX FP4 operators' entry points and which of their arguments are ints.
+_OPERATORS = {"tcb_mx_quantize": (0, 5), "tcb_mx_dequantize": (0,), "tcb_mx_gemm": (5, 8, 9, 10),
+              "tcb_mx_linear": (0, 6, 9, 10, 11)}
+
 _calls = None
 _bound_to: ctypes.CDLL | None = None
 
 
+class _CtypesCalls:
+    """The entry points as _tcb_calls has them, through ctypes: a size past an int's
+    range becomes -1, which each of them refuses (ctypes would cut it off)."""
+
+    def __init__(self, lib: ctypes.CDLL):
+        for name, ints in _OPERATORS.items():
+            setattr(self, name, self._checked(getattr(lib, name), ints))
+
+    @staticmethod
+    def _checked(fn, ints):
+        def call(*args):
+            if len(args) != len(fn.argtypes):
+                raise TypeError(f"{len(fn.argtypes)} arguments expected, got {len(args)}")
+            values = list(args)
+            for i, v in enumerate(values):
+                if v is not None and not isinstance(v, int):
+                    raise TypeError(f"argument {i} is an integer, got {type(v).__name__}")
+                if v is not None and not -(1 << 63) <= v < 1 << 63:
+                    raise OverflowError(f"argument {i} does not fit 64 bits")
+                if i in ints:
+                    values[i] = v if v is not None and 0 <= v < 1 << 31 else 0 if v is None else -1
+                elif v is None and fn.argtypes[i] is not ctypes.c_void_p:
+                    values[i] = 0
+            return fn(*values)
+        return call
+
+
 def calls():
-    """The module of the MX FP4 entry points (integers in, status out), bound to the
-    loaded library; raises NativeLibraryError when it has not been built."""
+    """The MX FP4 entry points (integers in, status out) of the loaded library: the
+    _tcb_calls module bound to it, or ctypes functions where that has not been built."""
     global _calls, _bound_to
     lib = load()
     if _bound_to is lib:
@@ -179,13 +210,12 @@ def calls():
     with _lock:
         try:
             from . import _tcb_calls
-        except ImportError as exc:
-            raise NativeLibraryError(
-                f"cannot import _tcb_calls ({exc}); build it with "
-                "`python -m triton_chip_benchmarks_b200.build`") from exc
-        _tcb_calls.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "tcb_mx_quantize", "tcb_mx_dequantize", "tcb_mx_gemm", "tcb_mx_linear")))
-        _calls, _bound_to = _tcb_calls, lib
+        except ImportError:
+            found = _CtypesCalls(lib)
+        else:
+            found = _tcb_calls
+            found.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _OPERATORS))
+        _calls, _bound_to = found, lib
     return _calls
 
 

@@ -3,8 +3,9 @@
 Compiles every ``csrc/*.cu`` for ``sm_100a`` with nvcc (object files in
 ``_build/`` beside this file, incremental on source/header timestamps) and
 links them, with the CUDA runtime linked statically, into
-``triton_chip_benchmarks_b200/libtcb.so``; compiles ``csrc/tcb_pycalls.c`` into the
-Python module ``_tcb_calls`` beside it.  Run ``python -m
+``triton_chip_benchmarks_b200/libtcb.so``; then compiles ``csrc/tcb_pycalls.c`` into the
+Python module ``_tcb_calls`` beside it, for this Python (without it the operators go
+through ctypes, 2 us a call slower).  Run ``python -m
 triton_chip_benchmarks_b200.build`` or call :func:`build`.
 """
 
@@ -24,7 +25,8 @@ CSRC = PACKAGE_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 BUILD_DIR = PACKAGE_DIR / "_build"
 LIBRARY = PACKAGE_DIR / "libtcb.so"
-CALLS = PACKAGE_DIR / "_tcb_calls.so"
+# Named for the Python that it is compiled for: another one builds its own.
+CALLS = PACKAGE_DIR / ("_tcb_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -71,18 +73,23 @@ def _compile(nvcc: str, source: Path, verbose: bool) -> Path:
 
 
 def _build_calls() -> None:
-    """The Python module of the MX FP4 entry points (no CUDA in it)."""
+    """The Python module of the MX FP4 entry points (no CUDA in it).  Optional: where it
+    cannot be compiled (no compiler, no Python.h) there is a warning."""
     source = CSRC / "tcb_pycalls.c"
+    untagged = PACKAGE_DIR / "_tcb_calls.so"  # would be imported by any Python
+    if untagged != CALLS:
+        untagged.unlink(missing_ok=True)
     if not _stale(CALLS, [source, *_headers()]):
         return
     cc = shutil.which("cc") or shutil.which("gcc")
     if cc is None:
-        raise RuntimeError("no C compiler on PATH")
+        print("warning: no C compiler on PATH, _tcb_calls is not built", file=sys.stderr)
+        return
     cmd = [cc, "-O2", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"], "-I", str(INCLUDE),
            "-o", str(CALLS), str(source)]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"cc failed for {source.name}:\n{result.stdout}\n{result.stderr}")
+        print(f"warning: {source.name} is not built:\n{result.stdout}{result.stderr}", file=sys.stderr)
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
@@ -92,13 +99,13 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     sources = sorted(CSRC.glob("*.cu"))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs or os.cpu_count() or 4) as pool:
         objects = list(pool.map(lambda src: _compile(nvcc, src, verbose), sources))
-    _build_calls()
     if _stale(LIBRARY, objects):
         cmd = [nvcc, *ARCH_FLAGS, "-shared", "-cudart", "static", "-o", str(LIBRARY),
                *map(str, objects)]
         result = subprocess.run(cmd, capture_output=True, text=True)
         if result.returncode != 0:
             raise RuntimeError(f"link failed:\n{result.stdout}\n{result.stderr}")
+    _build_calls()
     return LIBRARY
 
 
