@@ -350,28 +350,6 @@ def mx_quantize(dtype: int, x, rows: int, cols: int, ld: int, rule: int, codes, 
                                  _ptr(codes_t), _ptr(scales_t), _stream(stream)), "tcb_mx_quantize")
 
 
-def mx_dequantize(dtype: int, codes, scales, rows: int, cols: int, y, ld: int,
-                  stream=None) -> None:
-    check(load().tcb_mx_dequantize(dtype, _ptr(codes), _ptr(scales), rows, cols, _ptr(y), ld,
-                                   _stream(stream)), "tcb_mx_dequantize")
-
-
-def mx_gemm(a, scale_a, b, scale_b, c, m: int, n: int, k: int, *, dtype: int, ldc: int, bias=None,
-            status=None, stream=None) -> None:
-    """C = A . B^T (+ bias) of two MX FP4 matrices, C in `dtype`."""
-    check(load().tcb_mx_gemm(_ptr(a), _ptr(scale_a), _ptr(b), _ptr(scale_b), _ptr(bias), dtype,
-                             _ptr(c), ldc, m, n, k, _ptr(status), _stream(stream)), "tcb_mx_gemm")
-
-
-def mx_linear(x_dtype: int, x, ldx: int, w, scale_w, y, m: int, n: int, k: int, *, dtype: int,
-              ldy: int, workspace=None, workspace_bytes: int = 0, bias=None, status=None,
-              stream=None) -> None:
-    """Y = X . W^T (+ bias) with 16-bit X and an MX FP4 weight, Y in `dtype`."""
-    check(load().tcb_mx_linear(x_dtype, _ptr(x), ldx, _ptr(w), _ptr(scale_w), _ptr(bias), dtype,
-                               _ptr(y), ldy, m, n, k, _ptr(workspace), workspace_bytes,
-                               _ptr(status), _stream(stream)), "tcb_mx_linear")
-
-
 def mx_linear_workspace_bytes(m: int, k: int) -> int:
     """Bytes of mx_linear's workspace for m rows of k values."""
     n = load().tcb_mx_linear_workspace_bytes(m, k)
