@@ -246,7 +246,6 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Every thread of both CTAs of the cluster.
 // The two halves of a cluster barrier, without ordering of memory before it: a CTA
 // that has waited knows that the others have started, so that it may write to
 // their shared memory.
@@ -257,6 +256,7 @@ __device__ __forceinline__ void cluster_wait_started() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Every thread of all CTAs of the cluster.
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
                    : "memory");
