@@ -309,7 +309,10 @@ __device__ __forceinline__ void store_digits(const PairArgs& args, const uint32_
 
 // How C leaves: through the C tensor map (rows on 16-byte boundaries), by plain
 // stores through the same shared memory, or as a digit product.  A kernel each:
-// the epilogue has 64 of 80 registers in the accumulator slice.
+// the epilogue has 64 of 80 registers in the accumulator slice, and what else it holds
+// spills (bytes a thread stored: through the map 12 to 16, 68 with a 16-bit bias; plain
+// stores 20 to 148; digits 48).  Measured, it does not show: fp32 through the map takes
+// 41.9 us at 4096^3 (42.6 with the 8 bytes of a kernel of its own).
 enum StoreMode : int { kStoreTma = 0, kStorePlain = 1, kStoreDigits = 2 };
 
 template <int OUT, bool BIAS, int STORE>
