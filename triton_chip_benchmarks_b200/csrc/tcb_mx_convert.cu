@@ -26,8 +26,8 @@
 // column-wise loads conflict; a thread takes four times 16 values of a row, then
 // 32 rows of one word (two 16-bit columns, or one fp32), and the column codes
 // are turned round through shared memory into 64-byte runs.  8192 x 4096 bf16:
-// 20.5 us, 103 MB, 5.0 TB/s; the integer pipe is 70 % busy and the issue slots
-// 74 %, so instructions bound it (46 us with the loads one by one, 23.5 before the
+// 20.5 us, 103 MB, 5.0 TB/s; the integer pipe is 64 % busy and the issue slots
+// 72 %, so instructions bound it (46 us with the loads one by one, 23.5 before the
 // mixed-precision scaling).  Rows that do not start on 16-byte boundaries come through
 // the same tile: inside the matrix a thread reads the two aligned chunks that its
 // 16 bytes lie in and shifts them together (element by element 70 us instead of
