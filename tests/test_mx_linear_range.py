@@ -43,8 +43,7 @@ def rows_and_weight(m, n, k, dtype, shift, share, seed):
     codes[:, large] = 0
     low, unit = (129, 1.0) if dtype == BF16 else (1025, 2.0**-14)
     x = (2 * gen.integers(0, low // 2, (m, k)) + low) * unit * gen.choice([-1, 1], (m, k))  # full mantissas
-    if dtype == FP16:
-        x *= gen.random((m, k)) < min(1.0, 400 / k)  # so that the sums fit 24 bits
+    x *= gen.random((m, k)) < min(1.0, (400 if dtype == FP16 else 4000) / k)  # so that the sums fit 24 bits
     for g, at in enumerate(large):
         has = gen.random(m) < share
         if share < 1:
@@ -78,6 +77,16 @@ def test_linear_keeps_small_values_beside_large_ones(cuda, m, n, k, dtype, shift
     got = mx.linear(x.to(cuda), w, bias=bias, dtype=FP32, status=status)
     assert torch.equal(got.cpu(), torch.from_numpy(exact + bias.cpu().double().numpy()).float())
     assert status.item() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype,shift", [(BF16, 24), (FP16, 19)])
+@pytest.mark.parametrize("m,n,k", [(14, 140, 700), (15, 140, 700), (28, 140, 300), (29, 140, 300),  # full tiles
+                                   (130, 4300, 8300), (20, 18950, 300)])  # pairs, more than 32 blocks of K
+def test_linear_of_wide_rows_at_the_edges_of_tiles(cuda, m, n, k, dtype, shift):
+    for share in (1, 0.03):
+        x, w, values = rows_and_weight(m, n, k, dtype, shift, share, seed=m)
+        assert equal(mx.linear(x.to(cuda), w, dtype=FP32), x.double().numpy() @ values.T)
 
 
 @gpu

@@ -25,7 +25,7 @@
 // too short only counts, and its readers split the rows again (right for any rows, fast
 // for those that leave little: 16 x 4096 x 4096 bf16 takes 9.0 us for normal rows, 10.8 with
 // six channels and 12.3 with 24 a thousand times larger; 16 x 8192 x 8192 with a value
-// 2^20 times larger in every group 2.6 ms).
+// 2^20 times larger in every group 1.9 ms).
 // The few-row kernel takes its lists along with a stage and finds the weights in shared
 // memory.  The CTA-pair GEMM's spare warps gather them from L2, 32 bytes for half of
 // one (1024 x 8192 x 8192 with eight digits: 194 us became 258 in bf16, 755 in fp16), so
@@ -74,12 +74,6 @@ __device__ __forceinline__ bool is_large(float v) {
   return (__float_as_uint(v) & 0x7FFFFFFFu) >= 0x7E800000u;
 }
 
-// Packed E8M0 code of (row, group).
-__device__ __forceinline__ uint32_t packed_scale(const uint8_t* scales, int kblocks, long long row, int group) {
-  return scales[((row >> 7) * kblocks + (group >> 3)) * 1024 + ((group >> 2) & 1) * 512 + (row & 31) * 16 +
-                ((row & 127) >> 5) * 4 + (group & 3)];
-}
-
 // 16-bit rows [m][k], pitch ld elements; vec: every row starts on a 16-byte boundary.
 struct ValueRows {
   const uint16_t* x;
@@ -95,9 +89,6 @@ struct MxRows {
   const uint8_t* scales;
   int kblocks;
   long long n;
-  __device__ __forceinline__ float scale(long long row, int group) const {
-    return scale_value(packed_scale(scales, kblocks, row, group));
-  }
 };
 
 // The lane's eight of 256 values from k on, zeros past the end.
@@ -180,21 +171,20 @@ __device__ __forceinline__ int count_left(const float (&left)[8]) {
   return n;
 }
 
-// The sum of left . weight row n over K block kb, `left` being spread over the
-// warp's `lanes`.
-__device__ __forceinline__ float left_block(const float (&left)[8], uint32_t lanes, int kb, const MxRows& w,
-                                            long long n) {
+// The sum of left . a weight row (a row a lane) over a block of 256 values of K, `left`
+// being spread over the warp's `lanes`: codes(from) are the eight codes at lane from's
+// values, scale(group) their group's.
+template <typename Codes, typename Scale>
+__device__ __forceinline__ float left_block(const float (&left)[8], uint32_t lanes, Codes codes, Scale scale) {
   float sum = 0.0f;
-  while (lanes != 0) {
+  for (; lanes != 0; lanes &= lanes - 1) {
     const int from = __ffs(lanes) - 1;
-    lanes &= lanes - 1;
-    const bool in = n < w.n;
-    const uint32_t codes = in ? *reinterpret_cast<const uint32_t*>(w.codes + n * w.pitch + kb * 128ll + from * 4) : 0u;
-    const float scale = in ? w.scale(n, kb * 8 + from / 4) : 0.0f;
+    const uint32_t word = codes(from);
+    const float s = scale(from / 4);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float v = __shfl_sync(0xFFFFFFFFu, left[i], from);
-      if (v != 0.0f) sum += v * (decode1(codes >> (4 * i) & 15u) * scale);
+      if (v != 0.0f) sum += v * (decode1(word >> (4 * i) & 15u) * s);
     }
   }
   return sum;
@@ -242,17 +232,16 @@ __device__ __forceinline__ void append_left(LeftList* list, uint32_t at, uint32_
       list->entries[at++] = make_uint2(LeftEntry::of(token, lane * 8 + i).bits, __float_as_uint(left[i]));
 }
 
-// What the digits of a token leave in K block kb, split again, times weight row n (a
-// row a lane).
-template <int DIGITS>
-__device__ __forceinline__ float left_again(const ValueRows& rows, long long token, int kb, const MxRows& w,
-                                            long long n) {
+// What the digits of a token leave in K block kb, split again, times a weight row (a row
+// a lane; codes and scale as in left_block).
+template <int DIGITS, typename Codes, typename Scale>
+__device__ __forceinline__ float left_again(const ValueRows& rows, long long token, int kb, Codes codes, Scale scale) {
   const uint4 raw = load_values(rows, token, kb * 256 + (threadIdx.x & 31) * 8);
   float left[8];
   int e8;
   const bool any = split_digits<DIGITS>(raw, rows.bf16, left, e8, [](int, uint8_t, uint32_t) {});
   left_of<DIGITS>(raw, rows.bf16, left, e8);
-  return left_block(left, __ballot_sync(0xFFFFFFFFu, any), kb, w, n);
+  return left_block(left, __ballot_sync(0xFFFFFFFFu, any), codes, scale);
 }
 
 // acc[t] = the products of weight row n (a row a lane) with what the digits of token
@@ -313,9 +302,14 @@ __device__ __noinline__ bool left_products(const LeftList* lists, const ValueRow
         }
       }
     }
-    for (uint32_t full = __ballot_sync(0xFFFFFFFFu, count > kLeftEntries); full != 0; full &= full - 1)
+    for (uint32_t full = __ballot_sync(0xFFFFFFFFu, count > kLeftEntries); full != 0; full &= full - 1) {
+      const int kb = base + __ffs(full) - 1;
       for (int t = 0; t < Layout::kTokens && first + t < rows.m; ++t)
-        acc[t] += left_again<Layout::kDigits>(rows, first + t, base + __ffs(full) - 1, w, n);
+        acc[t] += left_again<Layout::kDigits>(
+            rows, first + t, kb,
+            [&](int from) { return *reinterpret_cast<const uint32_t*>(row + kb * 128ll + from * 4); },
+            [&](int group) { return scale_value(scales[kb * 1024ll + (group >> 2) * 512 + (group & 3)]); });
+    }
   }
   return any;
 }

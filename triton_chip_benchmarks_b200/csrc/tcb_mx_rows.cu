@@ -96,7 +96,6 @@ constexpr int rows_threads(int mode) { return (6 + (mode == kXInline ? kXWarps :
 struct RowsArgs {
   const uint8_t* sw;     // packed scales of W
   const uint8_t* sx;     // packed scales of X's rows or digits
-  const uint8_t* w;      // W's codes (products with what the digits leave)
   ValueRows x;           // 16-bit X
   const LeftList* lists; // what its digits leave
   const void* bias;
@@ -198,12 +197,20 @@ __global__ void __launch_bounds__(Layout::kTokens * 32)
   if (warp_total != 0) append_left(list, before, mine, static_cast<uint32_t>(warp), left);
 }
 
-// What a list that is too short counts, for one of its tokens: out of the way of the
-// stages' loop.
+// What a list that is too short counts, for one of its tokens, as add_listed; out of the
+// way of the stages' loop.
 template <typename Layout>
-__device__ __noinline__ float left_of_full_list(const RowsArgs& args, long long token, int kb, long long n) {
-  const MxRows w{args.w, args.pitch, args.sw, args.kblocks, args.n};
-  return token < args.x.m ? left_again<Layout::kDigits>(args.x, token, kb, w, n) : 0.0f;
+__device__ __noinline__ float left_of_full_list(const RowsArgs& args, long long token, int kb, const uint8_t* codes,
+                                                const uint8_t* scales, int row) {
+  if (token >= args.x.m) return 0.0f;
+  const uint8_t* mine = codes + row * kBlockBytes;
+  const uint8_t* scale = scales + (row & 31) * 16 + (row >> 5) * 4;
+  return left_again<Layout::kDigits>(
+      args.x, token, kb,
+      [&](int from) {
+        return *reinterpret_cast<const uint32_t*>(mine + ((from >> 2 ^ (row & 7)) << 4) + (from & 3) * 4);
+      },
+      [&](int group) { return scale_value(scale[(group >> 2) * 512 + (group & 3)]); });
 }
 
 // sums[t] += the weight row of this lane (row 0..127 of the tile) times what the lists of
@@ -467,8 +474,8 @@ __global__ void __launch_bounds__(rows_threads(XMODE), 2)
           for (; full != 0; full &= full - 1) {
             const int first = (__ffs(full) - 1) / 8 * Layout::kTokens;
             for (int t = first; t < first + Layout::kTokens; ++t)
-              left_sums[t] += left_of_full_list<Layout>(args, token0 + t, kb0 + it,
-                                                static_cast<long long>(tile) * kRowTile + row_of_lane);
+              left_sums[t] += left_of_full_list<Layout>(args, token0 + t, kb0 + it, smem + s * args.stage_bytes,
+                                                        sw - lane * 16, row_of_lane);
           }
           __syncwarp();
         }
@@ -743,7 +750,6 @@ int mx_rows_run(const RowsProblem& p, void* workspace, int* status, const Device
   RowsArgs args = {};
   args.sw = static_cast<const uint8_t*>(p.sw);
   args.sx = static_cast<const uint8_t*>(p.sx);
-  args.w = static_cast<const uint8_t*>(p.w);
   args.x = {static_cast<const uint16_t*>(p.x), p.ldx, p.m, p.k, p.x_type == kRowsBf16,
             aligned(p.x, 16) && (p.ldx % 8 == 0 || p.m == 1)};
   args.bias = p.bias;
