@@ -29,7 +29,7 @@
 // The few-row kernel takes its lists along with a stage and finds the weights in shared
 // memory.  The CTA-pair GEMM's spare warps gather them from L2, 32 bytes for half of
 // one (1024 x 8192 x 8192 with eight digits: 194 us became 258 in bf16, 755 in fp16), so
-// rows for it have nine digits (230, 250).
+// rows for it have nine digits (227, 238).
 #pragma once
 
 #include "tcb_mx.cuh"
@@ -246,69 +246,48 @@ __device__ __forceinline__ float left_again(const ValueRows& rows, long long tok
 
 // acc[t] = the products of weight row n (a row a lane) with what the digits of token
 // first + t, t < Layout::kTokens, leave; `lists` are that list's, a K block each.
-// Returns whether there is anything (acc is not written otherwise).
+// Returns whether there is anything (acc is not written otherwise).  One entry at a time:
+// there are few, and the code, which runs now and then, costs what fetching it takes
+// (64 x 16384 x 4096 bf16: 30.6 us so, 34.1 with eight weights in flight).
 template <typename Layout>
 __device__ __noinline__ bool left_products(const LeftList* lists, const ValueRows& rows, long long first,
                                            const MxRows& w, long long n, float* acc) {
-  constexpr int kBatch = 8;  // weights in flight
   const int lane = threadIdx.x & 31;
   const long long m = min(n, w.n - 1);  // rows past the end: any row
   const uint8_t* row = w.codes + m * w.pitch;
   const uint8_t* scales = w.scales + (m >> 7) * w.kblocks * 1024 + (m & 31) * 16 + ((m & 127) >> 5) * 4;
   bool any = false;
   for (int base = 0; base < w.kblocks; base += 32) {
-    const uint32_t count = base + lane < w.kblocks ? lists[base + lane].count : 0u;
-    if (!__any_sync(0xFFFFFFFFu, count != 0)) continue;
-    if (!any) {
+    // A list a lane: its count and first entry.
+    uint4 head = make_uint4(0, 0, 0, 0);
+    if (base + lane < w.kblocks) head = *reinterpret_cast<const uint4*>(lists + base + lane);
+    uint32_t some = __ballot_sync(0xFFFFFFFFu, head.x != 0);
+    if (some == 0) continue;
+    if (!any)
       for (int t = 0; t < Layout::kTokens; ++t) acc[t] = 0.0f;
-      any = true;
-    }
-    // The lists end to end, an entry a lane.
-    const uint32_t listed = count <= kLeftEntries ? count : 0u;
-    uint32_t end = listed;
-#pragma unroll
-    for (int step = 1; step < 32; step *= 2) {
-      const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, end, step);
-      if (lane >= step) end += before;
-    }
-    const int total = static_cast<int>(__shfl_sync(0xFFFFFFFFu, end, 31));
-    for (int from = 0; from < total; from += 32) {
-      const uint32_t e = static_cast<uint32_t>(from + lane);
-      int at = 0;  // the list that entry e lies in: as many end at or before it
-#pragma unroll
-      for (int step = 16; step > 0; step /= 2)
-        if (__shfl_sync(0xFFFFFFFFu, end, at + step - 1) <= e) at += step;
-      const uint32_t start = __shfl_sync(0xFFFFFFFFu, end - listed, at);
-      const bool own = e < static_cast<uint32_t>(total);
-      const uint2 entry = own ? lists[base + at].entries[e - start] : make_uint2(0, 0);
-      const int kb = own ? base + at : 0;
-      const int here = min(32, total - from);
-      for (int j = 0; j < here; j += kBatch) {
-        // Straight-line loads, whether there is an entry or not.
-        uint32_t codes[kBatch], scale[kBatch];
-        LeftEntry place[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          place[u].bits = __shfl_sync(0xFFFFFFFFu, entry.x, j + u);
-          const long long block = __shfl_sync(0xFFFFFFFFu, kb, j + u);
-          codes[u] = row[block * 128 + place[u].byte()];
-          scale[u] = scales[block * 1024 + place[u].scale()];
-        }
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-          const float v = __uint_as_float(__shfl_sync(0xFFFFFFFFu, entry.y, j + u));
-          const float term = v * (decode1(codes[u] >> place[u].shift() & 15u) * scale_value(scale[u]));
-          if (j + u < here) acc[place[u].token()] += term;
-        }
+    any = true;
+#pragma unroll 1
+    for (; some != 0; some &= some - 1) {
+      const int from = __ffs(some) - 1, kb = base + from;
+      const int count = static_cast<int>(__shfl_sync(0xFFFFFFFFu, head.x, from));
+      const uint8_t* codes = row + kb * 128ll;
+      const uint8_t* scale = scales + kb * 1024ll;
+      if (count > kLeftEntries) {
+        for (int t = 0; t < Layout::kTokens && first + t < rows.m; ++t)
+          acc[t] += left_again<Layout::kDigits>(
+              rows, first + t, kb, [&](int at) { return *reinterpret_cast<const uint32_t*>(codes + at * 4); },
+              [&](int group) { return scale_value(scale[(group >> 2) * 512 + (group & 3)]); });
+        continue;
       }
-    }
-    for (uint32_t full = __ballot_sync(0xFFFFFFFFu, count > kLeftEntries); full != 0; full &= full - 1) {
-      const int kb = base + __ffs(full) - 1;
-      for (int t = 0; t < Layout::kTokens && first + t < rows.m; ++t)
-        acc[t] += left_again<Layout::kDigits>(
-            rows, first + t, kb,
-            [&](int from) { return *reinterpret_cast<const uint32_t*>(row + kb * 128ll + from * 4); },
-            [&](int group) { return scale_value(scales[kb * 1024ll + (group >> 2) * 512 + (group & 3)]); });
+      uint2 entry = make_uint2(__shfl_sync(0xFFFFFFFFu, head.z, from), __shfl_sync(0xFFFFFFFFu, head.w, from));
+#pragma unroll 1
+      for (int e = 0;;) {
+        const LeftEntry at{entry.x};
+        acc[at.token()] += __uint_as_float(entry.y) *
+                           (decode1(codes[at.byte()] >> at.shift() & 15u) * scale_value(scale[at.scale()]));
+        if (++e >= count) break;
+        entry = lists[kb].entries[e];
+      }
     }
   }
   return any;

@@ -695,13 +695,18 @@ int run_16bit(const RowsProblem& p, RowsArgs args, const CUtensorMap& map_w, voi
   }
   uint8_t* base = static_cast<uint8_t*>(workspace);
   int rc;
-  // Column tiles while two of them fit an SM and all run at once.  Measured (us, column
-  // tiles / pairs, bf16 activations): 128 x 4096 x 4096 (256 tiles) 22.3/24.1, 48 x 12288 x
-  // 4096 (288) 20.9/25.1; 64 x 12288 x 4096 (384) 29.3/26.4, 33 x 16384 x 8192 (384)
-  // 45.0/36.7, 20 x 32768 x 4096 (512) 31.8/26.9.
+  // Column tiles while all of them run at once (two to an SM), unless there are more than
+  // SMs, three or more to a row tile (fewer stream the weight better) and the pairs' tiles
+  // are one round.  Measured (us, column tiles / pairs; tiles of either): 33 x 8192 x 4096
+  // bf16 (192, 64) 16.8/15.6, 96 x 4096 x 8192 bf16 (192, 64) 27.9/24.0, 64 x 4096 x 4096 fp16
+  // (160, 48) 16.5/17.2, 28 x 16384 x 4096 fp16 (256, 64; two to a row tile) 17.9/19.9, 128 x
+  // 4096 x 4096 bf16 (256, 80) 22.0/22.8, 48 x 12288 x 4096 bf16 (288, 96) 21.7/23.6, 64 x
+  // 12288 x 4096 bf16 (384, 144) 29.4/24.2, 64 x 16384 x 4096 bf16 (512, 192) 33.2/30.9.
   const long long row_tiles = (static_cast<long long>(p.n) + kRowTile - 1) / kRowTile;
   const long long col_tiles = (static_cast<long long>(p.m) + Layout::kTileTokens - 1) / Layout::kTileTokens;
-  if (col_tiles > 1 && col_tiles * row_tiles > 2ll * facts.sm_count) {
+  const long long pair_tiles = (row_tiles + 1) / 2 * ((SliceDigits::rows(p.m) + 255) / 256);
+  const bool one_round = col_tiles > 2 && pair_tiles <= facts.sm_count / 2;
+  if (col_tiles > 1 && col_tiles * row_tiles > (one_round ? 1 : 2) * static_cast<long long>(facts.sm_count)) {
     // Columns of the CTA-pair GEMM, whose M side is the weight.
     const DigitSpace space(SliceDigits{}, p.m, p.k);
     if ((rc = launch_digits<SliceDigits>(args, space, base, stream)) != TCB_OK) return rc;
